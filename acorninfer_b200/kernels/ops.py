@@ -140,6 +140,12 @@ class _Sigs:
     acorn_attention_plain = [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
                              c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int,
                              c_int, c_void_p, c_int, c_int, c_int, c_void_p, c_float, c_int, c_void_p]
+    acorn_qk_rope_kv_f8 = [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+                           c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                           c_float, c_float, c_void_p]
+    acorn_attention_f8_plain = [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
+                                c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int,
+                                c_void_p, c_void_p]
     acorn_scan_chunk = [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
                         c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p,
                         c_void_p]
@@ -621,6 +627,98 @@ def qk_rope_kv(qkv: torch.Tensor, q_weight32: torch.Tensor | None, k_weight32: t
         "qk_rope_kv")
 
 
+F8 = torch.float8_e4m3fn            # codes of the 8-bit cache
+F8_SCALE = torch.float8_e8m0fnu     # its powers of two, a byte each
+F8_MAX_HEAD = 256
+
+
+def _check_f8_pages(what: str, k_pages: torch.Tensor, v_pages: torch.Tensor, scales: torch.Tensor, num_kv_heads: int,
+                    head_dim: int) -> int:
+    """Checks the pages of an 8-bit cache and returns the page size."""
+    _check(k_pages, "k_pages", F8, 4)
+    _check(v_pages, "v_pages", F8, 4)
+    _check(scales, "scales", F8_SCALE, 4)
+    n, heads, P, d = k_pages.shape
+    if heads != num_kv_heads or d != head_dim or v_pages.shape != k_pages.shape or tuple(scales.shape) != (n, heads, P, 2):
+        raise KernelError(f"{what}: cache pages {tuple(k_pages.shape)} / {tuple(v_pages.shape)} / {tuple(scales.shape)} do not fit "
+                          f"nkv={num_kv_heads}, d={head_dim} (scales: [pages, nkv, page, 2])")
+    if P & (P - 1):
+        raise KernelError(f"{what}: the page size must be a power of two, got {P}")
+    if head_dim % 8 or not 8 <= head_dim <= F8_MAX_HEAD:
+        raise KernelError(f"{what}: head sizes are multiples of 8 up to {F8_MAX_HEAD}, got {head_dim}")
+    if k_pages.data_ptr() % 16 or v_pages.data_ptr() % 16 or scales.data_ptr() % 16:
+        raise KernelError(f"{what}: the cache pages must start on 16-byte boundaries")
+    return P
+
+
+def _stream_of(what: str, first: torch.Tensor, *others) -> int:
+    """The current stream's handle on the device of the given tensors, which must be one, and the current one."""
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise KernelError(f"{what}: tensors on {first.device} and {t.device}")
+    if first.device.index != torch.cuda.current_device():
+        raise KernelError(f"{what}: tensors on {first.device}, the current device is cuda:{torch.cuda.current_device()}")
+    return torch.cuda.current_stream().cuda_stream if _raw_stream is None else _raw_stream(first.device.index)
+
+
+def qk_rope_kv_f8(qkv: torch.Tensor, q_weight32: torch.Tensor | None, k_weight32: torch.Tensor | None, inv_freq: torch.Tensor,
+                  positions: torch.Tensor, token_row: torch.Tensor, block_table: torch.Tensor, page_base: torch.Tensor,
+                  k_pages: torch.Tensor, v_pages: torch.Tensor, scales: torch.Tensor, num_heads: int, num_kv_heads: int,
+                  head_dim: int, rotary_dim: int, interleaved: bool, eps: float, bias32: torch.Tensor | None = None,
+                  magnitude: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``qk_rope_kv`` into an 8-bit cache: per-head q/k norm, rotary encoding, keys and values quantised and written into
+    their pages.  Returns the queries (bfloat16 [T, nq d], or ``out``, whose rows may be wider); ``qkv`` (bfloat16, rows
+    ``[q | k | v]``, possibly wider) stays as it is.
+
+    A key or value row of ``head_dim`` entries becomes e4m3 codes and a power of two 2^e, ``row = code * 2^e``: e is the
+    smallest integer in -120..120 for which 448 * 2^e is not below the row's largest magnitude, a code the nearest e4m3
+    number (ties to even; at e = 120 codes end at 240, so that every row stands for finite numbers).  A row with an
+    infinity or a NaN is stored as zeros with the scale NaN.  ``k_pages`` / ``v_pages``: float8_e4m3fn [pages, nkv, page, d];
+    ``scales``: float8_e8m0fnu [pages, nkv, page, 2], a token's key scale and value scale.
+
+    ``bias32`` (float32, an entry per channel of a row) is added first; ``magnitude``: a factor on cos and sin.  Head sizes
+    are multiples of 8 up to 256; ``rotary_dim`` is a multiple of 16 (of 2 with ``interleaved`` pairs)."""
+    what = "qk_rope_kv_f8"
+    _check(qkv, "qkv", torch.bfloat16, 2)
+    P = _check_f8_pages(what, k_pages, v_pages, scales, num_kv_heads, head_dim)
+    T, channels = qkv.shape[0], (num_heads + 2 * num_kv_heads) * head_dim
+    if num_heads < 1 or num_kv_heads < 1 or qkv.shape[1] < channels or qkv.shape[1] % 8 or qkv.data_ptr() % 16:
+        raise KernelError(f"{what}: rows of {qkv.shape[1]} for {channels} channels (a multiple of 8, on 16-byte boundaries)")
+    if not 0 <= rotary_dim <= head_dim or rotary_dim % (2 if interleaved else 16):
+        raise KernelError(f"{what}: rotary_dim {rotary_dim} must be at most head_dim and a multiple of "
+                          f"{2 if interleaved else 16}")
+    _check(inv_freq, "inv_freq", torch.float32, 1)
+    if inv_freq.numel() != rotary_dim // 2:
+        raise KernelError("inv_freq must have rotary_dim / 2 entries")
+    for t, n in ((positions, "positions"), (token_row, "token_row"), (page_base, "page_base")):
+        _check(t, n, torch.int32, 1)
+    _check(block_table, "block_table", torch.int32, 2)
+    if positions.numel() < T or token_row.numel() < T or page_base.numel() < block_table.shape[0]:
+        raise KernelError(f"{what}: positions and token_row need an entry per token, page_base one per row")
+    for w, n in ((q_weight32, "q_norm weight"), (k_weight32, "k_norm weight")):
+        if w is not None:
+            _check(w, n, torch.float32, 1)
+            if w.numel() != head_dim:
+                raise KernelError(f"{n} must have head_dim entries")
+    if bias32 is not None:
+        _check(bias32, "bias", torch.float32, 1)
+        if bias32.numel() != channels:
+            raise KernelError(f"{what}: bias has {bias32.numel()} entries for {channels} channels")
+    if out is None:
+        out = torch.empty((T, num_heads * head_dim), dtype=qkv.dtype, device=qkv.device)
+    _check(out, "out", torch.bfloat16, 2)
+    if out.shape[0] != T or out.shape[1] < num_heads * head_dim or out.shape[1] % 8 or out.data_ptr() % 16:
+        raise KernelError(f"{what}: out {tuple(out.shape)} does not hold [{T}, {num_heads * head_dim}] in rows of a multiple of 8")
+    stream = _stream_of(what, qkv, q_weight32, k_weight32, inv_freq, positions, token_row, block_table, page_base, k_pages, v_pages,
+                        scales, bias32, out)
+    _ok(lib().acorn_qk_rope_kv_f8(qkv.data_ptr(), qkv.stride(0), _ptr(q_weight32), _ptr(k_weight32), _ptr(bias32),
+                                  inv_freq.data_ptr(), positions.data_ptr(), token_row.data_ptr(), block_table.data_ptr(),
+                                  page_base.data_ptr(), block_table.stride(0), k_pages.data_ptr(), v_pages.data_ptr(),
+                                  scales.data_ptr(), out.data_ptr(), out.stride(0), T, num_heads, num_kv_heads, head_dim,
+                                  rotary_dim, 1 if interleaved else 0, P, float(eps), float(magnitude), stream), what)
+    return out
+
+
 def qk_row_norm(proj: torch.Tensor, q_weight32: torch.Tensor | None, k_weight32: torch.Tensor | None, cos_sin: torch.Tensor | None,
                 positions: torch.Tensor, token_row: torch.Tensor, block_table: torch.Tensor, page_base: torch.Tensor,
                 k_pages: torch.Tensor, v_pages: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int, value_dim: int,
@@ -981,6 +1079,91 @@ def attention_prefill_tc(q: torch.Tensor, q_stride: int, k_pages: torch.Tensor, 
                                          float(softcap or 0.0), _stream()),
         "attention_prefill_tc")
     return out
+
+
+F8_PREFILL_TILE = 128       # query tokens of a tile of ``attention_prefill_f8``
+
+
+def f8_tile_tokens(num_heads: int, num_kv_heads: int) -> int:
+    """Query tokens of a tile of ``attention_decode_f8``: as many as fit 16 rows of (token, query head of a group)."""
+    return max(1, 16 // (num_heads // num_kv_heads))
+
+
+def _check_f8_attention(what: str, q, q_stride, k_pages, v_pages, scales, block_table, page_base, row_start, row_pos, tiles, num_tokens,
+                        num_heads, num_kv_heads, head_dim, window, out, chunk, keep_first, sink32):
+    """Checks the arguments that the attention kernels over an 8-bit cache share; returns (page size, out, stream)."""
+    if q.dtype != torch.bfloat16 or not q.is_cuda or q.stride(-1) != 1:
+        raise KernelError(f"{what} takes bfloat16 queries on the device, rows of neighbouring entries")
+    if num_kv_heads < 1 or num_heads < 1 or num_heads % num_kv_heads:
+        raise KernelError("num_heads must be a multiple of num_kv_heads")
+    P = _check_f8_pages(what, k_pages, v_pages, scales, num_kv_heads, head_dim)
+    width = num_heads * head_dim
+    if q_stride < width or q_stride % 8 or q.data_ptr() % 16 or (num_tokens > 0 and q.untyped_storage().nbytes() // 2 <
+                                                                 q.storage_offset() + (num_tokens - 1) * q_stride + width):
+        raise KernelError(f"{what}: q must hold {num_tokens} rows of {width} entries, a multiple of 8 entries apart, from a 16-byte "
+                          "boundary on")
+    for t, n in ((page_base, "page_base"), (row_start, "row_start"), (row_pos, "row_pos")):
+        _check(t, n, torch.int32, 1)
+    _check(block_table, "block_table", torch.int32, 2)
+    _check(tiles, "tiles", torch.int32, 2)
+    rows = block_table.shape[0]
+    if page_base.numel() < rows or row_pos.numel() < rows or row_start.numel() < rows + 1 or tiles.shape[1] != 2:
+        raise KernelError(f"{what}: page_base and row_pos need an entry per row, row_start one more, tiles two columns")
+    for v, n in ((window, "window"), (chunk, "chunk"), (keep_first, "keep_first")):
+        if v is not None and v < 0:
+            raise KernelError(f"{what}: {n} must not be negative, got {v}")
+    _check_sink(sink32, num_heads)
+    if out is None:
+        out = torch.empty((num_tokens, width), dtype=q.dtype, device=q.device)
+    _check(out, "out", torch.bfloat16, 2)
+    if out.shape[0] < num_tokens or out.shape[1] != width or out.data_ptr() % 16:
+        raise KernelError(f"{what}: out {tuple(out.shape)} does not hold [{num_tokens}, {width}]")
+    return P, out, _stream_of(what, q, k_pages, v_pages, scales, block_table, page_base, row_start, row_pos, tiles, out, sink32)
+
+
+def _attention_f8_plain(q, q_stride, out, k_pages, v_pages, scales, block_table, page_base, row_start, row_pos, tiles, tile_tokens,
+                        num_heads, num_kv_heads, head_dim, P, scale, window, chunk, keep_first, sink32, stream):
+    _ok(lib().acorn_attention_f8_plain(q.data_ptr(), q_stride, out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+                                       scales.data_ptr(), block_table.data_ptr(), page_base.data_ptr(), block_table.stride(0),
+                                       row_start.data_ptr(), row_pos.data_ptr(), tiles.data_ptr(), tiles.shape[0], tile_tokens,
+                                       num_heads, num_kv_heads, head_dim, P, float(scale), int(window or 0), int(chunk or 0),
+                                       int(keep_first or 0), _ptr(sink32), stream), "attention_f8_plain")
+    return out
+
+
+def attention_decode_f8(q: torch.Tensor, q_stride: int, k_pages: torch.Tensor, v_pages: torch.Tensor, scales: torch.Tensor,
+                        block_table: torch.Tensor, page_base: torch.Tensor, row_start: torch.Tensor, row_pos: torch.Tensor,
+                        tiles: torch.Tensor, num_tokens: int, num_heads: int, num_kv_heads: int, head_dim: int, scale: float,
+                        window: int | None, num_splits: int | None = None, out: torch.Tensor | None = None,
+                        chunk: int | None = None, keep_first: int = 0, sink32: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of single tokens, or of a few tokens a row, over the pages of an 8-bit cache (see ``qk_rope_kv_f8``), which
+    already hold the step's own keys and values; bfloat16 in and out, float32 sums.
+
+    ``tiles`` (int32 [n, 2]: row, first token within the row): a tile is up to ``f8_tile_tokens(nq, nkv)`` tokens of its row
+    from there on, which read the row's pages together.  Token i of row r is query ``row_start[r] + i`` at position
+    ``row_pos[r] + i`` and reads the keys up to its own.  ``out`` is [all tokens of the step, nq * d]; rows of tokens in no tile
+    are left as they are.  ``window`` / ``chunk`` / ``keep_first`` / ``sink32``: as for ``attention_plain``."""
+    what = "attention_decode_f8"
+    P, out, stream = _check_f8_attention(what, q, q_stride, k_pages, v_pages, scales, block_table, page_base, row_start, row_pos, tiles,
+                                         num_tokens, num_heads, num_kv_heads, head_dim, window, out, chunk, keep_first, sink32)
+    return _attention_f8_plain(q, q_stride, out, k_pages, v_pages, scales, block_table, page_base, row_start, row_pos, tiles,
+                               f8_tile_tokens(num_heads, num_kv_heads), num_heads, num_kv_heads, head_dim, P, scale, window, chunk,
+                               keep_first, sink32, stream)
+
+
+def attention_prefill_f8(q: torch.Tensor, q_stride: int, k_pages: torch.Tensor, v_pages: torch.Tensor, scales: torch.Tensor,
+                         block_table: torch.Tensor, page_base: torch.Tensor, row_start: torch.Tensor, row_pos: torch.Tensor,
+                         tiles: torch.Tensor, num_tokens: int, num_heads: int, num_kv_heads: int, head_dim: int, scale: float,
+                         window: int | None, out: torch.Tensor | None = None, chunk: int | None = None, keep_first: int = 0,
+                         sink32: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of prompts, or portions of them, over the pages of an 8-bit cache: as ``attention_decode_f8``, in tiles
+    of up to 128 tokens (``F8_PREFILL_TILE``).  CTAs start in the order of the list: give the tiles that read the most keys
+    first."""
+    what = "attention_prefill_f8"
+    P, out, stream = _check_f8_attention(what, q, q_stride, k_pages, v_pages, scales, block_table, page_base, row_start, row_pos, tiles,
+                                         num_tokens, num_heads, num_kv_heads, head_dim, window, out, chunk, keep_first, sink32)
+    return _attention_f8_plain(q, q_stride, out, k_pages, v_pages, scales, block_table, page_base, row_start, row_pos, tiles,
+                               F8_PREFILL_TILE, num_heads, num_kv_heads, head_dim, P, scale, window, chunk, keep_first, sink32, stream)
 
 
 def attention_tc_error() -> int:
