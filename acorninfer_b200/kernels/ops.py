@@ -78,7 +78,7 @@ def build_calls() -> None:
 
 _error_word: ctypes.c_int | None = None       # pinned host memory that kernels write when a bounded wait gives up
 _KERNEL_NAMES = {1: "gemm_tcgen05", 2: "attention_prefill_tc", 3: "attention_decode_tma", 4: "gemm_tcgen05_pair",
-                 5: "latent_prefill_tc", 6: "gemm_f32_tc", 9: "error-word self-test"}
+                 5: "latent_prefill_tc", 6: "gemm_f32_tc", 7: "attention_decode_f8", 9: "error-word self-test"}
 
 
 def _init_error_word(library) -> None:
@@ -89,7 +89,8 @@ def _init_error_word(library) -> None:
         raise KernelError(f"could not allocate the kernels' error word: CUDA error {code}")
     for setter in ("acorn_gemm_tc_set_error_word", "acorn_attention_tc_set_error_word",
                    "acorn_attention_decode_tma_set_error_word", "acorn_selftest_set_error_word",
-                   "acorn_gemm_tc_pair_set_error_word", "acorn_latent_prefill_tc_set_error_word", "acorn_gemm_f32_tc_set_error_word"):
+                   "acorn_gemm_tc_pair_set_error_word", "acorn_latent_prefill_tc_set_error_word", "acorn_gemm_f32_tc_set_error_word",
+                   "acorn_attention_decode_f8_set_error_word"):
         code = getattr(library, setter)(dev)
         if code != 0:
             raise KernelError(f"{setter}: CUDA error {code}")
@@ -103,7 +104,8 @@ def raise_on_kernel_error() -> None:
         return
     word = _error_word.value
     _error_word.value = 0
-    for getter in (gemm_tc_error, attention_tc_error, attention_decode_tma_error, gemm_tc_pair_error, latent_prefill_tc_error, gemm_f32_tc_error):   # clear the kernels' own flags
+    for getter in (gemm_tc_error, attention_tc_error, attention_decode_tma_error, gemm_tc_pair_error, latent_prefill_tc_error, gemm_f32_tc_error,
+                   attention_decode_f8_error):   # clear the kernels' own flags
         getter()
     raise KernelError(f"kernel {_KERNEL_NAMES.get(word // 100, word // 100)} gave up a bounded wait at point "
                       f"{word % 100}: the results of the step are not valid")
@@ -146,6 +148,13 @@ class _Sigs:
     acorn_attention_f8_plain = [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
                                 c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int,
                                 c_void_p, c_void_p]
+    acorn_attention_decode_f8 = [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p,
+                                 c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p, c_int,
+                                 c_void_p, c_void_p, c_void_p]
+    acorn_attention_decode_f8_supported = [c_int, c_int, c_int, c_int]
+    acorn_attention_decode_f8_merges = [c_int]
+    acorn_attention_decode_f8_error = []
+    acorn_attention_decode_f8_set_error_word = [c_void_p]
     acorn_scan_chunk = [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
                         c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p,
                         c_void_p]
@@ -1089,6 +1098,20 @@ def f8_tile_tokens(num_heads: int, num_kv_heads: int) -> int:
     return max(1, 16 // (num_heads // num_kv_heads))
 
 
+F8_MAX_SPLITS = 64
+
+
+@lru_cache(maxsize=4096)
+def decode_f8_splits(tiles: int, num_kv_heads: int, key_bound: int, head_dim: int, num_sms: int = 148) -> int:
+    """Splits of the key range for ``attention_decode_f8``."""
+    pairs = max(1, tiles * num_kv_heads)
+    best = 1
+    for s in (2, 3, 4, 5, 6, 7, 8, 16):
+        if pairs * s <= 2 * num_sms and key_bound >= 128 * s:
+            best = s
+    return best
+
+
 def _check_f8_attention(what: str, q, q_stride, k_pages, v_pages, scales, block_table, page_base, row_start, row_pos, tiles, num_tokens,
                         num_heads, num_kv_heads, head_dim, window, out, chunk, keep_first, sink32):
     """Checks the arguments that the attention kernels over an 8-bit cache share; returns (page size, out, stream)."""
@@ -1146,9 +1169,31 @@ def attention_decode_f8(q: torch.Tensor, q_stride: int, k_pages: torch.Tensor, v
     what = "attention_decode_f8"
     P, out, stream = _check_f8_attention(what, q, q_stride, k_pages, v_pages, scales, block_table, page_base, row_start, row_pos, tiles,
                                          num_tokens, num_heads, num_kv_heads, head_dim, window, out, chunk, keep_first, sink32)
-    return _attention_f8_plain(q, q_stride, out, k_pages, v_pages, scales, block_table, page_base, row_start, row_pos, tiles,
-                               f8_tile_tokens(num_heads, num_kv_heads), num_heads, num_kv_heads, head_dim, P, scale, window, chunk,
-                               keep_first, sink32, stream)
+    n = tiles.shape[0]
+    if n > 65535 or not lib().acorn_attention_decode_f8_supported(num_heads, num_kv_heads, head_dim, P):
+        return _attention_f8_plain(q, q_stride, out, k_pages, v_pages, scales, block_table, page_base, row_start, row_pos, tiles,
+                                   f8_tile_tokens(num_heads, num_kv_heads), num_heads, num_kv_heads, head_dim, P, scale, window, chunk,
+                                   keep_first, sink32, stream)
+    if num_splits is None:
+        spans = [v for v in (window, chunk) if v]
+        bound = block_table.shape[1] * P
+        num_splits = decode_f8_splits(n, num_kv_heads, min([bound] + [v + (keep_first or 0) for v in spans]), head_dim, device_sms(q.device))
+    if not 1 <= num_splits <= F8_MAX_SPLITS:
+        raise KernelError(f"{what}: num_splits must be in 1..{F8_MAX_SPLITS}, got {num_splits}")
+    part_o = part_lse = None
+    if n and not lib().acorn_attention_decode_f8_merges(num_splits):
+        part_o = torch.empty((n, num_kv_heads, num_splits, 16, head_dim), dtype=torch.float32, device=q.device)
+        part_lse = torch.empty((n, num_kv_heads, num_splits, 16), dtype=torch.float32, device=q.device)
+    _ok(lib().acorn_attention_decode_f8(q.data_ptr(), q_stride, out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+                                        scales.data_ptr(), k_pages.shape[0], block_table.data_ptr(), page_base.data_ptr(),
+                                        block_table.stride(0), row_start.data_ptr(), row_pos.data_ptr(), tiles.data_ptr(), n, num_heads,
+                                        num_kv_heads, head_dim, P, float(scale), int(window or 0), int(chunk or 0), int(keep_first or 0),
+                                        _ptr(sink32), num_splits, _ptr(part_o), _ptr(part_lse), stream), what)
+    return out
+
+
+def attention_decode_f8_error() -> int:
+    return int(lib().acorn_attention_decode_f8_error())
 
 
 def attention_prefill_f8(q: torch.Tensor, q_stride: int, k_pages: torch.Tensor, v_pages: torch.Tensor, scales: torch.Tensor,
