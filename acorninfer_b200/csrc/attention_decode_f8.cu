@@ -1,18 +1,22 @@
 // Attention of few tokens a row over the pages of the 8-bit cache (f8_cache.cuh), head sizes 64 and 128: split-K flash decoding.
 //
 // One CTA per (tile, kv head, split).  A tile is up to 16 / rep tokens of one row (rep = nq / nkv query heads share a kv head);
-// its (token, head) pairs are the 16 rows of an m16n8k16 tile, so the tokens of a tile read their row's pages together.
+// its (token, head) pairs are its query rows, so the tokens of a tile read their row's pages together.
 // A producer warp brings K and V codes by TMA (one box a page and head, swizzled) and their exponents by bulk copies into a ring of
-// stages of 64 keys; each of the four other warps takes 16 keys of a stage:
-//   S = Q K^T   codes become half-precision numbers by one conversion a pair (e4m3 is exact in it); the queries are
+// stages of 64 keys; each of the four other warps takes 16 keys of a stage through m16n8k16 products whose sixteen rows are the
+// keys (then the entries of the values) and whose eight columns are query rows; more than eight query rows are NH = 2 products on
+// the same operands:
+//   S' = K Q'   codes become half-precision numbers by one conversion a pair (e4m3 is exact in it); the queries are
 //               brought to half precision by a power of two per row (their largest entry to 2^14 .. 2^15, so that a bfloat16
 //               entry is exact unless it is 2^-28 of the largest), and both powers of two meet the score in float32.
-//   P = 2^(t + e_v - m)   t the score in units of log2, e_v the exponent of the key's value row, m the running maximum of t + e_v:
-//               the value's power of two rides in the exponent, so that a weight is at most 1 (2^8 before the reference moves) in
-//               half precision, with 11 bits where bfloat16 would keep 8, whatever the sizes of the value rows.
-//   O += P V    on value codes as half-precision numbers; the denominator sums 2^(t - m) in float32.
+//   P = 2^(t + e_v - m)   t the score in units of log2, e_v the exponent of the key's value row, m a reference near the largest
+//               t + e_v so far: the value's power of two rides in the exponent, so that a weight is at most 2^8 (the reference
+//               moves when it is outgrown by more) in half precision, with 11 bits where bfloat16 would keep 8, whatever the
+//               sizes of the value rows.  Against the reference the common step needs no maximum across lanes, only a vote.
+//   O' += V' P' on value codes as half-precision numbers (a weight's transpose within the warp is one movmatrix); the
+//               denominator sums 2^(t - m) in float32.
 // The layouts of the fragments are chosen so that a lane's codes are whole 16-byte pieces of rows: the order of the head's
-// entries in a product of K is free (Q is laid out the same way), and so is the order of the output's columns.
+// entries in a product over them is free (Q is laid out the same way), and so is the order of the output's rows.
 // Codes of keys that no query of the tile reads are replaced by zeros (a slot that was never written may hold anything).
 //
 // The warps are merged through shared memory, the splits of a (tile, kv head) by a thread-block cluster through
@@ -36,19 +40,19 @@ __device__ int g_attn_dec_f8_error = 0;
 
 struct DecodeF8Params {
     F8AttnParams a;
-    int tile_tokens, num_splits, cluster_merge;
+    int tile_tokens, num_splits, cluster_merge;     // tile_tokens: the most tokens a tile holds
     float* part_o;            // [n_tiles, nkv, splits, 16, D]  (more splits than a cluster merges)
     float* part_lse;          // [n_tiles, nkv, splits, 16]
 };
 
-template <int D> struct DecodeF8 {
+template <int D, int NH> struct DecodeF8 {
     static constexpr int STAGES = D == 128 ? 4 : 8;
     static constexpr int ROWS_BYTES = DF8_CHUNK * D;                  // the codes of a stage's keys (or values)
     static constexpr int STAGE_BYTES = 2 * ROWS_BYTES;
     static constexpr int SCALE_BYTES = 2 * DF8_CHUNK;
     static constexpr int RECV_ROW = D + 4;                            // floats a received partial row takes: the output, then its log-sum
     static constexpr int RING = STAGES * STAGE_BYTES;
-    static constexpr int MERGE = (2 * DF8_WARPS * 16 + DF8_WARPS * 16 * D) * 4;
+    static constexpr int MERGE = DF8_WARPS * 8 * NH * (2 + D) * 4;
     static constexpr int BARS = RING > MERGE ? RING : MERGE;          // offsets in shared memory
     static constexpr int SCALES = BARS + 2 * STAGES * 8;
     static constexpr int RECV = SCALES + STAGES * SCALE_BYTES;
@@ -87,13 +91,32 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                  :: "r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
-template <int D>
-__global__ void __launch_bounds__(DF8_THREADS) attention_decode_f8_kernel(const __grid_constant__ CUtensorMap map_k,
+// An 8 x 8 matrix of 16-bit elements across the warp (lane (g, i): row g, columns 2 i and 2 i + 1), transposed.
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+
+// max / sum over the eight lanes that share lane % 4
+__device__ __forceinline__ float column_max(float v) {
+    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+    return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+}
+__device__ __forceinline__ float column_sum(float v) {
+    v += __shfl_xor_sync(0xffffffffu, v, 4);
+    v += __shfl_xor_sync(0xffffffffu, v, 8);
+    return v + __shfl_xor_sync(0xffffffffu, v, 16);
+}
+
+template <int D, int NH>
+__global__ void __launch_bounds__(DF8_THREADS, NH == 1 ? 3 : 2) attention_decode_f8_kernel(const __grid_constant__ CUtensorMap map_k,
                                                                          const __grid_constant__ CUtensorMap map_v,
                                                                          const DecodeF8Params dp) {
-    using L = DecodeF8<D>;
-    constexpr int WORDS = D / 16;                              // 32-bit words of codes a lane holds of a key row; k-steps of a product
-    constexpr int NT = D / 8;                                  // column tiles of the output
+    using L = DecodeF8<D, NH>;
+    constexpr int WORDS = D / 16;                              // 32-bit words of codes a lane holds of a key row; k-steps of a product;
+                                                               // row tiles of the output
     extern __shared__ __align__(1024) uint8_t smem[];
     const F8AttnParams& p = dp.a;
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
@@ -130,8 +153,8 @@ __global__ void __launch_bounds__(DF8_THREADS) attention_decode_f8_kernel(const 
     const int c0 = min(n_chunks, split * per), c1 = min(n_chunks, c0 + per);
     auto key0_of = [&](int c) { return c < nkb ? c * DF8_CHUNK : base_key + (c - nkb) * DF8_CHUNK; };
 
-    float o[NT][4];
-    float m_ref[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+    float o[NH][WORDS][4];
+    float m_ref[NH][2], l_run[NH][2];
     const int g = lane >> 2, i = lane & 3;
 
     if (warp == DF8_WARPS) {
@@ -179,19 +202,18 @@ __global__ void __launch_bounds__(DF8_THREADS) attention_decode_f8_kernel(const 
         }
     } else {
         // ---------------------------------------------------------------- compute warps
-        // this lane's query entries: rows g and g + 8, entries i * D / 4 .. + D / 4 - 1 of the head
-        uint32_t qa[WORDS][4];
-        float back[2];                                            // what undoes the rows' powers of two
-        int qpos[2], first_seen[2];
+        // queries: this lane holds row g (of each half), entries i * D / 4 .. + D / 4 - 1 of the head, as the B operand
+        uint32_t qb[NH][WORDS][2];
+        float factor[NH][2];                                      // of query rows 2 i and 2 i + 1: the softmax scale, and what undoes
+                                                                  // the row's power of two
+        int qpos[NH][2], first_seen[NH][2];
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-            const int m = g + 8 * hh;
+        for (int h = 0; h < NH; ++h) {
+            const int m = 8 * h + g;
             const bool live = m < m_rows;
             const int j = live ? m / rep : 0;
-            qpos[hh] = pos0 + j;
-            first_seen[hh] = mask_lo(p.mask, qpos[hh]);
             const uint4* src = reinterpret_cast<const uint4*>(p.q + (int64_t)(tok0 + j) * p.q_stride +
-                                                              (int64_t)(kvh * rep + (m - j * rep)) * D + i * (D / 4));
+                                                              (int64_t)(kvh * rep + (live ? m - j * rep : 0)) * D + i * (D / 4));
             uint32_t w[2 * WORDS];
 #pragma unroll
             for (int k = 0; k < WORDS / 2; ++k) {
@@ -206,102 +228,118 @@ __global__ void __launch_bounds__(DF8_THREADS) attention_decode_f8_kernel(const 
             // 2^14 <= most * 2^up < 2^15; rows of zeros and of numbers that are none as they are
             const int ex = (int)(__float_as_uint(most) >> 23) - 127;
             const int up = most == 0.f || ex == 128 ? 0 : min(126, 14 - ex);
-            const float f = f8_pow2(up);
-            back[hh] = f8_pow2(-up);
+            const float f = f8_pow2(up), back = f8_pow2(-up);
 #pragma unroll
             for (int k = 0; k < WORDS; ++k)
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
-                    qa[k][hh + 2 * b] = pack_f16(__uint_as_float(w[2 * k + b] << 16) * f, __uint_as_float(w[2 * k + b] & 0xffff0000u) * f);
-        }
+                    qb[h][k][b] = pack_f16(__uint_as_float(w[2 * k + b] << 16) * f, __uint_as_float(w[2 * k + b] & 0xffff0000u) * f);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) { o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f; }
+            for (int b = 0; b < 2; ++b) {
+                factor[h][b] = __shfl_sync(0xffffffffu, back, 4 * (2 * i + b)) * p.scale_log2;
+                qpos[h][b] = pos0 + min((8 * h + 2 * i + b) / rep, max(n_q - 1, 0));
+                first_seen[h][b] = mask_lo(p.mask, qpos[h][b]);
+                m_ref[h][b] = -INFINITY;
+                l_run[h][b] = 0.f;
+            }
+#pragma unroll
+            for (int n = 0; n < WORDS; ++n) { o[h][n][0] = o[h][n][1] = o[h][n][2] = o[h][n][3] = 0.f; }
+        }
+        const int last_lo = mask_lo(p.mask, hi - 1);              // the last query's rule starts last
         bool good = true;
         for (int c = c0; c < c1; ++c) {
             const int n = c - c0, s = n % L::STAGES;
-            if (good && !mbar_wait(full0 + 8 * s, (n / L::STAGES) & 1)) {
+            if (!mbar_wait(full0 + 8 * s, (n / L::STAGES) & 1)) {
                 tc_fail(&g_attn_dec_f8_error, 2, ACORN_KERNEL_ATTN_DECODE_F8);
                 good = false;
             }
             good = __all_sync(0xffffffffu, good);
             if (!good) break;
             const int wkey0 = key0_of(c) + warp * 16;             // first key of this warp's 16
-            const int wlast = wkey0 + 15;
-            const bool any = wkey0 < hi && (wlast >= lo || wkey0 < p.mask.keep);
-            if (any) {
+            if (wkey0 < hi && (wkey0 + 15 >= lo || wkey0 < p.mask.keep)) {
                 const uint32_t kb = tc_smem(smem + s * L::STAGE_BYTES), vb = kb + L::ROWS_BYTES;
-                float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-                uint32_t kw[2][WORDS];
+                float sc[NH][4];
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                for (int h = 0; h < NH; ++h) { sc[h][0] = sc[h][1] = sc[h][2] = sc[h][3] = 0.f; }
+                uint32_t kw[2][WORDS];                            // codes of keys g and g + 8
+#pragma unroll
+                for (int r2 = 0; r2 < 2; ++r2)
 #pragma unroll
                     for (int q = 0; q < WORDS / 4; ++q) {
-                        const uint4 v = lds128(kb + L::at(warp * 16 + 8 * h + g, (WORDS / 4) * i + q));
-                        kw[h][4 * q] = v.x; kw[h][4 * q + 1] = v.y; kw[h][4 * q + 2] = v.z; kw[h][4 * q + 3] = v.w;
+                        const uint4 v = lds128(kb + L::at(warp * 16 + 8 * r2 + g, (WORDS / 4) * i + q));
+                        kw[r2][4 * q] = v.x; kw[r2][4 * q + 1] = v.y; kw[r2][4 * q + 2] = v.z; kw[r2][4 * q + 3] = v.w;
                     }
+                // exponents of keys g and g + 8: key byte, value byte
+                const uint8_t* sp = smem + L::SCALES + s * L::SCALE_BYTES + 2 * (warp * 16 + g);
+                const uint32_t sw[2] = {*reinterpret_cast<const uint16_t*>(sp), *reinterpret_cast<const uint16_t*>(sp + 16)};
 #pragma unroll
-                for (int k = 0; k < WORDS; ++k)
+                for (int k = 0; k < WORDS; ++k) {
+                    const uint32_t a[4] = {f8_to_f16x2((uint16_t)kw[0][k]), f8_to_f16x2((uint16_t)kw[1][k]),
+                                           f8_to_f16x2((uint16_t)(kw[0][k] >> 16)), f8_to_f16x2((uint16_t)(kw[1][k] >> 16))};
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        mma_f16_16816(sc[h], qa[k], f8_to_f16x2((uint16_t)kw[h][k]), f8_to_f16x2((uint16_t)(kw[h][k] >> 16)));
-                // exponents of this lane's keys (8 h + 2 i and the one after it): key byte, value byte, twice
-                uint32_t sw[2];
+                    for (int h = 0; h < NH; ++h) mma_f16_16816(sc[h], a, qb[h][k][0], qb[h][k][1]);
+                }
+                // all of the tile's queries see all 16 keys: no mask
+                const bool whole = wkey0 + 15 <= pos0 && wkey0 >= last_lo;
+                float ve[2], ks[2];
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    sw[h] = *reinterpret_cast<const uint32_t*>(smem + L::SCALES + s * L::SCALE_BYTES + 2 * (warp * 16 + 8 * h + 2 * i));
-                // all of the tile's queries see all 16 keys: no mask (the last query's rule starts last)
-                const bool whole = wlast <= pos0 && wkey0 >= mask_lo(p.mask, pos0 + n_q - 1);
-                float ve[2][2], mx[2] = {-INFINITY, -INFINITY};
+                for (int r2 = 0; r2 < 2; ++r2) {
+                    const uint32_t kbyte = sw[r2] & 255u, vbyte = sw[r2] >> 8;
+                    ks[r2] = vbyte == F8_NAN_BYTE ? f8_scale(vbyte) : f8_scale(kbyte);
+                    ve[r2] = (float)((int)vbyte - 127);
+                }
+                bool grew = false;
+                float mx[NH][2];
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                for (int h = 0; h < NH; ++h)
 #pragma unroll
                     for (int b = 0; b < 2; ++b) {
-                        const uint32_t kbyte = (sw[h] >> (16 * b)) & 255u, vbyte = (sw[h] >> (16 * b + 8)) & 255u;
-                        const float ks = p.scale_log2 * f8_scale(vbyte == F8_NAN_BYTE ? vbyte : kbyte);
-                        ve[h][b] = (float)((int)vbyte - 127);
 #pragma unroll
-                        for (int hh = 0; hh < 2; ++hh) {
-                            float t = sc[h][2 * hh + b] * back[hh] * ks;
+                        for (int r2 = 0; r2 < 2; ++r2) {
+                            float t = sc[h][2 * r2 + b] * factor[h][b] * ks[r2];
                             if (!whole) {
-                                const int key = wkey0 + 8 * h + 2 * i + b;
-                                if (!(key <= qpos[hh] && (key >= first_seen[hh] || key < p.mask.keep))) t = -INFINITY;
+                                const int key = wkey0 + 8 * r2 + g;
+                                if (!(key <= qpos[h][b] && (key >= first_seen[h][b] || key < p.mask.keep))) t = -INFINITY;
                             }
-                            sc[h][2 * hh + b] = t;
-                            mx[hh] = fmaxf(mx[hh], t + ve[h][b]);
+                            sc[h][2 * r2 + b] = t;
                         }
+                        mx[h][b] = fmaxf(sc[h][b] + ve[0], sc[h][2 + b] + ve[1]);
+                        grew = grew || mx[h][b] > m_ref[h][b] + DF8_GROW_LOG2;
                     }
-                bool grew = false;
-#pragma unroll
-                for (int hh = 0; hh < 2; ++hh) {
-                    mx[hh] = quad_max(mx[hh]);
-                    grew = grew || mx[hh] > m_ref[hh] + DF8_GROW_LOG2;
-                }
                 if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
-                    for (int hh = 0; hh < 2; ++hh) {
-                        if (mx[hh] > m_ref[hh] + DF8_GROW_LOG2) {
-                            const float corr = fast_exp2(m_ref[hh] - mx[hh]);          // from -inf: 0
-                            m_ref[hh] = mx[hh];
-                            l_run[hh] *= corr;
+                    for (int h = 0; h < NH; ++h)
 #pragma unroll
-                            for (int n2 = 0; n2 < NT; ++n2) { o[n2][2 * hh] *= corr; o[n2][2 * hh + 1] *= corr; }
+                        for (int b = 0; b < 2; ++b) {
+                            const float top = column_max(mx[h][b]);
+                            if (top > m_ref[h][b]) {
+                                const float corr = fast_exp2(m_ref[h][b] - top);          // from -inf: 0
+                                m_ref[h][b] = top;
+                                l_run[h][b] *= corr;
+#pragma unroll
+                                for (int n2 = 0; n2 < WORDS; ++n2) { o[h][n2][b] *= corr; o[h][n2][2 + b] *= corr; }
+                            }
+                        }
+                }
+                uint32_t pb[NH][2];                               // P as the B operand: query row g, keys 2 i.. and 8 + 2 i..
+#pragma unroll
+                for (int h = 0; h < NH; ++h) {
+                    float w[4];
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        const float neg = m_ref[h][b] == -INFINITY ? 0.f : -m_ref[h][b];
+#pragma unroll
+                        for (int r2 = 0; r2 < 2; ++r2) {
+                            const float a = sc[h][2 * r2 + b] + neg;
+                            l_run[h][b] += fast_exp2(a);
+                            w[2 * r2 + b] = fast_exp2(a + ve[r2]);
                         }
                     }
+                    pb[h][0] = movmatrix_trans(pack_f16(w[0], w[1]));
+                    pb[h][1] = movmatrix_trans(pack_f16(w[2], w[3]));
                 }
-                float neg[2];
-#pragma unroll
-                for (int hh = 0; hh < 2; ++hh) neg[hh] = m_ref[hh] == -INFINITY ? 0.f : -m_ref[hh];
-                uint32_t pa[4];                                   // P as the A operand: rows g, g + 8, keys 2 i.. and 8 + 2 i..
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int hh = 0; hh < 2; ++hh) {
-                        const float a = sc[h][2 * hh] + neg[hh], b = sc[h][2 * hh + 1] + neg[hh];
-                        l_run[hh] += fast_exp2(a) + fast_exp2(b);
-                        pa[2 * h + hh] = pack_f16(fast_exp2(a + ve[h][0]), fast_exp2(b + ve[h][1]));
-                    }
-                // value codes of keys 2 i, 2 i + 1, 8 + 2 i, 9 + 2 i: entries g * D / 8 .. of each
-                uint32_t vw[4][NT / 4];
+                // value codes of keys 2 i, 2 i + 1, 8 + 2 i, 9 + 2 i: entries g * D / 8 .. + D / 8 - 1 of each
+                uint32_t vw[4][WORDS / 2];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const int row = warp * 16 + 2 * i + (k & 1) + 8 * (k >> 1);
@@ -319,46 +357,50 @@ __global__ void __launch_bounds__(DF8_THREADS) attention_decode_f8_kernel(const 
                         const int key = wkey0 + 2 * i + (k & 1) + 8 * (k >> 1);
                         if (!(key < hi && (key >= lo || key < p.mask.keep))) {
 #pragma unroll
-                            for (int w = 0; w < NT / 4; ++w) vw[k][w] = 0u;
+                            for (int w = 0; w < WORDS / 2; ++w) vw[k][w] = 0u;
                         }
                     }
                 }
+                // row tile n: entries g * D / 8 + 2 n (rows g) and the one after it (rows g + 8)
 #pragma unroll
-                for (int w = 0; w < NT / 4; ++w) {
-                    const uint32_t a0 = __byte_perm(vw[0][w], vw[1][w], 0x5140), a1 = __byte_perm(vw[0][w], vw[1][w], 0x7362);
-                    const uint32_t b0 = __byte_perm(vw[2][w], vw[3][w], 0x5140), b1 = __byte_perm(vw[2][w], vw[3][w], 0x7362);
-                    mma_f16_16816(o[4 * w], pa, f8_to_f16x2((uint16_t)a0), f8_to_f16x2((uint16_t)b0));
-                    mma_f16_16816(o[4 * w + 1], pa, f8_to_f16x2((uint16_t)(a0 >> 16)), f8_to_f16x2((uint16_t)(b0 >> 16)));
-                    mma_f16_16816(o[4 * w + 2], pa, f8_to_f16x2((uint16_t)a1), f8_to_f16x2((uint16_t)b1));
-                    mma_f16_16816(o[4 * w + 3], pa, f8_to_f16x2((uint16_t)(a1 >> 16)), f8_to_f16x2((uint16_t)(b1 >> 16)));
-                }
+                for (int w = 0; w < WORDS / 2; ++w)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const uint32_t x = __byte_perm(vw[0][w], vw[1][w], half ? 0x7362 : 0x5140);
+                        const uint32_t y = __byte_perm(vw[2][w], vw[3][w], half ? 0x7362 : 0x5140);
+                        const uint32_t a[4] = {f8_to_f16x2((uint16_t)x), f8_to_f16x2((uint16_t)(x >> 16)), f8_to_f16x2((uint16_t)y),
+                                               f8_to_f16x2((uint16_t)(y >> 16))};
+#pragma unroll
+                        for (int h = 0; h < NH; ++h) mma_f16_16816(o[h][2 * w + half], a, pb[h][0], pb[h][1]);
+                    }
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(empty0 + 8 * s);
         }
-        l_run[0] = quad_sum(l_run[0]);
-        l_run[1] = quad_sum(l_run[1]);
+#pragma unroll
+        for (int h = 0; h < NH; ++h) { l_run[h][0] = column_sum(l_run[h][0]); l_run[h][1] = column_sum(l_run[h][1]); }
     }
     // every stage has been consumed (the compute warps waited for each); the ring is free for the merge
     __syncthreads();
-    float* sm_m = reinterpret_cast<float*>(smem);                 // [WARPS][16]
-    float* sm_l = sm_m + 16 * DF8_WARPS;
-    float* sm_o = sm_l + 16 * DF8_WARPS;                          // [WARPS][16][D]
+    constexpr int ROWS = 8 * NH;
+    float* sm_m = reinterpret_cast<float*>(smem);                 // [WARPS][ROWS]
+    float* sm_l = sm_m + ROWS * DF8_WARPS;
+    float* sm_o = sm_l + ROWS * DF8_WARPS;                        // [WARPS][ROWS][D]
     if (warp < DF8_WARPS) {
-        if (i == 0) {
-            sm_m[warp * 16 + g] = m_ref[0];
-            sm_m[warp * 16 + g + 8] = m_ref[1];
-            sm_l[warp * 16 + g] = l_run[0];
-            sm_l[warp * 16 + g + 8] = l_run[1];
-        }
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh)
+        for (int h = 0; h < NH; ++h)
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
+            for (int b = 0; b < 2; ++b) {
+                const int m = warp * ROWS + 8 * h + 2 * i + b;
+                if (g == 0) {
+                    sm_m[m] = m_ref[h][b];
+                    sm_l[m] = l_run[h][b];
+                }
 #pragma unroll
-                for (int n = 0; n < NT; n += 4)
-                    *reinterpret_cast<float4*>(sm_o + (warp * 16 + g + 8 * hh) * D + (2 * i + b) * NT + n) =
-                        make_float4(o[n][2 * hh + b], o[n + 1][2 * hh + b], o[n + 2][2 * hh + b], o[n + 3][2 * hh + b]);
+                for (int n = 0; n < WORDS; n += 2)
+                    *reinterpret_cast<float4*>(sm_o + m * D + g * (D / 8) + 2 * n) =
+                        make_float4(o[h][n][b], o[h][n][2 + b], o[h][n + 1][b], o[h][n + 1][2 + b]);
+            }
     }
     __syncthreads();
     // received partial rows: recv[rank of the sender][slot][RECV_ROW]
@@ -372,15 +414,15 @@ __global__ void __launch_bounds__(DF8_THREADS) attention_decode_f8_kernel(const 
         const float sink = p.sink && split == 0 ? p.sink[head] * 1.4426950408889634f : -INFINITY;
         float mstar = sink;
 #pragma unroll
-        for (int w = 0; w < DF8_WARPS; ++w) mstar = fmaxf(mstar, sm_m[w * 16 + m]);
+        for (int w = 0; w < DF8_WARPS; ++w) mstar = fmaxf(mstar, sm_m[w * ROWS + m]);
         float sum = sink == -INFINITY ? 0.f : exp2f(sink - mstar), acc = 0.f;
 #pragma unroll
         for (int w = 0; w < DF8_WARPS; ++w) {
             // a warp without keys has maximum -inf and sum 0; one whose keys are all NaN a sum that is NaN
-            const float mw = sm_m[w * 16 + m], lw = sm_l[w * 16 + m];
+            const float mw = sm_m[w * ROWS + m], lw = sm_l[w * ROWS + m];
             const float f = mw == -INFINITY ? 0.f : exp2f(mw - mstar);
             sum += f * lw;
-            acc += f * sm_o[(w * 16 + m) * D + e];
+            acc += f * sm_o[(w * ROWS + m) * D + e];
         }
         const bool empty = mstar == -INFINITY && sum == 0.f;      // no key of this split is seen by the query
         if (dp.num_splits == 1) {
@@ -461,9 +503,9 @@ static int make_map_codes(CUtensorMap* map, const void* base, int64_t rows, int 
     return r == CUDA_SUCCESS ? 0 : 20000 + (int)r;
 }
 
-template <int D>
+template <int D, int NH>
 static int launch_decode_f8(const DecodeF8Params& dp, int64_t num_pages, int n_tiles, cudaStream_t stream) {
-    using L = DecodeF8<D>;
+    using L = DecodeF8<D, NH>;
     const F8AttnParams& p = dp.a;
     CUtensorMap mk, mv;
     const int P = 1 << p.logP, box_rows = P < DF8_CHUNK ? P : DF8_CHUNK;
@@ -476,9 +518,9 @@ static int launch_decode_f8(const DecodeF8Params& dp, int64_t num_pages, int n_t
     const size_t smem = L::RECV + recv, smem_max = L::RECV + (size_t)32 * L::RECV_ROW * 4;
     static AcornPerDevice configured;
     if (!configured.seen()) {
-        cudaError_t e = cudaFuncSetAttribute(attention_decode_f8_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_max);
+        cudaError_t e = cudaFuncSetAttribute(attention_decode_f8_kernel<D, NH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_max);
         if (e != cudaSuccess) return (int)e;
-        e = cudaFuncSetAttribute(attention_decode_f8_kernel<D>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        e = cudaFuncSetAttribute(attention_decode_f8_kernel<D, NH>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return (int)e;
         configured.mark();
     }
@@ -496,7 +538,7 @@ static int launch_decode_f8(const DecodeF8Params& dp, int64_t num_pages, int n_t
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = acorn_pdl_enabled() ? 2 : 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, attention_decode_f8_kernel<D>, mk, mv, dp);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, attention_decode_f8_kernel<D, NH>, mk, mv, dp);
     if (e == cudaSuccess) e = cudaGetLastError();
     if (e != cudaSuccess || dp.num_splits == 1 || dp.cluster_merge) return (int)e;
     return acorn_launch(attention_decode_f8_merge_kernel<D>, dim3(p.nkv, rows, n_tiles), dim3(D), 0, stream, dp);
@@ -506,9 +548,11 @@ extern "C" int acorn_attention_decode_f8(const void* q, int64_t q_stride, void* 
                                          const void* scales, int64_t num_pages, const int* block_table, const int* page_base,
                                          int table_stride, const int* row_start, const int* row_pos, const int* tiles, int n_tiles,
                                          int nq, int nkv, int d, int P, float scale, int window, int chunk, int keep,
-                                         const float* sink, int num_splits, float* part_o, float* part_lse, cudaStream_t stream) {
+                                         const float* sink, int tile_tokens, int num_splits, float* part_o, float* part_lse,
+                                         cudaStream_t stream) {
     if (n_tiles <= 0) return 0;
-    if (!acorn_attention_decode_f8_supported(nq, nkv, d, P) || n_tiles > 65535 || num_splits < 1 || num_splits > 65535 || q_stride % 8)
+    if (!acorn_attention_decode_f8_supported(nq, nkv, d, P) || n_tiles > 65535 || num_splits < 1 || num_splits > 65535 || q_stride % 8 ||
+        tile_tokens < 1 || tile_tokens > 16 / (nq / nkv))
         return ACORN_ERR_UNSUPPORTED;
     DecodeF8Params dp;
     F8AttnParams& p = dp.a;
@@ -517,12 +561,15 @@ extern "C" int acorn_attention_decode_f8(const void* q, int64_t q_stride, void* 
     p.row_start = row_start; p.row_pos = row_pos; p.tiles = tiles; p.sink = sink; p.table_stride = table_stride;
     p.nq = nq; p.nkv = nkv; p.mask = {window, chunk, keep}; p.scale_log2 = scale * 1.4426950408889634f;
     p.logP = acorn_log2_exact_tc(P);
-    dp.tile_tokens = 16 / (nq / nkv);
+    dp.tile_tokens = tile_tokens;
     dp.num_splits = num_splits;
     dp.cluster_merge = num_splits > 1 && acorn_attention_decode_f8_merges(num_splits);
     dp.part_o = part_o; dp.part_lse = part_lse;
     if (num_splits > 1 && !dp.cluster_merge && (part_o == nullptr || part_lse == nullptr)) return ACORN_ERR_UNSUPPORTED;
-    return d == 128 ? launch_decode_f8<128>(dp, num_pages, n_tiles, stream) : launch_decode_f8<64>(dp, num_pages, n_tiles, stream);
+    const bool one = tile_tokens * (nq / nkv) <= 8;
+    if (d == 128)
+        return one ? launch_decode_f8<128, 1>(dp, num_pages, n_tiles, stream) : launch_decode_f8<128, 2>(dp, num_pages, n_tiles, stream);
+    return one ? launch_decode_f8<64, 1>(dp, num_pages, n_tiles, stream) : launch_decode_f8<64, 2>(dp, num_pages, n_tiles, stream);
 }
 
 extern "C" int acorn_attention_decode_f8_error() {

@@ -150,7 +150,7 @@ class _Sigs:
                                 c_void_p, c_void_p]
     acorn_attention_decode_f8 = [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p,
                                  c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p, c_int,
-                                 c_void_p, c_void_p, c_void_p]
+                                 c_int, c_void_p, c_void_p, c_void_p]
     acorn_attention_decode_f8_supported = [c_int, c_int, c_int, c_int]
     acorn_attention_decode_f8_merges = [c_int]
     acorn_attention_decode_f8_error = []
@@ -1158,21 +1158,28 @@ def attention_decode_f8(q: torch.Tensor, q_stride: int, k_pages: torch.Tensor, v
                         block_table: torch.Tensor, page_base: torch.Tensor, row_start: torch.Tensor, row_pos: torch.Tensor,
                         tiles: torch.Tensor, num_tokens: int, num_heads: int, num_kv_heads: int, head_dim: int, scale: float,
                         window: int | None, num_splits: int | None = None, out: torch.Tensor | None = None,
-                        chunk: int | None = None, keep_first: int = 0, sink32: torch.Tensor | None = None) -> torch.Tensor:
+                        chunk: int | None = None, keep_first: int = 0, sink32: torch.Tensor | None = None,
+                        tile_tokens: int | None = None) -> torch.Tensor:
     """Attention of single tokens, or of a few tokens a row, over the pages of an 8-bit cache (see ``qk_rope_kv_f8``), which
     already hold the step's own keys and values; bfloat16 in and out, float32 sums.
 
     ``tiles`` (int32 [n, 2]: row, first token within the row): a tile is up to ``f8_tile_tokens(nq, nkv)`` tokens of its row
     from there on, which read the row's pages together.  Token i of row r is query ``row_start[r] + i`` at position
     ``row_pos[r] + i`` and reads the keys up to its own.  ``out`` is [all tokens of the step, nq * d]; rows of tokens in no tile
-    are left as they are.  ``window`` / ``chunk`` / ``keep_first`` / ``sink32``: as for ``attention_plain``."""
+    are left as they are.  No token is in two tiles, and no tile is empty.  ``tile_tokens``: the most tokens a tile holds, where
+    that is less than ``f8_tile_tokens`` (tiles of single tokens among longer rows).  ``num_splits``: into how many parts a row's
+    keys are cut (None: by a rule).  ``window`` / ``chunk`` / ``keep_first`` / ``sink32``: as for ``attention_plain``."""
     what = "attention_decode_f8"
     P, out, stream = _check_f8_attention(what, q, q_stride, k_pages, v_pages, scales, block_table, page_base, row_start, row_pos, tiles,
                                          num_tokens, num_heads, num_kv_heads, head_dim, window, out, chunk, keep_first, sink32)
-    n = tiles.shape[0]
+    n, most = tiles.shape[0], f8_tile_tokens(num_heads, num_kv_heads)
+    if tile_tokens is None:
+        tile_tokens = 1 if n == num_tokens else most              # as many tiles as tokens: one token in each
+    if not 1 <= tile_tokens <= most:
+        raise KernelError(f"{what}: tile_tokens must be in 1..{most}, got {tile_tokens}")
     if n > 65535 or not lib().acorn_attention_decode_f8_supported(num_heads, num_kv_heads, head_dim, P):
         return _attention_f8_plain(q, q_stride, out, k_pages, v_pages, scales, block_table, page_base, row_start, row_pos, tiles,
-                                   f8_tile_tokens(num_heads, num_kv_heads), num_heads, num_kv_heads, head_dim, P, scale, window, chunk,
+                                   tile_tokens, num_heads, num_kv_heads, head_dim, P, scale, window, chunk,
                                    keep_first, sink32, stream)
     if num_splits is None:
         spans = [v for v in (window, chunk) if v]
@@ -1188,7 +1195,7 @@ def attention_decode_f8(q: torch.Tensor, q_stride: int, k_pages: torch.Tensor, v
                                         scales.data_ptr(), k_pages.shape[0], block_table.data_ptr(), page_base.data_ptr(),
                                         block_table.stride(0), row_start.data_ptr(), row_pos.data_ptr(), tiles.data_ptr(), n, num_heads,
                                         num_kv_heads, head_dim, P, float(scale), int(window or 0), int(chunk or 0), int(keep_first or 0),
-                                        _ptr(sink32), num_splits, _ptr(part_o), _ptr(part_lse), stream), what)
+                                        _ptr(sink32), tile_tokens, num_splits, _ptr(part_o), _ptr(part_lse), stream), what)
     return out
 
 
