@@ -2,8 +2,9 @@
 //
 // One CTA per (tile, kv head, split).  A tile is up to 16 / rep tokens of one row (rep = nq / nkv query heads share a kv head);
 // its (token, head) pairs are its query rows, so the tokens of a tile read their row's pages together.
-// A producer warp brings K and V codes by TMA (one box a page and head, swizzled) and their exponents by bulk copies into a ring of
-// stages of 64 keys; each of the four other warps takes 16 keys of a stage through m16n8k16 products whose sixteen rows are the
+// A producer warp brings the codes by TMA (swizzled; a box is the keys and the values of one page and head, through a map whose
+// third dimension is the distance between the two page tensors) and their exponents by asynchronous copies into a ring of
+// stages of 64 keys: an issued copy costs the warp some 130 clocks, which is what bounds a CTA at small pages.  Each of the four other warps takes 16 keys of a stage through m16n8k16 products whose sixteen rows are the
 // keys (then the entries of the values) and whose eight columns are query rows; more than eight query rows are NH = 2 products on
 // the same operands:
 //   S' = K Q'   codes become half-precision numbers by one conversion a pair (e4m3 is exact in it); the queries are
@@ -41,6 +42,7 @@ __device__ int g_attn_dec_f8_error = 0;
 struct DecodeF8Params {
     F8AttnParams a;
     int tile_tokens, num_splits, cluster_merge;     // tile_tokens: the most tokens a tile holds
+    int joint, v_first;       // one box brings keys and values (the tensor at the lower address first), else two do
     float* part_o;            // [n_tiles, nkv, splits, 16, D]  (more splits than a cluster merges)
     float* part_lse;          // [n_tiles, nkv, splits, 16]
 };
@@ -56,14 +58,18 @@ template <int D, int NH> struct DecodeF8 {
     static constexpr int BARS = RING > MERGE ? RING : MERGE;          // offsets in shared memory
     static constexpr int SCALES = BARS + 2 * STAGES * 8;
     static constexpr int RECV = SCALES + STAGES * SCALE_BYTES;
-    // byte offset of the 16-byte piece `seg` of row `key` in a stage's region, as the TMA's swizzle places it
-    static __device__ __forceinline__ uint32_t at(int key, int seg) {
-        return D == 128 ? (uint32_t)(key * 128 + ((seg ^ (key & 7)) << 4)) : (uint32_t)(key * 64 + ((seg ^ ((key >> 1) & 3)) << 4));
+    // byte offset of the 16-byte piece `seg` of row `row` of a stage (boxes of 2^log_box keys, then as many values), as the
+    // TMA's swizzle places it
+    static __device__ __forceinline__ uint32_t at(int row, int seg) {
+        return D == 128 ? (uint32_t)(row * 128 + ((seg ^ (row & 7)) << 4)) : (uint32_t)(row * 64 + ((seg ^ ((row >> 1) & 3)) << 4));
     }
+    // the row of key `key` of a stage (its value's: 2^log_box further)
+    static __device__ __forceinline__ int row_of(int key, int log_box) { return ((key >> log_box) << (log_box + 1)) + (key & ((1 << log_box) - 1)); }
 };
 
+// (not volatile: the compiler may move it among the conversions that feed it; two products on different sums are independent)
 __device__ __forceinline__ void mma_f16_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -74,21 +80,19 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-    return v;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t addr) {
-    uint2 v;
-    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
-    return v;
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
 }
 
-// Untiled bulk copy global -> shared (16-byte aligned, a multiple of 16 bytes).
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 :: "r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+// Four bytes global -> shared, and this thread's arrival at `bar` once its copies so far are there (the barrier's count has
+// room for it).
+__device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" :: "r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(bar) : "memory");
 }
 
 // An 8 x 8 matrix of 16-bit elements across the warp (lane (g, i): row g, columns 2 i and 2 i + 1), transposed.
@@ -127,7 +131,7 @@ __global__ void __launch_bounds__(DF8_THREADS, NH == 1 ? 3 : 2) attention_decode
         return;
     }
     if (threadIdx.x == 0) {
-        for (int s = 0; s < L::STAGES; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, DF8_WARPS); }
+        for (int s = 0; s < L::STAGES; ++s) { mbar_init(full0 + 8 * s, 33); mbar_init(empty0 + 8 * s, DF8_WARPS); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
@@ -156,47 +160,38 @@ __global__ void __launch_bounds__(DF8_THREADS, NH == 1 ? 3 : 2) attention_decode
     float o[NH][WORDS][4];
     float m_ref[NH][2], l_run[NH][2];
     const int g = lane >> 2, i = lane & 3;
+    const int log_box = min(p.logP, 6);
 
     if (warp == DF8_WARPS) {
         // ---------------------------------------------------------------- producer
-        // The whole warp: lane l looks up the cache rows of the l-th box (one page, or 64 keys of a larger one) of a batch of
-        // 32, a batch ahead of the loads; an elected lane issues the loads.
+        // The whole warp: lane l looks up the cache row of keys 2 l and 2 l + 1 of a chunk, a chunk ahead of the loads, and
+        // copies their exponents; an elected lane issues the boxes (one page, or 64 keys of a larger one).
         const int* table = p.block_table + (int64_t)r * p.table_stride - p.page_base[r];
-        const int P = 1 << p.logP;
-        const int rows_per_op = P < DF8_CHUNK ? P : DF8_CHUNK;
-        const int log_ops = 6 - (p.logP < 6 ? p.logP : 6);       // boxes a chunk: 64 / rows_per_op
-        const int n_ops = (c1 - c0) << log_ops;
-        const int first_key = p.page_base[r] << p.logP;
-        auto row_of = [&](int idx) -> int {
-            const int b = idx < n_ops ? idx : 0;
-            int key = key0_of(c0 + (b >> log_ops)) + (b & ((1 << log_ops) - 1)) * rows_per_op;
-            if (key >= hi) key = hi - 1 - ((hi - 1) & (rows_per_op - 1));        // masked later: any rows that exist
-            if (key < first_key) key = first_key;
-            const int page = table[key >> p.logP];
-            return ((page * p.nkv + kvh) << p.logP) + (key & (P - 1));
+        const int box = 1 << log_box, first_key = p.page_base[r] << p.logP;
+        auto row_at = [&](int c) -> int {
+            const int key = key0_of(c) + 2 * lane;
+            int b = key & ~(box - 1);
+            if (b >= hi) b = (hi - 1) & ~(box - 1);               // masked later: any box that exists
+            if (b < first_key) b = first_key;
+            const int page = table[b >> p.logP];
+            return ((page * p.nkv + kvh) << p.logP) + (b & ((1 << p.logP) - 1)) + (key & (box - 1));
         };
-        int rows_next = n_ops > 0 ? row_of(lane) : 0;
-        bool good = true;
-        for (int b0 = 0; b0 < n_ops && good; b0 += 32) {
-            const int rows_cur = rows_next;
-            if (b0 + 32 < n_ops) rows_next = row_of(b0 + 32 + lane);
-            const int n_here = min(32, n_ops - b0);
-            for (int l = 0; l < n_here; ++l) {
-                const int idx = b0 + l, n = idx >> log_ops, k = idx & ((1 << log_ops) - 1), s = n % L::STAGES;
-                if (k == 0) {                                     // first box of a chunk: its stage must be free
-                    const bool got = mbar_wait(empty0 + 8 * s, ((n / L::STAGES) & 1) ^ 1);
-                    if (!got && lane == 0) tc_fail(&g_attn_dec_f8_error, 1, ACORN_KERNEL_ATTN_DECODE_F8);
-                    good = __all_sync(0xffffffffu, got);
-                    if (!good) break;
-                    if (elect_one()) mbar_expect_tx(full0 + 8 * s, L::STAGE_BYTES + L::SCALE_BYTES);
-                }
-                const int row = __shfl_sync(0xffffffffu, rows_cur, l);
+        int row_next = c0 < c1 ? row_at(c0) : 0;
+        for (int c = c0; c < c1; ++c) {
+            const int row = row_next, n = c - c0, s = n % L::STAGES;
+            if (c + 1 < c1) row_next = row_at(c + 1);
+            const bool got = mbar_wait(empty0 + 8 * s, ((n / L::STAGES) & 1) ^ 1);
+            if (!got && lane == 0) tc_fail(&g_attn_dec_f8_error, 1, ACORN_KERNEL_ATTN_DECODE_F8);
+            if (!__all_sync(0xffffffffu, got)) break;
+            if (elect_one()) mbar_expect_tx(full0 + 8 * s, L::STAGE_BYTES);
+            cp_async_4(tc_smem(smem + L::SCALES + s * L::SCALE_BYTES) + 4 * lane, p.scales + 2 * (int64_t)row);
+            cp_async_arrive(full0 + 8 * s);
+            for (int k = 0; k < DF8_CHUNK; k += box) {
+                const int y = __shfl_sync(0xffffffffu, row, k >> 1);
                 if (elect_one()) {
-                    const uint32_t dst = tc_smem(smem + s * L::STAGE_BYTES) + (uint32_t)(k * rows_per_op) * D;
-                    tma_load_2d(dst, &map_k, full0 + 8 * s, 0, row);
-                    tma_load_2d(dst + L::ROWS_BYTES, &map_v, full0 + 8 * s, 0, row);
-                    bulk_load(tc_smem(smem + L::SCALES + s * L::SCALE_BYTES) + 2 * k * rows_per_op, p.scales + 2 * (int64_t)row,
-                              2 * rows_per_op, full0 + 8 * s);
+                    const uint32_t dst = tc_smem(smem + s * L::STAGE_BYTES) + (uint32_t)(2 * k * D);
+                    tma_load_3d(dst, &map_k, full0 + 8 * s, 0, y, 0);
+                    if (!dp.joint) tma_load_3d(dst + box * D, &map_v, full0 + 8 * s, 0, y, 0);
                 }
             }
         }
@@ -246,6 +241,16 @@ __global__ void __launch_bounds__(DF8_THREADS, NH == 1 ? 3 : 2) attention_decode
             for (int n = 0; n < WORDS; ++n) { o[h][n][0] = o[h][n][1] = o[h][n][2] = o[h][n][3] = 0.f; }
         }
         const int last_lo = mask_lo(p.mask, hi - 1);              // the last query's rule starts last
+        // this lane's pieces of a stage: keys g and g + 8, values of keys 2 i, 2 i + 1, 8 + 2 i, 9 + 2 i of the warp's 16
+        const int k_skip = dp.v_first ? 1 << log_box : 0, v_skip = (1 << log_box) - k_skip;
+        uint32_t k_at[2], v_at[4];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) k_at[k] = L::at(L::row_of(warp * 16 + 8 * k + g, log_box) + k_skip, (WORDS / 4) * i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int row = L::row_of(warp * 16 + 2 * i + (k & 1) + 8 * (k >> 1), log_box) + v_skip;
+            v_at[k] = D == 128 ? L::at(row, g) : L::at(row, g >> 1) + 8 * (g & 1);
+        }
         bool good = true;
         for (int c = c0; c < c1; ++c) {
             const int n = c - c0, s = n % L::STAGES;
@@ -257,16 +262,18 @@ __global__ void __launch_bounds__(DF8_THREADS, NH == 1 ? 3 : 2) attention_decode
             if (!good) break;
             const int wkey0 = key0_of(c) + warp * 16;             // first key of this warp's 16
             if (wkey0 < hi && (wkey0 + 15 >= lo || wkey0 < p.mask.keep)) {
-                const uint32_t kb = tc_smem(smem + s * L::STAGE_BYTES), vb = kb + L::ROWS_BYTES;
-                float sc[NH][4];
+                const uint8_t* stage = smem + s * L::STAGE_BYTES;
+                float sc[NH][4], sd[NH][4];                       // two chains of products
 #pragma unroll
-                for (int h = 0; h < NH; ++h) { sc[h][0] = sc[h][1] = sc[h][2] = sc[h][3] = 0.f; }
+                for (int h = 0; h < NH; ++h)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sc[h][e] = sd[h][e] = 0.f;
                 uint32_t kw[2][WORDS];                            // codes of keys g and g + 8
 #pragma unroll
                 for (int r2 = 0; r2 < 2; ++r2)
 #pragma unroll
                     for (int q = 0; q < WORDS / 4; ++q) {
-                        const uint4 v = lds128(kb + L::at(warp * 16 + 8 * r2 + g, (WORDS / 4) * i + q));
+                        const uint4 v = *reinterpret_cast<const uint4*>(stage + (k_at[r2] ^ (16 * q)));          // pieces 2 i and 2 i + 1 differ in one bit, swizzled or not
                         kw[r2][4 * q] = v.x; kw[r2][4 * q + 1] = v.y; kw[r2][4 * q + 2] = v.z; kw[r2][4 * q + 3] = v.w;
                     }
                 // exponents of keys g and g + 8: key byte, value byte
@@ -277,7 +284,7 @@ __global__ void __launch_bounds__(DF8_THREADS, NH == 1 ? 3 : 2) attention_decode
                     const uint32_t a[4] = {f8_to_f16x2((uint16_t)kw[0][k]), f8_to_f16x2((uint16_t)kw[1][k]),
                                            f8_to_f16x2((uint16_t)(kw[0][k] >> 16)), f8_to_f16x2((uint16_t)(kw[1][k] >> 16))};
 #pragma unroll
-                    for (int h = 0; h < NH; ++h) mma_f16_16816(sc[h], a, qb[h][k][0], qb[h][k][1]);
+                    for (int h = 0; h < NH; ++h) mma_f16_16816(k & 1 ? sd[h] : sc[h], a, qb[h][k][0], qb[h][k][1]);
                 }
                 // all of the tile's queries see all 16 keys: no mask
                 const bool whole = wkey0 + 15 <= pos0 && wkey0 >= last_lo;
@@ -296,7 +303,7 @@ __global__ void __launch_bounds__(DF8_THREADS, NH == 1 ? 3 : 2) attention_decode
                     for (int b = 0; b < 2; ++b) {
 #pragma unroll
                         for (int r2 = 0; r2 < 2; ++r2) {
-                            float t = sc[h][2 * r2 + b] * factor[h][b] * ks[r2];
+                            float t = (sc[h][2 * r2 + b] + sd[h][2 * r2 + b]) * factor[h][b] * ks[r2];
                             if (!whole) {
                                 const int key = wkey0 + 8 * r2 + g;
                                 if (!(key <= qpos[h][b] && (key >= first_seen[h][b] || key < p.mask.keep))) t = -INFINITY;
@@ -342,12 +349,11 @@ __global__ void __launch_bounds__(DF8_THREADS, NH == 1 ? 3 : 2) attention_decode
                 uint32_t vw[4][WORDS / 2];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const int row = warp * 16 + 2 * i + (k & 1) + 8 * (k >> 1);
                     if constexpr (D == 128) {
-                        const uint4 v = lds128(vb + L::at(row, g));
+                        const uint4 v = *reinterpret_cast<const uint4*>(stage + v_at[k]);
                         vw[k][0] = v.x; vw[k][1] = v.y; vw[k][2] = v.z; vw[k][3] = v.w;
                     } else {
-                        const uint2 v = lds64(vb + L::at(row, g >> 1) + 8 * (g & 1));
+                        const uint2 v = *reinterpret_cast<const uint2*>(stage + v_at[k]);
                         vw[k][0] = v.x; vw[k][1] = v.y;
                     }
                 }
@@ -489,29 +495,34 @@ extern "C" int acorn_attention_decode_f8_supported(int nq, int nkv, int d, int P
 // Whether this many splits are merged inside the kernel (by a cluster, without scratch).
 extern "C" int acorn_attention_decode_f8_merges(int num_splits) { return num_splits <= 8 || num_splits == DF8_CLUSTER_MAX; }
 
-// Codes [rows, D bytes], boxes of box_rows rows, swizzled over rows of D bytes.
-static int make_map_codes(CUtensorMap* map, const void* base, int64_t rows, int d, int box_rows) {
+// Codes [planes, rows, D bytes], boxes of box_rows rows of every plane, swizzled over rows of D bytes.
+static int make_map_codes(CUtensorMap* map, const void* base, int64_t rows, int planes, int64_t plane_bytes, int d, int box_rows) {
     EncodeTiledFn fn = encode_tiled_fn();
     if (fn == nullptr || rows > 0x7fffffff) return ACORN_ERR_UNSUPPORTED;
-    const cuuint64_t dims[2] = {(cuuint64_t)d, (cuuint64_t)rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)d};
-    const cuuint32_t box[2] = {(cuuint32_t)d, (cuuint32_t)box_rows};
-    const cuuint32_t elem[2] = {1, 1};
-    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem,
+    const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)rows, (cuuint64_t)planes};
+    const cuuint64_t strides[2] = {(cuuint64_t)d, (cuuint64_t)plane_bytes};
+    const cuuint32_t box[3] = {(cuuint32_t)d, (cuuint32_t)box_rows, (cuuint32_t)planes};
+    const cuuint32_t elem[3] = {1, 1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, elem,
                           CU_TENSOR_MAP_INTERLEAVE_NONE, d == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? 0 : 20000 + (int)r;
 }
 
 template <int D, int NH>
-static int launch_decode_f8(const DecodeF8Params& dp, int64_t num_pages, int n_tiles, cudaStream_t stream) {
+static int launch_decode_f8(DecodeF8Params dp, int64_t num_pages, int n_tiles, cudaStream_t stream) {
     using L = DecodeF8<D, NH>;
     const F8AttnParams& p = dp.a;
     CUtensorMap mk, mv;
     const int P = 1 << p.logP, box_rows = P < DF8_CHUNK ? P : DF8_CHUNK;
-    int rc = make_map_codes(&mk, p.k_pages, num_pages * p.nkv * P, D, box_rows);
+    // keys and values through one map whose planes are the two tensors, where their distance fits a map's stride
+    const int64_t rows_all = num_pages * p.nkv * P, apart = p.v_pages - p.k_pages, distance = apart < 0 ? -apart : apart;
+    dp.joint = distance > 0 && distance < (int64_t)1 << 40 && distance % 16 == 0;
+    dp.v_first = dp.joint && apart < 0;
+    int rc = make_map_codes(&mk, dp.v_first ? p.v_pages : p.k_pages, rows_all, dp.joint ? 2 : 1, dp.joint ? distance : rows_all * D, D,
+                            box_rows);
     if (rc) return rc;
-    rc = make_map_codes(&mv, p.v_pages, num_pages * p.nkv * P, D, box_rows);
+    rc = make_map_codes(&mv, p.v_pages, rows_all, 1, rows_all * D, D, box_rows);
     if (rc) return rc;
     const int rows = dp.tile_tokens * (p.nq / p.nkv);
     const size_t recv = dp.cluster_merge ? (size_t)dp.num_splits * ((rows + dp.num_splits - 1) / dp.num_splits) * L::RECV_ROW * 4 : 0;
