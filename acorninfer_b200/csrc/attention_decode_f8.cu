@@ -25,9 +25,8 @@
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
-#include "f8_cache.cuh"
+#include "f8_tma.cuh"
 #include "mma_helpers.cuh"
-#include "tcgen05_helpers.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -63,8 +62,6 @@ template <int D, int NH> struct DecodeF8 {
     static __device__ __forceinline__ uint32_t at(int row, int seg) {
         return D == 128 ? (uint32_t)(row * 128 + ((seg ^ (row & 7)) << 4)) : (uint32_t)(row * 64 + ((seg ^ ((row >> 1) & 3)) << 4));
     }
-    // the row of key `key` of a stage (its value's: 2^log_box further)
-    static __device__ __forceinline__ int row_of(int key, int log_box) { return ((key >> log_box) << (log_box + 1)) + (key & ((1 << log_box) - 1)); }
 };
 
 // (not volatile: the compiler may move it among the conversions that feed it; two products on different sums are independent)
@@ -78,21 +75,6 @@ __device__ __forceinline__ void mma_f16_16816(float (&c)[4], const uint32_t (&a)
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
-}
-
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-        :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
-}
-
-// Four bytes global -> shared, and this thread's arrival at `bar` once its copies so far are there (the barrier's count has
-// room for it).
-__device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" :: "r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(bar) : "memory");
 }
 
 // An 8 x 8 matrix of 16-bit elements across the warp (lane (g, i): row g, columns 2 i and 2 i + 1), transposed.
@@ -184,7 +166,7 @@ __global__ void __launch_bounds__(DF8_THREADS, NH == 1 ? 3 : 2) attention_decode
             if (!got && lane == 0) tc_fail(&g_attn_dec_f8_error, 1, ACORN_KERNEL_ATTN_DECODE_F8);
             if (!__all_sync(0xffffffffu, got)) break;
             if (elect_one()) mbar_expect_tx(full0 + 8 * s, L::STAGE_BYTES);
-            cp_async_4(tc_smem(smem + L::SCALES + s * L::SCALE_BYTES) + 4 * lane, p.scales + 2 * (int64_t)row);
+            cp_async_bytes<4>(tc_smem(smem + L::SCALES + s * L::SCALE_BYTES) + 4 * lane, p.scales + 2 * (int64_t)row);
             cp_async_arrive(full0 + 8 * s);
             for (int k = 0; k < DF8_CHUNK; k += box) {
                 const int y = __shfl_sync(0xffffffffu, row, k >> 1);
@@ -245,10 +227,10 @@ __global__ void __launch_bounds__(DF8_THREADS, NH == 1 ? 3 : 2) attention_decode
         const int k_skip = dp.v_first ? 1 << log_box : 0, v_skip = (1 << log_box) - k_skip;
         uint32_t k_at[2], v_at[4];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) k_at[k] = L::at(L::row_of(warp * 16 + 8 * k + g, log_box) + k_skip, (WORDS / 4) * i);
+        for (int k = 0; k < 2; ++k) k_at[k] = L::at(f8_stage_row(warp * 16 + 8 * k + g, log_box) + k_skip, (WORDS / 4) * i);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const int row = L::row_of(warp * 16 + 2 * i + (k & 1) + 8 * (k >> 1), log_box) + v_skip;
+            const int row = f8_stage_row(warp * 16 + 2 * i + (k & 1) + 8 * (k >> 1), log_box) + v_skip;
             v_at[k] = D == 128 ? L::at(row, g) : L::at(row, g >> 1) + 8 * (g & 1);
         }
         bool good = true;
@@ -495,34 +477,14 @@ extern "C" int acorn_attention_decode_f8_supported(int nq, int nkv, int d, int P
 // Whether this many splits are merged inside the kernel (by a cluster, without scratch).
 extern "C" int acorn_attention_decode_f8_merges(int num_splits) { return num_splits <= 8 || num_splits == DF8_CLUSTER_MAX; }
 
-// Codes [planes, rows, D bytes], boxes of box_rows rows of every plane, swizzled over rows of D bytes.
-static int make_map_codes(CUtensorMap* map, const void* base, int64_t rows, int planes, int64_t plane_bytes, int d, int box_rows) {
-    EncodeTiledFn fn = encode_tiled_fn();
-    if (fn == nullptr || rows > 0x7fffffff) return ACORN_ERR_UNSUPPORTED;
-    const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)rows, (cuuint64_t)planes};
-    const cuuint64_t strides[2] = {(cuuint64_t)d, (cuuint64_t)plane_bytes};
-    const cuuint32_t box[3] = {(cuuint32_t)d, (cuuint32_t)box_rows, (cuuint32_t)planes};
-    const cuuint32_t elem[3] = {1, 1, 1};
-    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, elem,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, d == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? 0 : 20000 + (int)r;
-}
-
 template <int D, int NH>
 static int launch_decode_f8(DecodeF8Params dp, int64_t num_pages, int n_tiles, cudaStream_t stream) {
     using L = DecodeF8<D, NH>;
     const F8AttnParams& p = dp.a;
     CUtensorMap mk, mv;
     const int P = 1 << p.logP, box_rows = P < DF8_CHUNK ? P : DF8_CHUNK;
-    // keys and values through one map whose planes are the two tensors, where their distance fits a map's stride
-    const int64_t rows_all = num_pages * p.nkv * P, apart = p.v_pages - p.k_pages, distance = apart < 0 ? -apart : apart;
-    dp.joint = distance > 0 && distance < (int64_t)1 << 40 && distance % 16 == 0;
-    dp.v_first = dp.joint && apart < 0;
-    int rc = make_map_codes(&mk, dp.v_first ? p.v_pages : p.k_pages, rows_all, dp.joint ? 2 : 1, dp.joint ? distance : rows_all * D, D,
-                            box_rows);
-    if (rc) return rc;
-    rc = make_map_codes(&mv, p.v_pages, rows_all, 1, rows_all * D, D, box_rows);
+    const int rc = make_code_maps(&mk, &mv, p, num_pages, D, box_rows,
+                                  D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, &dp.joint, &dp.v_first);
     if (rc) return rc;
     const int rows = dp.tile_tokens * (p.nq / p.nkv);
     const size_t recv = dp.cluster_merge ? (size_t)dp.num_splits * ((rows + dp.num_splits - 1) / dp.num_splits) * L::RECV_ROW * 4 : 0;

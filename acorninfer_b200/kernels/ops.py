@@ -78,7 +78,7 @@ def build_calls() -> None:
 
 _error_word: ctypes.c_int | None = None       # pinned host memory that kernels write when a bounded wait gives up
 _KERNEL_NAMES = {1: "gemm_tcgen05", 2: "attention_prefill_tc", 3: "attention_decode_tma", 4: "gemm_tcgen05_pair",
-                 5: "latent_prefill_tc", 6: "gemm_f32_tc", 7: "attention_decode_f8", 9: "error-word self-test"}
+                 5: "latent_prefill_tc", 6: "gemm_f32_tc", 7: "attention_decode_f8", 8: "attention_prefill_f8", 9: "error-word self-test"}
 
 
 def _init_error_word(library) -> None:
@@ -90,7 +90,7 @@ def _init_error_word(library) -> None:
     for setter in ("acorn_gemm_tc_set_error_word", "acorn_attention_tc_set_error_word",
                    "acorn_attention_decode_tma_set_error_word", "acorn_selftest_set_error_word",
                    "acorn_gemm_tc_pair_set_error_word", "acorn_latent_prefill_tc_set_error_word", "acorn_gemm_f32_tc_set_error_word",
-                   "acorn_attention_decode_f8_set_error_word"):
+                   "acorn_attention_decode_f8_set_error_word", "acorn_attention_prefill_f8_set_error_word"):
         code = getattr(library, setter)(dev)
         if code != 0:
             raise KernelError(f"{setter}: CUDA error {code}")
@@ -105,7 +105,7 @@ def raise_on_kernel_error() -> None:
     word = _error_word.value
     _error_word.value = 0
     for getter in (gemm_tc_error, attention_tc_error, attention_decode_tma_error, gemm_tc_pair_error, latent_prefill_tc_error, gemm_f32_tc_error,
-                   attention_decode_f8_error):   # clear the kernels' own flags
+                   attention_decode_f8_error, attention_prefill_f8_error):   # clear the kernels' own flags
         getter()
     raise KernelError(f"kernel {_KERNEL_NAMES.get(word // 100, word // 100)} gave up a bounded wait at point "
                       f"{word % 100}: the results of the step are not valid")
@@ -151,6 +151,12 @@ class _Sigs:
     acorn_attention_decode_f8 = [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p,
                                  c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p, c_int,
                                  c_int, c_void_p, c_void_p, c_void_p]
+    acorn_attention_prefill_f8 = [c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int,
+                                  c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int,
+                                  c_void_p, c_void_p]
+    acorn_attention_prefill_f8_supported = [c_int, c_int, c_int, c_int]
+    acorn_attention_prefill_f8_error = []
+    acorn_attention_prefill_f8_set_error_word = [c_void_p]
     acorn_attention_decode_f8_supported = [c_int, c_int, c_int, c_int]
     acorn_attention_decode_f8_merges = [c_int]
     acorn_attention_decode_f8_error = []
@@ -1214,8 +1220,20 @@ def attention_prefill_f8(q: torch.Tensor, q_stride: int, k_pages: torch.Tensor, 
     what = "attention_prefill_f8"
     P, out, stream = _check_f8_attention(what, q, q_stride, k_pages, v_pages, scales, block_table, page_base, row_start, row_pos, tiles,
                                          num_tokens, num_heads, num_kv_heads, head_dim, window, out, chunk, keep_first, sink32)
-    return _attention_f8_plain(q, q_stride, out, k_pages, v_pages, scales, block_table, page_base, row_start, row_pos, tiles,
-                               F8_PREFILL_TILE, num_heads, num_kv_heads, head_dim, P, scale, window, chunk, keep_first, sink32, stream)
+    if not (scale > 0 and lib().acorn_attention_prefill_f8_supported(num_heads, num_kv_heads, head_dim, P)):
+        return _attention_f8_plain(q, q_stride, out, k_pages, v_pages, scales, block_table, page_base, row_start, row_pos, tiles,
+                                   F8_PREFILL_TILE, num_heads, num_kv_heads, head_dim, P, scale, window, chunk, keep_first, sink32,
+                                   stream)
+    _ok(lib().acorn_attention_prefill_f8(q.data_ptr(), q_stride, num_tokens, out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+                                         scales.data_ptr(), k_pages.shape[0], block_table.data_ptr(), page_base.data_ptr(),
+                                         block_table.stride(0), row_start.data_ptr(), row_pos.data_ptr(), tiles.data_ptr(),
+                                         tiles.shape[0], num_heads, num_kv_heads, head_dim, P, float(scale), int(window or 0),
+                                         int(chunk or 0), int(keep_first or 0), _ptr(sink32), stream), what)
+    return out
+
+
+def attention_prefill_f8_error() -> int:
+    return int(lib().acorn_attention_prefill_f8_error())
 
 
 def attention_tc_error() -> int:
