@@ -10,11 +10,6 @@
 #define F8P_THREADS 128
 #define F8P_MAX_D 256
 
-__device__ __forceinline__ float2 f8_codes2(uint32_t two) {
-    const uint32_t h = f8_to_f16x2((uint16_t)two);
-    return __half22float2(*reinterpret_cast<const __half2*>(&h));
-}
-
 __global__ void __launch_bounds__(F8P_THREADS) attention_f8_plain_kernel(const F8AttnParams p, int d, int tile_tokens) {
     __shared__ float sq[F8P_MAX_D];
     __shared__ float so[4][F8P_MAX_D];

@@ -1,95 +1,175 @@
-// Prefill attention over the pages of the 8-bit cache (f8_cache.cuh) on the 5th-generation tensor cores, head sizes 64 and 128:
-// causal attention of a tile of 128 consecutive queries of one request, S = Q K^T and O += P V by tcgen05.mma with the
-// accumulators in tensor memory.
+// Prefill attention over the pages of the 8-bit cache (f8_cache.cuh), head sizes 64 and 128: causal attention of tiles of 128
+// consecutive queries of one request, on the 5th-generation tensor cores.
 //
-// One CTA per (tile of 128 queries, pair of query heads that share a key/value head), one CTA to an SM, as in
-// attention_prefill_tc.cu: the two heads ("units") read the same tiles and take turns on the tensor cores.  What is new is that K
-// and V arrive as codes and are turned into bfloat16 on the way, which is exact (code * 2^e is a bfloat16 number), so that the
-// products are those of a bfloat16 cache of the same numbers.  Why not 8-bit matrix instructions: the queries and the weights
-// would have to be cut into e4m3 parts, two at least, and a product would take as long as one in bfloat16.
-//   warps 0-3  softmax of unit 0, warps 4-7 of unit 1: thread r owns query row r (= TMEM lane r): masks, exponentiates
-//              in float32 base 2 against a reference maximum that moves when a row outgrew it by 2^8, writes P (bfloat16) over S.
-//   warps 8-11 turn a block's codes into the operand tiles, 32 keys a warp: 16 codes a lane (16 bytes in, 32 out, swizzled as the
-//              matrix instruction wants them).  s eeee mmm shifted into a bfloat16 number's places reads 2^-120 times its value,
-//              subnormal codes included; one multiplication by 2^(120 + e) makes it the entry (a second one where e > 7).
-//              Keys that no query of the tile reads get zero values (a slot that was never written may hold anything);
-//              a row that is no number gets a NaN key, which spoils the queries that read it, and zero values.
-//   warp 12    producer: TMA loads of Q (once) and of the codes of each block of 128 keys (a box is the keys and the values of one
-//              page and head), asynchronous copies of their exponents, into two stages of 32 KB.
-//   warp 13    MMA issuer (converged; one elected lane issues): per block j and unit u, O_u += P_u[j] V_j with P from
-//              tensor memory, then S_u = Q_u K_{j+1}^T into the columns P_u[j] was read from.
-// The softmax warps need 184 registers a thread, sixteen warps get 128 each: the warpgroups share 4 x 128 out as 184, 184,
-// 80 (codes) and 64 (the rest).  Operand tiles K_0 V_0 K_1 V_1 ... go through a ring of three.  Tensor memory (512 columns): S / P of unit u at columns 128 u,
-// O of unit u at 256 + 128 u.
+// Three kernels.
+// 1. The keys and values that the tiles read become bfloat16 rows, [slot][kv head][key], which is exact (code * 2^e is a
+//    bfloat16 number).  Done once a call, it reads and writes 5 bytes a number; turned into operand tiles by warps of the attention
+//    kernel itself, every (tile, pair of heads) did it again, in competition with the softmax for the integer pipe and with the matrix
+//    instructions for shared memory (8,192 tokens, 32 heads over 8: 840 us).
+//    Keys outside a row's range within its blocks of 128 get zero rows, so that whatever a slot of a page holds that was never
+//    written, nothing of it is read; a row that is no number gets a NaN key, which spoils the queries that read it, and a zero value.
+// 2. S = Q K^T and O += P V by tcgen05.mma with the accumulators in tensor memory.  One CTA per (tile, pair of query heads
+//    that share a key/value head, split), one CTA to an SM.  The two heads ("units") read the same K and V tiles and take turns on
+//    the tensor cores.
+//      warps 0-7   softmax of unit 0, warps 8-15 of unit 1.  A query row (= TMEM lane) belongs to two threads, 64 keys of a
+//                  block each: a block's scores pass through the softmax in half the time that one thread a row takes, and
+//                  that time, not the tensor cores' or the exponentials', is what a unit's turn waits for.
+//                  Weights are taken against a reference maximum that both threads of a row share; it moves when either of them
+//                  saw a score beyond it by more than 2^8 (one vote of the unit's 256 threads a block; always so in the first
+//                  block), and only then the two exchange their maxima, read the block again and scale O.
+//      warp 16     producer: Q (once), K and V tiles by TMA into a ring of five.
+//      warp 17     MMA issuer (converged; one elected lane issues): per block j and unit u, O_u += P_u[j] V_j with P from
+//                  tensor memory, then S_u = Q_u K_{j+1}^T into the columns P_u[j] was read from.
+//    The softmax warps take 104 registers a thread, the fourth of a warpgroup's that the others leave them (twenty warps get
+//    96 each; two are there for the split, which goes by warpgroups).
+//    Tensor memory (512 columns): S / P of unit u at columns 128 u, O of unit u at 256 + 128 u.
+// 3. Where the tiles are few, a tile's keys are split over several CTAs, whose results (float32, normalised, with the logarithm of
+//    their sums) are joined by a third kernel.
 //
 // Every mbarrier wait is bounded; a wait that gives up records g_attn_pre_f8_error and the CTA drains.
 #include "f8_tma.cuh"
 
 #define PF8_BM 128
 #define PF8_BN 128
-#define PF8_SLOTS 3
-#define PF8_STAGES 2
-#define PF8_THREADS 512               // two of the 16 warps are there for the register split, which goes by warpgroups
-#define PF8_RESCALE_LOG2 8.0f
+#define PF8_SLOTS 5
+#define PF8_THREADS 640
+#define PF8_GROW_LOG2 8.0f
 #define PF8_TMEM_COLS 512
 
 __device__ int g_attn_pre_f8_error = 0;
 
 struct PrefillF8Params {
     F8AttnParams a;
-    int pairs, joint, v_first;       // pairs = ceil((nq / nkv) / 2): CTAs per (tile, kv head)
+    int pairs;                // ceil((nq / nkv) / 2): CTAs per (tile, kv head, split)
+    int n_tiles, rows;        // rows: of the block table
+    int cap;                  // keys a slot has room for, a multiple of 128
+    int kvh0, kvhs;           // the kv heads of this pass
+    int num_splits;
+    bf16* k_rows;             // [slots, kvhs, cap, D]
+    bf16* v_rows;
+    float* part_o;            // [splits, n_tiles, 128, nq, D] where num_splits > 1
+    float* part_lse;          // [splits, n_tiles, 128, nq]
 };
+
+// A row's blocks of 128 keys: those a rule's range covers, lo .. hi, with the kept first keys in front as blocks of their own.
+struct F8Blocks {
+    int lo, hi, nkb, n;
+    __device__ __forceinline__ F8Blocks(const AttnMask& m, int pos0, int n_q) {
+        hi = pos0 + n_q;                                             // keys < hi are read
+        lo = mask_lo(m, pos0) & ~(PF8_BN - 1);                       // the first query's rule starts first
+        nkb = (m.keep > 0 && lo > 0) ? min((m.keep + PF8_BN - 1) / PF8_BN, lo / PF8_BN) : 0;
+        n = n_q > 0 ? nkb + (hi - lo + PF8_BN - 1) / PF8_BN : 0;
+    }
+    __device__ __forceinline__ int key0(int j) const { return j < nkb ? j * PF8_BN : lo + (j - nkb) * PF8_BN; }
+};
+
+// The slot that holds a row's keys: the row itself, or where there are fewer tiles than rows the first tile of that row.
+// All threads of a warp call it.
+__device__ __forceinline__ int f8_slot(const PrefillF8Params& pp, int r) {
+    if (pp.n_tiles >= pp.rows) return r;
+    const int lane = threadIdx.x & 31;
+    for (int t0 = 0; t0 < pp.n_tiles; t0 += 32) {
+        const uint32_t hit = __ballot_sync(0xffffffffu, t0 + lane < pp.n_tiles && pp.a.tiles[2 * min(t0 + lane, pp.n_tiles - 1)] == r);
+        if (hit) return t0 + __ffs(hit) - 1;
+    }
+    return 0;
+}
+// The key that a row's slot starts with: the first whose page the row still holds, down to a multiple of 128.
+__device__ __forceinline__ int f8_slot_key(const F8AttnParams& p, int r) { return (p.page_base[r] << p.logP) & ~(PF8_BN - 1); }
+
+// ---------------------------------------------------------------- 1. pages to rows of bfloat16
+
+#define RB_THREADS 256
+
+// One CTA per (block of 128 keys, kv head of the pass, slot); 16 codes a thread at a time.
+template <int D>
+__global__ void __launch_bounds__(RB_THREADS) read_pages_f8_kernel(const PrefillF8Params pp) {
+    const F8AttnParams& p = pp.a;
+    pdl_wait();
+    pdl_trigger();
+    const int slot = blockIdx.z, kvh = pp.kvh0 + blockIdx.y;
+    int r = slot;
+    if (pp.n_tiles < pp.rows) {
+        r = p.tiles[2 * slot];
+        if (f8_slot(pp, r) != slot) return;                          // another tile of the row came first
+    }
+    const F8Blocks b(p.mask, p.row_pos[r], p.row_start[r + 1] - p.row_start[r]);
+    const int* table = p.block_table + (int64_t)r * p.table_stride - p.page_base[r];
+    const int first_key = p.page_base[r] << p.logP, slot_key = f8_slot_key(p, r), pmask = (1 << p.logP) - 1;
+    constexpr int PIECES = D / 16;
+    for (int j = blockIdx.x; j < b.n; j += gridDim.x) {
+        const int key0 = b.key0(j);
+        if (key0 < slot_key) continue;                               // (a kept block whose pages are gone)
+        const int64_t out0 = ((int64_t)(slot * pp.kvhs + blockIdx.y) * pp.cap + (key0 - slot_key)) * D;
+#pragma unroll 2
+        for (int idx = threadIdx.x; idx < PF8_BN * PIECES; idx += RB_THREADS) {
+            const int row = idx / PIECES, piece = idx % PIECES, key = key0 + row;
+            uint4 kc = make_uint4(0u, 0u, 0u, 0u), vc = kc;
+            float ks = 0.f, vs = 0.f;
+            if (key >= first_key && key < b.hi) {
+                const int64_t at = (((int64_t)table[key >> p.logP] * p.nkv + kvh) << p.logP) + (key & pmask);
+                kc = *reinterpret_cast<const uint4*>(p.k_pages + at * D + 16 * piece);
+                vc = *reinterpret_cast<const uint4*>(p.v_pages + at * D + 16 * piece);
+                const uint32_t bytes = *reinterpret_cast<const uint16_t*>(p.scales + 2 * at);
+                ks = f8_scale(bytes & 255u);
+                vs = f8_scale(bytes >> 8);
+                if (isnan(ks) || isnan(vs)) { ks = __uint_as_float(0x7fc00000u); vs = 0.f; }
+            }
+            const uint32_t kw[4] = {kc.x, kc.y, kc.z, kc.w}, vw[4] = {vc.x, vc.y, vc.z, vc.w};
+            uint32_t ko[8], vo[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const float2 a = f8_codes2(kw[q >> 1] >> (16 * (q & 1))), c = f8_codes2(vw[q >> 1] >> (16 * (q & 1)));
+                const __nv_bfloat162 ab = __floats2bfloat162_rn(a.x * ks, a.y * ks), cb = __floats2bfloat162_rn(c.x * vs, c.y * vs);
+                ko[q] = *reinterpret_cast<const uint32_t*>(&ab);
+                vo[q] = *reinterpret_cast<const uint32_t*>(&cb);
+            }
+            uint4* kd = reinterpret_cast<uint4*>(pp.k_rows + out0 + (int64_t)row * D + 16 * piece);
+            uint4* vd = reinterpret_cast<uint4*>(pp.v_rows + out0 + (int64_t)row * D + 16 * piece);
+            kd[0] = make_uint4(ko[0], ko[1], ko[2], ko[3]); kd[1] = make_uint4(ko[4], ko[5], ko[6], ko[7]);
+            vd[0] = make_uint4(vo[0], vo[1], vo[2], vo[3]); vd[1] = make_uint4(vo[4], vo[5], vo[6], vo[7]);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- 2. attention
 
 template <int D> struct PrefillF8 {
     static constexpr int HALVES = D / 64;
     static constexpr int HALF_BYTES = PF8_BN * 128;                  // [128 rows x 64 entries] bf16
     static constexpr int Q_BYTES = HALVES * PF8_BM * 128;            // one unit
-    static constexpr int TILE_BYTES = HALVES * HALF_BYTES;           // a K or V operand tile
-    static constexpr int RAW_BYTES = 2 * PF8_BN * D;                 // the codes of a block's keys and values
-    static constexpr int SCALE_BYTES = 2 * PF8_BN;
+    static constexpr int TILE_BYTES = HALVES * HALF_BYTES;           // a K or V tile
     static constexpr int TILES = 2 * Q_BYTES;                        // offsets in shared memory
-    static constexpr int RAW = TILES + PF8_SLOTS * TILE_BYTES;
-    static constexpr int SCALES = RAW + PF8_STAGES * RAW_BYTES;
-    static constexpr int BARS = SCALES + PF8_STAGES * SCALE_BYTES;
-    // q_full, raw_full, raw_empty [STAGES], full, empty [SLOTS], s_full, p_full, o_done [unit]
-    static constexpr int NUM_BARS = 1 + 2 * PF8_STAGES + 2 * PF8_SLOTS + 6;
-    static constexpr int SMEM = BARS + NUM_BARS * 8 + 16;
+    static constexpr int BARS = TILES + PF8_SLOTS * TILE_BYTES;
+    // q_full, full, empty [SLOTS], s_full, p_full, o_done [unit]
+    static constexpr int NUM_BARS = 1 + 2 * PF8_SLOTS + 6;
+    static constexpr int SHARED = BARS + NUM_BARS * 8 + 16;          // [unit][half][row]: what the two threads of a row exchange
+    static constexpr int SMEM = SHARED + 2 * 2 * PF8_BM * 4;
 };
 
-__device__ __forceinline__ void pf8_mask(float (&s)[64], int key0, int qpos, bool row_ok, int first_seen, int keep) {
+// Of columns c, those up to `last` are seen that are not before `first` or are before `keep` (all relative to the first one).
+__device__ __forceinline__ void pf8_mask(float (&s)[32], int last, int first, int keep) {
 #pragma unroll
-    for (int c = 0; c < 64; ++c) {
-        const int key = key0 + c;
-        const bool seen = key <= qpos && row_ok && (key >= first_seen || key < keep);
-        s[c] = seen ? s[c] : -INFINITY;
-    }
+    for (int c = 0; c < 32; ++c) s[c] = c <= last && (c >= first || c < keep) ? s[c] : -INFINITY;
 }
 
-__device__ __forceinline__ float pf8_max(const float (&s)[64]) {
-    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+__device__ __forceinline__ float pf8_max(const float (&s)[32], float m) {
+    float a = m, b = -INFINITY;
 #pragma unroll
-    for (int c = 0; c < 64; c += 4) {
-        m[0] = fmaxf(m[0], s[c]); m[1] = fmaxf(m[1], s[c + 1]);
-        m[2] = fmaxf(m[2], s[c + 2]); m[3] = fmaxf(m[3], s[c + 3]);
+    for (int c = 0; c < 32; c += 4) {
+        a = fmaxf(a, fmaxf(s[c], s[c + 1]));
+        b = fmaxf(b, fmaxf(s[c + 2], s[c + 3]));
     }
-    return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+    return fmaxf(a, b);
 }
 
-// w[i] = bf16x2(2^((s[2i] - ref) * scale), 2^((s[2i+1] - ref) * scale)); returns the sum of the 64 values.  The rounding of
-// ref * scale is a factor that all weights of a row share; where it could be a large one (scores beyond 2^20), the
-// difference is taken first.
-__device__ __forceinline__ float pf8_exp_pack(float (&s)[64], float scale_log2, float ref, uint32_t (&w)[32]) {
+// w[i] = bf16x2(2^(s[2i] * scale - m), 2^(s[2i+1] * scale - m)); returns the sum of the 32 values.
+__device__ __forceinline__ float pf8_exp_pack(const float (&s)[32], float scale, float neg_m, uint32_t* w) {
     float ps[4] = {0.f, 0.f, 0.f, 0.f};
-    float neg_ref = -(ref * scale_log2);
-    if (__any_sync(0xffffffffu, fabsf(neg_ref) > 1048576.f)) {
 #pragma unroll
-        for (int c = 0; c < 64; ++c) s[c] -= ref;
-        neg_ref = 0.f;
-    }
-#pragma unroll
-    for (int c = 0; c < 64; c += 2) {
-        const float a = fast_exp2(fmaf(s[c], scale_log2, neg_ref));
-        const float b = fast_exp2(fmaf(s[c + 1], scale_log2, neg_ref));
+    for (int c = 0; c < 32; c += 2) {
+        const float a = fast_exp2(fmaf(s[c], scale, neg_m));
+        const float b = fast_exp2(fmaf(s[c + 1], scale, neg_m));
         ps[(c >> 1) & 3] += a + b;
         const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
         w[c >> 1] = *reinterpret_cast<const uint32_t*>(&v);
@@ -97,16 +177,23 @@ __device__ __forceinline__ float pf8_exp_pack(float (&s)[64], float scale_log2, 
     return (ps[0] + ps[1]) + (ps[2] + ps[3]);
 }
 
-__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
+// The scale with which a row whose reference is m (in units of log2, at the softmax's scale) is exponentiated.  A weight's
+// exponent is one rounding of s * scale - m, so that the rounding of m itself is a factor that all weights of the row share;
+// beyond 2^29 it could be one that overflows.  There neighbouring float32 scores differ by 32 or more, so that all weights but those
+// of the largest score vanish, and they still do at a scale that brings m to 2^29.
+__device__ __forceinline__ float pf8_row_scale(float scale_log2, float m) {
+    const int beyond = (int)(__float_as_uint(m) >> 23 & 255u) - 127 - 29;
+    return beyond > 0 ? scale_log2 * f8_pow2(-beyond) : scale_log2;
 }
 
-// Two neighbouring codes (bytes `sel` and `sel` + 1 of w) as bfloat16 numbers times 2^-120.
-template <int SEL> __device__ __forceinline__ uint32_t codes_to_bf16x2(uint32_t w) {
-    const uint32_t x = __byte_perm(w, 0u, SEL == 0 ? 0x1404 : 0x3424);       // each code in the high byte of its half
-    return ((x >> 4) & 0x07f007f0u) | (x & 0x80008000u);
+// Meets the 256 threads of a unit; whether `v` holds for any of them.
+__device__ __forceinline__ bool unit_any(int unit, bool v) {
+    uint32_t r;
+    tc_fence_before();
+    asm volatile("{\n .reg .pred a, b;\n setp.ne.u32 a, %1, 0;\n barrier.cta.red.or.pred b, %2, 256, a;\n selp.u32 %0, 1, 0, b;\n}\n"
+                 : "=r"(r) : "r"((uint32_t)v), "r"(unit + 1) : "memory");
+    tc_fence_after();
+    return r != 0;
 }
 
 template <int D>
@@ -119,18 +206,17 @@ __global__ void __launch_bounds__(PF8_THREADS, 1) attention_prefill_f8_kernel(co
     const F8AttnParams& p = pp.a;
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
     const uint32_t q_full = tc_smem(bars);
-    const uint32_t raw_full0 = q_full + 8, raw_empty0 = raw_full0 + 8 * PF8_STAGES;
-    const uint32_t full0 = raw_empty0 + 8 * PF8_STAGES, empty0 = full0 + 8 * PF8_SLOTS;
+    const uint32_t full0 = q_full + 8, empty0 = full0 + 8 * PF8_SLOTS;
     const uint32_t s_full0 = empty0 + 8 * PF8_SLOTS, p_full0 = s_full0 + 16, o_done0 = p_full0 + 16;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L::NUM_BARS);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // CTAs are started in the order of the tile list; CTAs next to one another share a tile and mostly a key/value head.
-    const int per_tile = p.nkv * pp.pairs;
-    const int tile = (int)(blockIdx.x / per_tile);
-    const int kvh = (int)(blockIdx.x % per_tile) / pp.pairs, pair = (int)(blockIdx.x % per_tile) % pp.pairs;
+    const int per_tile = pp.kvhs * pp.pairs;
+    const int tile = (int)(blockIdx.x / per_tile), split = blockIdx.y;
+    const int kvp = (int)(blockIdx.x % per_tile) / pp.pairs, pair = (int)(blockIdx.x % per_tile) % pp.pairs;
     const int rep = p.nq / p.nkv;
-    const int head0 = kvh * rep + 2 * pair;
+    const int head0 = (pp.kvh0 + kvp) * rep + 2 * pair;
     const int units = (2 * pair + 1 < rep) ? 2 : 1;
     if (tc_smem(smem) & 1023u) {            // the swizzled tiles need a 1024-byte aligned base
         if (threadIdx.x == 0) tc_fail(&g_attn_pre_f8_error, 9, ACORN_KERNEL_ATTN_PREFILL_F8);
@@ -138,12 +224,11 @@ __global__ void __launch_bounds__(PF8_THREADS, 1) attention_prefill_f8_kernel(co
     }
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
-        for (int s = 0; s < PF8_STAGES; ++s) { mbar_init(raw_full0 + 8 * s, 33); mbar_init(raw_empty0 + 8 * s, 4); }
-        for (int s = 0; s < PF8_SLOTS; ++s) { mbar_init(full0 + 8 * s, 4); mbar_init(empty0 + 8 * s, 1); }
-        for (int u = 0; u < 2; ++u) { mbar_init(s_full0 + 8 * u, 1); mbar_init(p_full0 + 8 * u, 4); mbar_init(o_done0 + 8 * u, 1); }
+        for (int s = 0; s < PF8_SLOTS; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
+        for (int u = 0; u < 2; ++u) { mbar_init(s_full0 + 8 * u, 1); mbar_init(p_full0 + 8 * u, 8); mbar_init(o_done0 + 8 * u, 1); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 13) {
+    if (warp == 17) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      :: "r"(tc_smem(tmem_slot)), "r"((uint32_t)PF8_TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -160,276 +245,204 @@ __global__ void __launch_bounds__(PF8_THREADS, 1) attention_prefill_f8_kernel(co
     const int tok0 = p.row_start[r] + q0;
     const int n_q = min(PF8_BM, p.row_start[r + 1] - tok0);
     const int pos0 = p.row_pos[r] + q0;
-    const int hi = pos0 + n_q;                                           // keys < hi are read by the tile
-    const int lo_seen = mask_lo(p.mask, pos0);                           // the first query's rule starts first
-    const int lo = lo_seen & ~(PF8_BN - 1);                              // blocks start at multiples of 128 keys
-    // the kept first keys, where the rule's range starts beyond them, are nkb blocks of their own in front
-    const int nkb = (p.mask.keep > 0 && lo > 0) ? min((p.mask.keep + PF8_BN - 1) / PF8_BN, lo / PF8_BN) : 0;
-    const int nb = n_q > 0 ? nkb + (hi - lo + PF8_BN - 1) / PF8_BN : 0;
-    auto key0_of = [&](int j) { return j < nkb ? j * PF8_BN : lo + (j - nkb) * PF8_BN; };
-    const int log_box = min(p.logP, 7), box = 1 << log_box;
+    const F8Blocks blocks(p.mask, pos0, n_q);
+    const int per = (blocks.n + pp.num_splits - 1) / pp.num_splits;
+    const int j0 = min(blocks.n, split * per), nb = min(blocks.n, j0 + per) - j0;        // this split's blocks
 
-    if (warp >= 12) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-      if (warp == 12) {
-        // ---------------------------------------------------------------- producer
-        // The whole warp: lane l looks up the cache row of keys 4 l .. 4 l + 3 of a block, a block ahead of the loads, and copies
-        // their exponents; an elected lane issues the boxes (one page, or 128 keys of a larger one).
-        if (nb > 0 && elect_one()) {
-            mbar_expect_tx(q_full, units * L::Q_BYTES);
-            for (int u = 0; u < units; ++u)
-                for (int h = 0; h < L::HALVES; ++h)
-                    tma_load_2d(tc_smem(smem) + u * L::Q_BYTES + h * PF8_BM * 128, &map_q, q_full, (head0 + u) * D + 64 * h, tok0);
-        }
-        const int* table = p.block_table + (int64_t)r * p.table_stride - p.page_base[r];
-        const int first_key = p.page_base[r] << p.logP;
-        auto row_at = [&](int j) -> int {
-            const int key = key0_of(j) + 4 * lane;
-            int b = key & ~(box - 1);
-            if (b >= hi) b = (hi - 1) & ~(box - 1);                      // masked later: any box that exists
-            if (b < first_key) b = first_key;
-            const int page = table[b >> p.logP];
-            return ((page * p.nkv + kvh) << p.logP) + (b & ((1 << p.logP) - 1)) + (key & (box - 1));
-        };
-        int row_next = nb > 0 ? row_at(0) : 0;
-        for (int j = 0; j < nb; ++j) {
-            const int row = row_next, s = j % PF8_STAGES;
-            if (j + 1 < nb) row_next = row_at(j + 1);
-            const bool got = mbar_wait(raw_empty0 + 8 * s, ((j / PF8_STAGES) & 1) ^ 1);
-            if (!got && lane == 0) tc_fail(&g_attn_pre_f8_error, 1, ACORN_KERNEL_ATTN_PREFILL_F8);
-            if (!__all_sync(0xffffffffu, got)) break;
-            if (elect_one()) mbar_expect_tx(raw_full0 + 8 * s, L::RAW_BYTES);
-            cp_async_bytes<8>(tc_smem(smem + L::SCALES + s * L::SCALE_BYTES) + 8 * lane, p.scales + 2 * (int64_t)row);
-            cp_async_arrive(raw_full0 + 8 * s);
-            for (int k = 0; k < PF8_BN; k += box) {
-                const int y = __shfl_sync(0xffffffffu, row, k >> 2);
-                if (elect_one()) {
-                    const uint32_t dst = tc_smem(smem + L::RAW + s * L::RAW_BYTES) + (uint32_t)(2 * k * D);
-                    tma_load_3d(dst, &map_k, raw_full0 + 8 * s, 0, y, 0);
-                    if (!pp.joint) tma_load_3d(dst + box * D, &map_v, raw_full0 + 8 * s, 0, y, 0);
-                }
+    if (warp >= 16) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if (warp == 16) {
+            // ------------------------------------------------------------ producer
+            const int row0 = (f8_slot(pp, r) * pp.kvhs + kvp) * pp.cap - f8_slot_key(p, r);
+            const int first = f8_slot_key(p, r);
+            if (nb > 0 && elect_one()) {
+                mbar_expect_tx(q_full, units * L::Q_BYTES);
+                for (int u = 0; u < units; ++u)
+                    for (int h = 0; h < L::HALVES; ++h)
+                        tma_load_2d(tc_smem(smem) + u * L::Q_BYTES + h * PF8_BM * 128, &map_q, q_full, (head0 + u) * D + 64 * h, tok0);
             }
-        }
-      } else if (warp == 13) {
-        // ---------------------------------------------------------------- MMA issuer
-        constexpr uint32_t IDESC_QK = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(PF8_BN >> 3) << 17) |
-                                      ((uint32_t)(PF8_BM >> 4) << 24);
-        constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) |
-                                      ((uint32_t)(D >> 3) << 17) | ((uint32_t)(PF8_BM >> 4) << 24);
-        auto wait_all = [&](uint32_t bar, uint32_t parity, int code) -> bool {
-            const bool ok = mbar_wait(bar, parity);
-            if (!ok && lane == 0) tc_fail(&g_attn_pre_f8_error, code, ACORN_KERNEL_ATTN_PREFILL_F8);
-            return __all_sync(0xffffffffu, ok);
-        };
-        const uint32_t qlo = umma_lo(tc_smem(smem)), klo0 = umma_lo(tc_smem(smem + L::TILES));
-        const uint32_t vlo0 = umma_lo_mn(tc_smem(smem + L::TILES), L::HALF_BYTES);
-        auto issue_qk = [&](int u, int slot) {                          // S_u = Q_u K^T, K in `slot`
-            const uint32_t klo = klo0 + slot * (L::TILE_BYTES >> 4);
+            int slot = 0, phase = 0;
+            for (int n = 0; n < 2 * nb; ++n) {                           // K_0 V_0 K_1 V_1 ...
+                const bool got = mbar_wait(empty0 + 8 * slot, phase ^ 1);
+                if (!got && lane == 0) tc_fail(&g_attn_pre_f8_error, 1, ACORN_KERNEL_ATTN_PREFILL_F8);
+                if (!__all_sync(0xffffffffu, got)) break;
+                const CUtensorMap* map = n & 1 ? &map_v : &map_k;
+                const int y = row0 + max(blocks.key0(j0 + (n >> 1)), first);
+                if (elect_one()) {
+                    mbar_expect_tx(full0 + 8 * slot, L::TILE_BYTES);
+                    for (int h = 0; h < L::HALVES; ++h)
+                        tma_load_2d(tc_smem(smem + L::TILES) + slot * L::TILE_BYTES + h * L::HALF_BYTES, map, full0 + 8 * slot, 64 * h, y);
+                }
+                if (++slot == PF8_SLOTS) { slot = 0; phase ^= 1; }
+            }
+        } else if (warp == 17) {
+            // ------------------------------------------------------------ MMA issuer
+            constexpr uint32_t IDESC_QK = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(PF8_BN >> 3) << 17) |
+                                          ((uint32_t)(PF8_BM >> 4) << 24);
+            constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) |
+                                          ((uint32_t)(D >> 3) << 17) | ((uint32_t)(PF8_BM >> 4) << 24);
+            auto wait_all = [&](uint32_t bar, uint32_t parity, int code) -> bool {
+                const bool ok = mbar_wait(bar, parity);
+                if (!ok && lane == 0) tc_fail(&g_attn_pre_f8_error, code, ACORN_KERNEL_ATTN_PREFILL_F8);
+                return __all_sync(0xffffffffu, ok);
+            };
+            const uint32_t qlo = umma_lo(tc_smem(smem)), klo0 = umma_lo(tc_smem(smem + L::TILES));
+            const uint32_t vlo0 = umma_lo_mn(tc_smem(smem + L::TILES), L::HALF_BYTES);
+            auto issue_qk = [&](int u, int slot) {                      // S_u = Q_u K^T, K in `slot`
+                const uint32_t klo = klo0 + slot * (L::TILE_BYTES >> 4);
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k)
-                umma_bf16_elect(tmem_s + u * 128, qlo + ((u * L::Q_BYTES + (k >> 2) * PF8_BM * 128) >> 4) + 2 * (k & 3),
-                                klo + (((k >> 2) * L::HALF_BYTES) >> 4) + 2 * (k & 3), IDESC_QK, k > 0 ? 1u : 0u);
-            umma_commit_elect(s_full0 + 8 * u);
-        };
-        bool good = nb > 0 && wait_all(q_full, 0, 2);
-        int slot = 0, phase = 0;                                         // the next tile of the ring
-        if (good) {
-            good = wait_all(full0, 0, 3);
-            tc_fence_after();
+                for (int k = 0; k < D / 16; ++k)
+                    umma_bf16_elect(tmem_s + u * 128, qlo + ((u * L::Q_BYTES + (k >> 2) * PF8_BM * 128) >> 4) + 2 * (k & 3),
+                                    klo + (((k >> 2) * L::HALF_BYTES) >> 4) + 2 * (k & 3), IDESC_QK, k > 0 ? 1u : 0u);
+                umma_commit_elect(s_full0 + 8 * u);
+            };
+            bool good = nb > 0 && wait_all(q_full, 0, 2) && wait_all(full0, 0, 3);
+            int slot = 0, phase = 0;                                     // the next tile of the ring
             if (good) {
                 for (int u = 0; u < units; ++u) issue_qk(u, 0);
                 umma_commit_elect(empty0);
                 slot = 1;
             }
-        }
-        for (int j = 0; j < nb && good; ++j) {
-            const int sv = slot, pv = phase;                             // V_j
-            if (++slot == PF8_SLOTS) { slot = 0; phase ^= 1; }
-            const int sk = slot, pk = phase;                             // K_{j+1}
-            const bool has_next = j + 1 < nb;
-            if (has_next) { if (++slot == PF8_SLOTS) { slot = 0; phase ^= 1; } }
-            good = wait_all(full0 + 8 * sv, pv, 3);
-            if (!good) break;
-            const uint32_t vlo = vlo0 + sv * (L::TILE_BYTES >> 4);
-            for (int u = 0; u < units && good; ++u) {
-                good = wait_all(p_full0 + 8 * u, j & 1, 4);
-                if (!good) break;
-                tc_fence_after();
-                // 16 keys a step: P advances 8 columns, V 16 rows of 128 bytes
-#pragma unroll
-                for (int k = 0; k < PF8_BN / 16; ++k)
-                    umma_bf16_ts_elect(tmem_o + u * 128, tmem_s + u * 128 + 8 * k, vlo + ((k * 16 * 128) >> 4), IDESC_PV,
-                                       k > 0 || j > 0 ? 1u : 0u);
-                if (u == units - 1) umma_commit_elect(empty0 + 8 * sv);
-                // the next scores go where P was: the pipe runs them after the product above
-                if (has_next) {
-                    if (u == 0) good = wait_all(full0 + 8 * sk, pk, 5);
-                    if (good) issue_qk(u, sk);
-                } else {
-                    umma_commit_elect(o_done0 + 8 * u);
-                }
-            }
-            if (good && has_next) umma_commit_elect(empty0 + 8 * sk);
-        }
-      }
-    } else if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-        // ---------------------------------------------------------------- codes to operand tiles
-        constexpr int PIECES = D / 16, KEYS = 32 / PIECES;               // 16-byte pieces of a row; keys the warp takes at a time
-        const int w0 = (warp - 8) * 32;
-        const int piece = lane % PIECES, sub = lane / PIECES;
-        const int chunk0 = (2 * piece) & 7;                              // the first of the piece's two 16-byte chunks in its half
-        const int half_off = (piece >> 2) * L::HALF_BYTES;
-        // (lanes of the second half write their second chunk first: the two halves' chunks then lie in different banks)
-        const int swap = D == 128 ? piece >> 2 : 0;
-        int slot = 0, phase = 0;
-        for (int j = 0; j < nb; ++j) {
-            const int s = j % PF8_STAGES;
-            bool got = mbar_wait(raw_full0 + 8 * s, (j / PF8_STAGES) & 1);
-            if (!got) tc_fail(&g_attn_pre_f8_error, 11, ACORN_KERNEL_ATTN_PREFILL_F8);
-            if (!__all_sync(0xffffffffu, got)) break;
-            const uint32_t bytes = *reinterpret_cast<const uint16_t*>(smem + L::SCALES + s * L::SCALE_BYTES + 2 * (w0 + lane));
-            const int kbyte = bytes & 255u, vbyte = bytes >> 8, key = key0_of(j) + w0 + lane;
-            const bool read = key < hi && (key >= lo_seen || key < p.mask.keep);
-            bool fine = true;
-            for (int kv = 0; kv < 2; ++kv) {
-                // this lane's key: 2^(120 + e) = 2^(byte - 7), as two factors where that is beyond bfloat16
-                const int byte = kv ? vbyte : kbyte;
-                const bool none = kbyte == F8_NAN_BYTE || vbyte == F8_NAN_BYTE;
-                const bool large = byte > 134;
-                uint32_t f1 = (uint32_t)(large ? 127 + 120 : byte + 120) << 7, f2 = large ? (uint32_t)byte << 7 : 0x3f80u;
-                if (none) { f1 = kv ? 0u : 0x7fc0u; f2 = 0x3f80u; }
-                if (kv && !read) { f1 = 0u; f2 = 0x3f80u; }
-                const bool any_large = __any_sync(0xffffffffu, f2 != 0x3f80u);
-                const uint32_t both = f1 | f2 << 16;
-                got = mbar_wait(empty0 + 8 * slot, phase ^ 1);
-                if (!got) tc_fail(&g_attn_pre_f8_error, 12, ACORN_KERNEL_ATTN_PREFILL_F8);
-                fine = __all_sync(0xffffffffu, got);
-                if (!fine) break;
-                const uint8_t* raw = smem + L::RAW + s * L::RAW_BYTES;
-                uint8_t* tile_at = smem + L::TILES + slot * L::TILE_BYTES + half_off;
-                const int skip = (kv ^ pp.v_first) << log_box;           // the values' rows follow the keys', or the other way round
-#pragma unroll 4
-                for (int it = 0; it < 32 / KEYS; ++it) {
-                    const int k = it * KEYS + sub;
-                    const uint4 c = *reinterpret_cast<const uint4*>(raw + (f8_stage_row(w0 + k, log_box) + skip) * D + 16 * piece);
-                    const uint32_t f = __shfl_sync(0xffffffffu, both, k);
-                    const uint32_t fa = __byte_perm(f, 0u, 0x1010), fb = __byte_perm(f, 0u, 0x3232);
-                    const uint32_t cw[4] = {c.x, c.y, c.z, c.w};
-                    uint32_t v[8];
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        v[2 * q] = mul_bf16x2(codes_to_bf16x2<0>(cw[q]), fa);
-                        v[2 * q + 1] = mul_bf16x2(codes_to_bf16x2<2>(cw[q]), fa);
-                    }
-                    if (any_large) {
-#pragma unroll
-                        for (int q = 0; q < 8; ++q) v[q] = mul_bf16x2(v[q], fb);
-                    }
-                    const int row = w0 + k;
-                    uint8_t* at = tile_at + row * 128;
-                    const uint4 lo4 = make_uint4(v[0], v[1], v[2], v[3]), hi4 = make_uint4(v[4], v[5], v[6], v[7]);
-                    *reinterpret_cast<uint4*>(at + (((chunk0 + swap) ^ (row & 7)) << 4)) = swap ? hi4 : lo4;
-                    *reinterpret_cast<uint4*>(at + (((chunk0 + 1 - swap) ^ (row & 7)) << 4)) = swap ? lo4 : hi4;
-                }
-                fence_proxy_async();                                     // the matrix instructions read what was written here
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(full0 + 8 * slot);
-                    if (kv) mbar_arrive(raw_empty0 + 8 * s);
-                }
+            for (int j = 0; j < nb && good; ++j) {
+                const int sv = slot, pv = phase;                         // V_j
                 if (++slot == PF8_SLOTS) { slot = 0; phase ^= 1; }
+                const int sk = slot, pk = phase;                         // K_{j+1}
+                const bool has_next = j + 1 < nb;
+                if (has_next) { if (++slot == PF8_SLOTS) { slot = 0; phase ^= 1; } }
+                good = wait_all(full0 + 8 * sv, pv, 3);
+                if (good && has_next) good = wait_all(full0 + 8 * sk, pk, 3);
+                if (!good) break;
+                const uint32_t vlo = vlo0 + sv * (L::TILE_BYTES >> 4);
+                for (int u = 0; u < units && good; ++u) {
+                    good = wait_all(p_full0 + 8 * u, j & 1, 4);
+                    if (!good) break;
+                    tc_fence_after();
+                    // 16 keys a step: P advances 8 columns, V 16 rows of 128 bytes
+#pragma unroll
+                    for (int k = 0; k < PF8_BN / 16; ++k)
+                        umma_bf16_ts_elect(tmem_o + u * 128, tmem_s + u * 128 + 8 * k, vlo + ((k * 16 * 128) >> 4), IDESC_PV,
+                                           k > 0 || j > 0 ? 1u : 0u);
+                    // the next scores go where P was: the pipe runs them after the product above
+                    if (has_next) issue_qk(u, sk);
+                    else umma_commit_elect(o_done0 + 8 * u);
+                }
+                if (!good) break;
+                umma_commit_elect(empty0 + 8 * sv);
+                if (has_next) umma_commit_elect(empty0 + 8 * sk);
             }
-            if (!fine) break;
         }
     } else {
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
-      if (warp < 4 * units) {
-        // ---------------------------------------------------------------- softmax and output
-        const int u = warp >> 2;
-        const int row = (warp & 3) * 32 + lane;                          // query row = TMEM lane
-        const int head = head0 + u;
-        const int qpos = pos0 + row;
-        const int first_seen = mask_lo(p.mask, qpos);
-        const bool row_ok = row < n_q;
-        const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t my_s = tmem_s + lane_addr + u * 128, my_o = tmem_o + lane_addr + u * 128;
-        const uint32_t s_full = s_full0 + 8 * u, p_full = p_full0 + 8 * u, o_done = o_done0 + 8 * u;
-        const int last_lo = n_q > 0 ? mask_lo(p.mask, hi - 1) : 0;       // the last query's rule starts last
-        float m_ref = -INFINITY, ref = 0.f, l_run = 0.f;                 // the reference in units of log2, and of the scores
-        bool good = nb > 0;
-        for (int j = 0; j < nb; ++j) {
-            // S of block j is complete; so is P V of block j-1, issued before it: O is stable
-            if (!mbar_wait(s_full, j & 1)) { tc_fail(&g_attn_pre_f8_error, 6, ACORN_KERNEL_ATTN_PREFILL_F8); good = false; }
-            good = __all_sync(0xffffffffu, good);
-            if (!good) break;
-            tc_fence_after();
-            const int key0 = key0_of(j);
-            // a block that every query of the tile sees whole needs no mask
-            const bool masked = key0 + PF8_BN - 1 > pos0 || key0 < last_lo || n_q < PF8_BM;
-            // One pass in the common case: exponentiate against the reference maximum the row already has while the block's own
-            // maximum is taken; only a row whose maximum outgrew the reference by more than 2^8 (always so in its first
-            // block) moves the reference, and then the warp reads the block again.
-            float s[64];
-            uint32_t w_lo[32], w_hi[32];
-            tmem_ld64(my_s, s);
-            if (masked) pf8_mask(s, key0, qpos, row_ok, first_seen, p.mask.keep);
-            float mx = pf8_max(s);
-            float psum = pf8_exp_pack(s, p.scale_log2, ref, w_lo);
-            tmem_ld64(my_s + 64, s);
-            if (masked) pf8_mask(s, key0 + 64, qpos, row_ok, first_seen, p.mask.keep);
-            const float top = fmaxf(mx, pf8_max(s));
-            mx = top * p.scale_log2;                                     // the scale is positive
-            float corr = 1.f;
-            const bool grew = mx > m_ref + PF8_RESCALE_LOG2;
-            if (__any_sync(0xffffffffu, grew)) {
-                if (grew) {
-                    corr = fast_exp2(m_ref - mx);                        // m_ref = -inf: 0
-                    l_run *= corr;
-                    m_ref = mx;
-                    ref = top;
-                }
-                psum = pf8_exp_pack(s, p.scale_log2, ref, w_hi);
-                tmem_ld64(my_s, s);
-                if (masked) pf8_mask(s, key0, qpos, row_ok, first_seen, p.mask.keep);
-                psum += pf8_exp_pack(s, p.scale_log2, ref, w_lo);
-            } else {
-                psum += pf8_exp_pack(s, p.scale_log2, ref, w_hi);
-            }
-            l_run += psum;
-            if (j > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+        const int u = warp >> 3, half = (warp >> 2) & 1;
+        if (u < units) {
+            // ------------------------------------------------------------ softmax and output
+            const int row = (warp & 3) * 32 + lane;                      // query row = TMEM lane
+            const int head = head0 + u;
+            const bool row_ok = row < n_q;
+            const int last_seen = row_ok ? pos0 + row : -1, first_seen = mask_lo(p.mask, pos0 + row);
+            const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
+            const uint32_t unit_s = tmem_s + lane_addr + u * 128, my_s = unit_s + 64 * half, my_p = unit_s + 32 * half;
+            const uint32_t my_o = tmem_o + lane_addr + u * 128 + half * (D / 2);
+            const uint32_t s_full = s_full0 + 8 * u, p_full = p_full0 + 8 * u, o_done = o_done0 + 8 * u;
+            float* mine = reinterpret_cast<float*>(smem + L::SHARED) + (2 * u + half) * PF8_BM + row;
+            float* other = reinterpret_cast<float*>(smem + L::SHARED) + (2 * u + 1 - half) * PF8_BM + row;
+            const int last_lo = n_q > 0 ? mask_lo(p.mask, blocks.hi - 1) : 0;            // the last query's rule starts last
+            float m_ref = -INFINITY, l_run = 0.f;                        // the reference in units of log2
+            float scale = p.scale_log2, neg_m = 0.f;                     // what the row's scores are exponentiated with
+            bool good = nb > 0;
+            for (int j = 0; j < nb; ++j) {
+                // S of block j is complete; so is P V of block j-1, issued before it: O is stable
+                bool got = mbar_wait(s_full, j & 1);
+                if (!got) tc_fail(&g_attn_pre_f8_error, 6, ACORN_KERNEL_ATTN_PREFILL_F8);
+                tc_fence_after();
+                const int block0 = blocks.key0(j0 + j), key0 = block0 + 64 * half;
+                // a block that every query of the tile sees whole needs no mask
+                const bool masked = block0 + PF8_BN - 1 > pos0 || block0 < last_lo || n_q < PF8_BM;
+                float s[32];
+                uint32_t w[32];
+                float top = -INFINITY, psum = 0.f;
 #pragma unroll
-                for (int c = 0; c < D; c += 32) {
+                for (int h = 0; h < 2; ++h) {
+                    tmem_ld32(my_s + 32 * h, s);
+                    if (masked) pf8_mask(s, last_seen - key0 - 32 * h, first_seen - key0 - 32 * h, p.mask.keep - key0 - 32 * h);
+                    top = pf8_max(s, top);
+                    psum += pf8_exp_pack(s, scale, neg_m, w + 16 * h);
+                }
+                const float mx = top * p.scale_log2;                     // the scale is positive
+                // (a wait that gave up makes the whole unit stop, through the same vote)
+                if (unit_any(u, !got || mx > m_ref + PF8_GROW_LOG2)) {
+                    *mine = got ? top : INFINITY;
+                    good = !unit_any(u, !got);
+                    if (!good) break;
+                    const float both = fmaxf(top, *other), mb = both * p.scale_log2;
+                    float corr = 1.f;
+                    if (mb > m_ref + PF8_GROW_LOG2) {
+                        corr = fast_exp2(m_ref - mb);                    // m_ref = -inf: 0
+                        l_run *= corr;
+                        m_ref = mb;
+                        scale = pf8_row_scale(p.scale_log2, mb);
+                        neg_m = -(both * scale);
+                    }
+                    psum = 0.f;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        tmem_ld32(my_s + 32 * h, s);
+                        if (masked) pf8_mask(s, last_seen - key0 - 32 * h, first_seen - key0 - 32 * h, p.mask.keep - key0 - 32 * h);
+                        psum += pf8_exp_pack(s, scale, neg_m, w + 16 * h);
+                    }
+                    if (j > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
+#pragma unroll 1
+                        for (int c = 0; c < D / 2; c += 32) {
+                            tmem_ld32(my_o + c, s);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) s[i] *= corr;
+                            tmem_st32(my_o + c, s);
+                        }
+                    }
+                    unit_any(u, false);                                  // nobody reads S any more: P may be written over it
+                }
+                l_run += psum;
+                tmem_st32_raw(my_p, w);                                  // column c of P holds keys 2c and 2c + 1
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full);
+            }
+            if (good) {
+                const bool got = mbar_wait(o_done, 0);
+                if (!got) tc_fail(&g_attn_pre_f8_error, 8, ACORN_KERNEL_ATTN_PREFILL_F8);
+                unit_any(u, false);                                      // (the last exchange's values have been read)
+                *mine = l_run;
+                unit_any(u, false);
+                good = __all_sync(0xffffffffu, got);
+            }
+            if (good) {
+                tc_fence_after();
+                float total = l_run + *other;
+                // a sink is one more term of the denominator, against the same reference maximum as the keys' terms; the first
+                // split has it
+                const float sink = p.sink && row_ok && split == 0 ? p.sink[head] * 1.4426950408889634f : -INFINITY;
+                // (a split that holds no key of the row: the sink alone; NaN keys leave no maximum, but a NaN sum)
+                const bool empty = m_ref == -INFINITY && total == 0.f;
+                if (sink != -INFINITY && !empty) total += exp2f(sink - m_ref);
+                const float inv = row_ok ? 1.f / total : 0.f;
+                const int64_t out_row = (int64_t)(tok0 + row) * p.nq + head;
+                const int64_t part_row = (((int64_t)split * pp.n_tiles + tile) * PF8_BM + row) * p.nq + head;
+                if (pp.num_splits > 1 && row_ok && half == 0) pp.part_lse[part_row] = empty ? sink : m_ref + log2f(total);
+#pragma unroll 1
+                for (int c = 0; c < D / 2; c += 32) {
                     float part[32];
                     tmem_ld32(my_o + c, part);
+                    if (!row_ok) continue;
+                    if (pp.num_splits > 1) {
+                        float4* dst = reinterpret_cast<float4*>(pp.part_o + part_row * D + half * (D / 2) + c);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) part[i] *= corr;
-                    tmem_st32(my_o + c, part);
-                }
-            }
-            // P over the first 64 columns of S: column c holds keys 2c and 2c + 1
-            tmem_st32_raw(my_s, w_lo);
-            tmem_st32_raw(my_s + 32, w_hi);
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(p_full);
-        }
-        if (good) {
-            if (!mbar_wait(o_done, 0)) { tc_fail(&g_attn_pre_f8_error, 8, ACORN_KERNEL_ATTN_PREFILL_F8); good = false; }
-            good = __all_sync(0xffffffffu, good);
-        }
-        if (good) {
-            tc_fence_after();
-            // a sink is one more term of the denominator, against the same reference maximum as the keys' terms
-            if (p.sink && row_ok) l_run += exp2f(p.sink[head] * 1.4426950408889634f - m_ref);
-            const float inv = row_ok ? 1.f / l_run : 0.f;
-            bf16* orow = p.out + ((int64_t)(tok0 + row) * p.nq + head) * D;
-#pragma unroll
-            for (int c = 0; c < D; c += 32) {
-                float part[32];
-                tmem_ld32(my_o + c, part);
-                if (row_ok) {
+                        for (int i = 0; i < 32; i += 4)
+                            dst[i >> 2] = empty ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                                : make_float4(part[i] * inv, part[i + 1] * inv, part[i + 2] * inv, part[i + 3] * inv);
+                        continue;
+                    }
+                    uint4* dst = reinterpret_cast<uint4*>(p.out + out_row * D + half * (D / 2) + c);
 #pragma unroll
                     for (int i = 0; i < 32; i += 8) {
                         uint32_t ww[4];
@@ -438,34 +451,79 @@ __global__ void __launch_bounds__(PF8_THREADS, 1) attention_prefill_f8_kernel(co
                             const __nv_bfloat162 v = __floats2bfloat162_rn(part[i + 2 * q] * inv, part[i + 2 * q + 1] * inv);
                             ww[q] = *reinterpret_cast<const uint32_t*>(&v);
                         }
-                        *reinterpret_cast<uint4*>(orow + c + i) = make_uint4(ww[0], ww[1], ww[2], ww[3]);
+                        dst[i >> 3] = make_uint4(ww[0], ww[1], ww[2], ww[3]);
                     }
                 }
+            } else if (nb == 0 && pp.num_splits > 1 && row_ok && half == 0) {
+                // no blocks for this split (never the first): no weight in the join, its outputs are not read
+                pp.part_lse[(((int64_t)split * pp.n_tiles + tile) * PF8_BM + row) * p.nq + head] = -INFINITY;
             }
         }
-      }
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 13) {
+    if (warp == 17) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;"
                      :: "r"(tmem_base), "r"((uint32_t)PF8_TMEM_COLS) : "memory");
     }
 }
 
-// What this kernel takes (a scale that is not positive goes to the general kernel).
+// ---------------------------------------------------------------- 3. the splits joined
+
+// One warp per (query of a tile, head of the pass); 4 entries a lane (2 at head size 64).
+template <int D>
+__global__ void __launch_bounds__(256) attention_prefill_f8_join_kernel(const PrefillF8Params pp) {
+    constexpr int E = D / 32;
+    pdl_wait();
+    pdl_trigger();
+    const F8AttnParams& p = pp.a;
+    const int rep = p.nq / p.nkv, heads = pp.kvhs * rep;
+    const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (item >= (int64_t)pp.n_tiles * PF8_BM * heads) return;
+    const int head = pp.kvh0 * rep + (int)(item % heads), row = (int)(item / heads % PF8_BM), tile = (int)(item / heads / PF8_BM);
+    const int r = p.tiles[2 * tile], tok = p.row_start[r] + p.tiles[2 * tile + 1] + row;
+    if (tok >= p.row_start[r + 1]) return;
+    const int64_t step = (int64_t)pp.n_tiles * PF8_BM * p.nq, at0 = ((int64_t)tile * PF8_BM + row) * p.nq + head;
+    float top = -INFINITY;
+    for (int s = 0; s < pp.num_splits; ++s) top = fmaxf(top, pp.part_lse[at0 + s * step]);
+    float sum = 0.f, acc[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) acc[i] = 0.f;
+    for (int s = 0; s < pp.num_splits; ++s) {
+        const float lse = pp.part_lse[at0 + s * step];
+        if (lse == -INFINITY) continue;
+        const float f = exp2f(lse - top);
+        sum += f;
+        const float* o = pp.part_o + (at0 + s * step) * D + lane * E;
+#pragma unroll
+        for (int i = 0; i < E; ++i) acc[i] = fmaf(f, o[i], acc[i]);
+    }
+    bf16* dst = p.out + ((int64_t)tok * p.nq + head) * D + lane * E;
+    const float inv = 1.f / sum;
+#pragma unroll
+    for (int i = 0; i < E; i += 2) *reinterpret_cast<__nv_bfloat162*>(dst + i) = __floats2bfloat162_rn(acc[i] * inv, acc[i + 1] * inv);
+}
+
+// ---------------------------------------------------------------- host
+
+// What these kernels take (a scale that is not positive goes to the general kernel).
 extern "C" int acorn_attention_prefill_f8_supported(int nq, int nkv, int d, int P) {
-    return nkv > 0 && nq % nkv == 0 && (d == 64 || d == 128) && P >= 8 && P <= 4096 && (P & (P - 1)) == 0;
+    return nkv > 0 && nq % nkv == 0 && (d == 64 || d == 128) && P >= 1 && P <= 4096 && (P & (P - 1)) == 0;
 }
 
 template <int D>
-static int launch_prefill_f8(PrefillF8Params pp, int64_t num_pages, int tokens, int64_t ctas, cudaStream_t stream) {
+static int launch_prefill_f8(const PrefillF8Params& pp, int tokens, int slots, int blocks, cudaStream_t stream) {
     using L = PrefillF8<D>;
     const F8AttnParams& p = pp.a;
     CUtensorMap mq, mk, mv;
+    const int64_t rows = (int64_t)slots * pp.kvhs * pp.cap;
+    if (rows > 0x7fffffff) return ACORN_ERR_UNSUPPORTED;
     int rc = make_map(&mq, p.q, tokens, (int64_t)p.nq * D, p.q_stride, 64, PF8_BM);
     if (rc) return rc;
-    rc = make_code_maps(&mk, &mv, p, num_pages, D, p.logP < 7 ? 1 << p.logP : PF8_BN, CU_TENSOR_MAP_SWIZZLE_NONE, &pp.joint, &pp.v_first);
+    rc = make_map(&mk, pp.k_rows, rows, D, D, 64, PF8_BN);
+    if (rc) return rc;
+    rc = make_map(&mv, pp.v_rows, rows, D, D, 64, PF8_BN);
     if (rc) return rc;
     static AcornPerDevice configured;
     if (!configured.seen()) {
@@ -473,16 +531,28 @@ static int launch_prefill_f8(PrefillF8Params pp, int64_t num_pages, int tokens, 
         if (e != cudaSuccess) return (int)e;
         configured.mark();
     }
-    return acorn_launch(attention_prefill_f8_kernel<D>, dim3((unsigned)ctas), dim3(PF8_THREADS), L::SMEM, stream, mq, mk, mv, pp);
+    rc = acorn_launch(read_pages_f8_kernel<D>, dim3(blocks, pp.kvhs, slots), dim3(RB_THREADS), 0, stream, pp);
+    if (rc) return rc;
+    const int64_t ctas = (int64_t)pp.n_tiles * pp.kvhs * pp.pairs;
+    rc = acorn_launch(attention_prefill_f8_kernel<D>, dim3((unsigned)ctas, pp.num_splits), dim3(PF8_THREADS), L::SMEM, stream, mq, mk, mv, pp);
+    if (rc || pp.num_splits == 1) return rc;
+    const int64_t items = (int64_t)pp.n_tiles * PF8_BM * pp.kvhs * (p.nq / p.nkv);
+    return acorn_launch(attention_prefill_f8_join_kernel<D>, dim3((unsigned)((items + 7) / 8)), dim3(256), 0, stream, pp);
 }
 
+// `slots`: min(rows of the table, tiles); k_rows / v_rows: [slots, kvhs, cap, d] bfloat16 for the kv heads kvh0 .. kvh0 + kvhs - 1
+// of this pass; blocks: CTAs along a row's blocks of 128 keys.
 extern "C" int acorn_attention_prefill_f8(const void* q, int64_t q_stride, int tokens, void* out, const void* k_pages,
-                                          const void* v_pages, const void* scales, int64_t num_pages, const int* block_table,
-                                          const int* page_base, int table_stride, const int* row_start, const int* row_pos,
-                                          const int* tiles, int n_tiles, int nq, int nkv, int d, int P, float scale, int window,
-                                          int chunk, int keep, const float* sink, cudaStream_t stream) {
+                                          const void* v_pages, const void* scales, const int* block_table, const int* page_base,
+                                          int table_stride, int rows, const int* row_start, const int* row_pos, const int* tiles,
+                                          int n_tiles, int nq, int nkv, int d, int P, float scale, int window, int chunk, int keep,
+                                          const float* sink, int kvh0, int kvhs, void* k_rows, void* v_rows, int slots, int cap,
+                                          int blocks, int num_splits, float* part_o, float* part_lse, cudaStream_t stream) {
     if (n_tiles <= 0) return 0;
-    if (!acorn_attention_prefill_f8_supported(nq, nkv, d, P) || q_stride % 8 != 0 || ((uintptr_t)q & 15) || !(scale > 0.f))
+    if (!acorn_attention_prefill_f8_supported(nq, nkv, d, P) || q_stride % 8 != 0 || ((uintptr_t)q & 15) || !(scale > 0.f) ||
+        cap % PF8_BN || slots < 1 || slots > 65535 || kvhs < 1 || kvhs > 65535 || kvh0 < 0 || kvh0 + kvhs > nkv || blocks < 1 ||
+        num_splits < 1 || num_splits > 65535 || (num_splits > 1 && (part_o == nullptr || part_lse == nullptr)) ||
+        slots != (n_tiles < rows ? n_tiles : rows))
         return ACORN_ERR_UNSUPPORTED;
     PrefillF8Params pp;
     F8AttnParams& p = pp.a;
@@ -491,10 +561,10 @@ extern "C" int acorn_attention_prefill_f8(const void* q, int64_t q_stride, int t
     p.row_start = row_start; p.row_pos = row_pos; p.tiles = tiles; p.sink = sink; p.table_stride = table_stride;
     p.nq = nq; p.nkv = nkv; p.mask = {window, chunk, keep}; p.scale_log2 = scale * 1.4426950408889634f;
     p.logP = acorn_log2_exact_tc(P);
-    pp.pairs = (nq / nkv + 1) / 2;
-    const int64_t ctas = (int64_t)n_tiles * nkv * pp.pairs;
-    if (ctas > 0x7fffffff) return ACORN_ERR_UNSUPPORTED;
-    return d == 128 ? launch_prefill_f8<128>(pp, num_pages, tokens, ctas, stream) : launch_prefill_f8<64>(pp, num_pages, tokens, ctas, stream);
+    pp.pairs = (nq / nkv + 1) / 2; pp.n_tiles = n_tiles; pp.rows = rows; pp.cap = cap; pp.kvh0 = kvh0; pp.kvhs = kvhs;
+    pp.num_splits = num_splits; pp.k_rows = (bf16*)k_rows; pp.v_rows = (bf16*)v_rows; pp.part_o = part_o; pp.part_lse = part_lse;
+    if ((int64_t)n_tiles * kvhs * pp.pairs > 0x7fffffff || (int64_t)n_tiles * PF8_BM * nq > ((int64_t)1 << 33)) return ACORN_ERR_UNSUPPORTED;
+    return d == 128 ? launch_prefill_f8<128>(pp, tokens, slots, blocks, stream) : launch_prefill_f8<64>(pp, tokens, slots, blocks, stream);
 }
 
 extern "C" int acorn_attention_prefill_f8_error() {

@@ -14,6 +14,8 @@
 // 2 * page bytes, which a bulk copy takes from pages of 8 tokens on.
 #pragma once
 
+#include <cuda_fp16.h>
+
 #include "common.cuh"
 #include "attention_mask.cuh"
 
@@ -48,6 +50,12 @@ __device__ __forceinline__ uint32_t f8_to_f16x2(uint16_t codes) {
     uint32_t r;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(codes));
     return r;
+}
+
+// Two codes as numbers, the low byte's first.
+__device__ __forceinline__ float2 f8_codes2(uint32_t two) {
+    const uint32_t h = f8_to_f16x2((uint16_t)two);
+    return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
 // What the attention kernels over these pages are given.

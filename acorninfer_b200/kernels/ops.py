@@ -151,9 +151,9 @@ class _Sigs:
     acorn_attention_decode_f8 = [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p,
                                  c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p, c_int,
                                  c_int, c_void_p, c_void_p, c_void_p]
-    acorn_attention_prefill_f8 = [c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int,
+    acorn_attention_prefill_f8 = [c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
                                   c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int,
-                                  c_void_p, c_void_p]
+                                  c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]
     acorn_attention_prefill_f8_supported = [c_int, c_int, c_int, c_int]
     acorn_attention_prefill_f8_error = []
     acorn_attention_prefill_f8_set_error_word = [c_void_p]
@@ -1107,6 +1107,21 @@ def f8_tile_tokens(num_heads: int, num_kv_heads: int) -> int:
 F8_MAX_SPLITS = 64
 
 
+F8_PREFILL_SCRATCH = 1 << 30      # bytes of bfloat16 keys and values that a call of ``attention_prefill_f8`` makes at a time
+
+
+@lru_cache(maxsize=4096)
+def prefill_f8_splits(ctas: int, blocks: int, num_sms: int = 148) -> int:
+    """Splits of the keys for ``attention_prefill_f8``: ``ctas`` (tile, pair of heads) with up to ``blocks`` blocks of 128 keys
+    each."""
+    best, best_us = 1, None
+    for s in range(1, min(blocks, 16) + 1):
+        us = -(-ctas * s // num_sms) * (-(-blocks // s) * 2.0 + 4.0) + (3.0 + s if s > 1 else 0.0)
+        if best_us is None or us < best_us:
+            best, best_us = s, us
+    return best
+
+
 @lru_cache(maxsize=4096)
 def decode_f8_splits(tiles: int, num_kv_heads: int, key_bound: int, head_dim: int, num_sms: int = 148) -> int:
     """Splits of the key range for ``attention_decode_f8``."""
@@ -1213,10 +1228,11 @@ def attention_prefill_f8(q: torch.Tensor, q_stride: int, k_pages: torch.Tensor, 
                          block_table: torch.Tensor, page_base: torch.Tensor, row_start: torch.Tensor, row_pos: torch.Tensor,
                          tiles: torch.Tensor, num_tokens: int, num_heads: int, num_kv_heads: int, head_dim: int, scale: float,
                          window: int | None, out: torch.Tensor | None = None, chunk: int | None = None, keep_first: int = 0,
-                         sink32: torch.Tensor | None = None) -> torch.Tensor:
+                         sink32: torch.Tensor | None = None, num_splits: int | None = None) -> torch.Tensor:
     """Causal attention of prompts, or portions of them, over the pages of an 8-bit cache: as ``attention_decode_f8``, in tiles
     of up to 128 tokens (``F8_PREFILL_TILE``).  CTAs start in the order of the list: give the tiles that read the most keys
-    first."""
+    first.  Head sizes 64 and 128 with a positive scale run on the tensor cores, from bfloat16 rows of the keys and values that
+    the call makes in scratch of its own (of at most ``F8_PREFILL_SCRATCH`` bytes or one kv head's)."""
     what = "attention_prefill_f8"
     P, out, stream = _check_f8_attention(what, q, q_stride, k_pages, v_pages, scales, block_table, page_base, row_start, row_pos, tiles,
                                          num_tokens, num_heads, num_kv_heads, head_dim, window, out, chunk, keep_first, sink32)
@@ -1224,11 +1240,34 @@ def attention_prefill_f8(q: torch.Tensor, q_stride: int, k_pages: torch.Tensor, 
         return _attention_f8_plain(q, q_stride, out, k_pages, v_pages, scales, block_table, page_base, row_start, row_pos, tiles,
                                    F8_PREFILL_TILE, num_heads, num_kv_heads, head_dim, P, scale, window, chunk, keep_first, sink32,
                                    stream)
-    _ok(lib().acorn_attention_prefill_f8(q.data_ptr(), q_stride, num_tokens, out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-                                         scales.data_ptr(), k_pages.shape[0], block_table.data_ptr(), page_base.data_ptr(),
-                                         block_table.stride(0), row_start.data_ptr(), row_pos.data_ptr(), tiles.data_ptr(),
-                                         tiles.shape[0], num_heads, num_kv_heads, head_dim, P, float(scale), int(window or 0),
-                                         int(chunk or 0), int(keep_first or 0), _ptr(sink32), stream), what)
+    n, rows, width = tiles.shape[0], block_table.shape[0], block_table.shape[1]
+    if n == 0:
+        return out
+    # the keys of every row that has tiles, as rows of bfloat16, for as many kv heads at a time as the scratch has room for
+    slots, cap = min(rows, n), ((width * P + 127) // 128 + 1) * 128
+    kvhs = max(1, min(num_kv_heads, F8_PREFILL_SCRATCH // (slots * cap * head_dim * 4)))
+    if slots > 65535 or slots * kvhs * cap >= 1 << 31:
+        raise KernelError(f"{what}: {slots} rows of {width} pages are too many for one call")
+    pairs = -(-(num_heads // num_kv_heads) // 2)
+    spans = [v for v in (window, chunk) if v]
+    keys = min([width * P] + [v + F8_PREFILL_TILE + (keep_first or 0) for v in spans])
+    if num_splits is None:
+        num_splits = prefill_f8_splits(n * kvhs * pairs, -(-keys // 128), device_sms(q.device))
+    if not 1 <= num_splits <= F8_MAX_SPLITS:
+        raise KernelError(f"{what}: num_splits must be in 1..{F8_MAX_SPLITS}, got {num_splits}")
+    scratch = torch.empty((2, slots, kvhs, cap, head_dim), dtype=torch.bfloat16, device=q.device)
+    part_o = part_lse = None
+    if num_splits > 1:
+        part_o = torch.empty((num_splits, n, F8_PREFILL_TILE, num_heads, head_dim), dtype=torch.float32, device=q.device)
+        part_lse = torch.empty((num_splits, n, F8_PREFILL_TILE, num_heads), dtype=torch.float32, device=q.device)
+    for first in range(0, num_kv_heads, kvhs):
+        _ok(lib().acorn_attention_prefill_f8(q.data_ptr(), q_stride, num_tokens, out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+                                             scales.data_ptr(), block_table.data_ptr(), page_base.data_ptr(), block_table.stride(0),
+                                             rows, row_start.data_ptr(), row_pos.data_ptr(), tiles.data_ptr(), n, num_heads,
+                                             num_kv_heads, head_dim, P, float(scale), int(window or 0), int(chunk or 0),
+                                             int(keep_first or 0), _ptr(sink32), first, min(kvhs, num_kv_heads - first),
+                                             scratch[0].data_ptr(), scratch[1].data_ptr(), slots, cap, min(cap // 128, 1024), num_splits,
+                                             _ptr(part_o), _ptr(part_lse), stream), what)
     return out
 
 
