@@ -11,7 +11,7 @@
 //               brought to half precision by a power of two per row (their largest entry to 2^14 .. 2^15, so that a bfloat16
 //               entry is exact unless it is 2^-28 of the largest), and both powers of two meet the score in float32.
 //   P = 2^(t + e_v - m)   t the score in units of log2, e_v the exponent of the key's value row, m a reference near the largest
-//               t + e_v so far: the value's power of two rides in the exponent, so that a weight is at most 2^8 (the reference
+//               t + e_v so far: the value's power of two rides in the exponent, so that a weight is at most 2^14 (the reference
 //               moves when it is outgrown by more) in half precision, with 11 bits where bfloat16 would keep 8, whatever the
 //               sizes of the value rows.  Against the reference the common step needs no maximum across lanes, only a vote.
 //   O' += V' P' on value codes as half-precision numbers (a weight's transpose within the warp is one movmatrix); the
@@ -34,7 +34,8 @@ namespace cg = cooperative_groups;
 #define DF8_THREADS (32 * DF8_WARPS + 32)
 #define DF8_CHUNK (16 * DF8_WARPS)
 #define DF8_CLUSTER_MAX 16
-#define DF8_GROW_LOG2 8.f                   // the reference maximum moves when a row's maximum outgrew it by more than this
+#define DF8_GROW_LOG2 14.f                  // the reference maximum moves when a row's maximum outgrew it by more than this
+                                            // (half-precision weights end at 2^16)
 
 __device__ int g_attn_dec_f8_error = 0;
 

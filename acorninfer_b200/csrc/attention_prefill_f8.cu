@@ -15,8 +15,11 @@
 //                  block each: a block's scores pass through the softmax in half the time that one thread a row takes, and
 //                  that time, not the tensor cores' or the exponentials', is what a unit's turn waits for.
 //                  Weights are taken against a reference maximum that both threads of a row share; it moves when either of them
-//                  saw a score beyond it by more than 2^8 (one vote of the unit's 256 threads a block; always so in the first
-//                  block), and only then the two exchange their maxima, read the block again and scale O.
+//                  saw a score beyond it by more than 2^24 (one vote of the unit's 256 threads a block; the first block is looked
+//                  through for its maximum before anything else), and only then the two exchange their maxima, read the
+//                  block again and scale O.  2^24: a weight keeps its 8 bits in bfloat16 whatever its size, and a move costs a unit
+//                  half a block's time again (at 2^8 every third block of 8,192 tokens had one, 595 us; float32 sums of 2^17
+//                  such weights overflow at values of 2^86).
 //      warp 16     producer: Q (once), K and V tiles by TMA into a ring of five.
 //      warp 17     MMA issuer (converged; one elected lane issues): per block j and unit u, O_u += P_u[j] V_j with P from
 //                  tensor memory, then S_u = Q_u K_{j+1}^T into the columns P_u[j] was read from.
@@ -33,7 +36,7 @@
 #define PF8_BN 128
 #define PF8_SLOTS 5
 #define PF8_THREADS 640
-#define PF8_GROW_LOG2 8.0f
+#define PF8_GROW_LOG2 24.0f
 #define PF8_TMEM_COLS 512
 
 __device__ int g_attn_pre_f8_error = 0;
@@ -350,7 +353,29 @@ __global__ void __launch_bounds__(PF8_THREADS, 1) attention_prefill_f8_kernel(co
             float m_ref = -INFINITY, l_run = 0.f;                        // the reference in units of log2
             float scale = p.scale_log2, neg_m = 0.f;                     // what the row's scores are exponentiated with
             bool good = nb > 0;
-            for (int j = 0; j < nb; ++j) {
+            auto refer = [&](float top) {                                // to the larger of the two threads' maxima
+                m_ref = top * p.scale_log2;                              // the scale is positive
+                scale = pf8_row_scale(p.scale_log2, m_ref);
+                neg_m = -(top * scale);
+            };
+            if (good) {
+                const bool got = mbar_wait(s_full, 0);
+                if (!got) tc_fail(&g_attn_pre_f8_error, 5, ACORN_KERNEL_ATTN_PREFILL_F8);
+                tc_fence_after();
+                const int block0 = blocks.key0(j0), key0 = block0 + 64 * half;
+                float s[32], top = -INFINITY;
+#pragma unroll 1
+                for (int h = 0; h < 2; ++h) {
+                    tmem_ld32(my_s + 32 * h, s);
+                    pf8_mask(s, last_seen - key0 - 32 * h, first_seen - key0 - 32 * h, p.mask.keep - key0 - 32 * h);
+                    top = pf8_max(s, top);
+                }
+                *mine = top;
+                good = !unit_any(u, !got);                               // (a wait that gave up makes the whole unit stop)
+                top = fmaxf(top, *other);
+                if (top > -INFINITY) refer(top);
+            }
+            for (int j = 0; j < nb && good; ++j) {
                 // S of block j is complete; so is P V of block j-1, issued before it: O is stable
                 bool got = mbar_wait(s_full, j & 1);
                 if (!got) tc_fail(&g_attn_pre_f8_error, 6, ACORN_KERNEL_ATTN_PREFILL_F8);
@@ -369,9 +394,8 @@ __global__ void __launch_bounds__(PF8_THREADS, 1) attention_prefill_f8_kernel(co
                     psum += pf8_exp_pack(s, scale, neg_m, w + 16 * h);
                 }
                 const float mx = top * p.scale_log2;                     // the scale is positive
-                // (a wait that gave up makes the whole unit stop, through the same vote)
                 if (unit_any(u, !got || mx > m_ref + PF8_GROW_LOG2)) {
-                    *mine = got ? top : INFINITY;
+                    *mine = top;
                     good = !unit_any(u, !got);
                     if (!good) break;
                     const float both = fmaxf(top, *other), mb = both * p.scale_log2;
@@ -379,9 +403,7 @@ __global__ void __launch_bounds__(PF8_THREADS, 1) attention_prefill_f8_kernel(co
                     if (mb > m_ref + PF8_GROW_LOG2) {
                         corr = fast_exp2(m_ref - mb);                    // m_ref = -inf: 0
                         l_run *= corr;
-                        m_ref = mb;
-                        scale = pf8_row_scale(p.scale_log2, mb);
-                        neg_m = -(both * scale);
+                        refer(both);
                     }
                     psum = 0.f;
 #pragma unroll
