@@ -79,6 +79,7 @@ def main(argv=None) -> int:
     p.add_argument("--random-preset", default=None, help="the same from a model's published sizes: " + ", ".join(sorted(PRESETS)))
     p.add_argument("--device", default="cuda:0")
     p.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    p.add_argument("--kv-dtype", default=None, choices=["float8"], help="keep keys and values in 8 bits (default: as --dtype)")
     p.add_argument("--num-blocks", type=int, default=1024)
     p.add_argument("--page-size", type=int, default=16)
     p.add_argument("--max-running", type=int, default=8)
@@ -96,7 +97,7 @@ def main(argv=None) -> int:
         p.error("give exactly one of --model-dir, --random-config and --random-preset")
 
     kw = dict(dtype=args.dtype, device=args.device, num_blocks=args.num_blocks, page_size=args.page_size,
-              max_requests=args.max_running,
+              max_requests=args.max_running, kv_dtype=args.kv_dtype,
               max_step_tokens=max(8192, args.chunked_budget or 0, (args.prompt_range or [0, args.in_tokens])[1]))
     if args.model_dir is not None:
         print(f"loading {args.model_dir} -> {args.device} ({args.dtype}) ...")

@@ -4,7 +4,8 @@ state of fixed size in slots, and the bookkeeping of who holds what.
 Layers are sorted into *groups* by what they need (``KVNeeds.group_key``: head count,
 head size, all keys or a window of them).  A group has a page pool of its own and one
 storage tensor ``[layers_in_group, 2, num_pages, kv_heads, page_size, head_dim]`` (1 instead of 2 for
-groups that keep no separate values): a page
+groups that keep no separate values; of an 8-bit group the codes, its rows' powers of two lie in
+tensors ``[num_pages, kv_heads, page_size, 2]`` beside it, one a layer): a page
 id names the same page in every layer of its group.  A request has one block table per
 group; the token at position p lives in ``table[p // page_size - page_base]``, slot
 ``p % page_size``.  ``page_base`` counts pages given back at the front of a windowed
@@ -38,6 +39,7 @@ class CacheGroup:
     pool: IdPool
     storage: object = None              # torch tensor [len(entries), 2, pages, nkv, P, d] or None
     value_storage: object = None        # [len(entries), pages, nkv, P, dv] where values have a width of their own
+    scales: list = field(default_factory=list)   # per layer [pages, nkv, P, 2] float8_e8m0fnu in an 8-bit group
 
     @property
     def window(self) -> int | None:
@@ -105,8 +107,15 @@ class CacheManager:
             for g in self.groups:
                 n = g.needs
                 own_values = n.values and n.value_width != n.head_dim
-                g.storage = torch.zeros((len(g.entries), 2 if (n.values and not own_values) else 1, g.pool.total + 1,
-                                         n.num_kv_heads, page_size, n.head_dim), dtype=n.dtype or dtype, device=device)
+                shape = (len(g.entries), 2 if (n.values and not own_values) else 1, g.pool.total + 1, n.num_kv_heads, page_size, n.head_dim)
+                if n.eight_bit:
+                    if own_values or not n.values:
+                        raise ValueError("an 8-bit cache keeps keys and values of one width")
+                    g.storage = torch.zeros(shape, dtype=torch.uint8, device=device).view(n.dtype)
+                    g.scales = [torch.zeros((*shape[2:5], 2), dtype=torch.uint8, device=device).view(torch.float8_e8m0fnu)
+                                for _ in g.entries]
+                    continue
+                g.storage = torch.zeros(shape, dtype=n.dtype or dtype, device=device)
                 if own_values:
                     g.value_storage = torch.zeros((len(g.entries), g.pool.total + 1, n.num_kv_heads, page_size,
                                                    n.value_width), dtype=n.dtype or dtype, device=device)
@@ -125,15 +134,20 @@ class CacheManager:
             return st[li, 0], self.groups[gi].value_storage[li]
         return st[li, 0], (st[li, 1] if st.shape[1] > 1 else None)
 
+    def kv_scales(self, entry: int):
+        """The powers of two of an 8-bit entry's rows [num_pages, nkv, P, 2]; None for other caches."""
+        gi, li = self.entry_group[entry]
+        return self.groups[gi].scales[li] if self.groups[gi].scales else None
+
     def group_of(self, entry: int) -> int:
         return self.entry_group[entry][0]
 
     def bytes_per_token(self) -> int:
         total = 0
         for g in self.groups:
-            width = 2 if g.storage is None else g.storage.element_size()
+            width = (1 if g.needs.eight_bit else 2) if g.storage is None else g.storage.element_size()
             per_head = g.needs.head_dim + (g.needs.value_width if g.needs.values else 0)
-            total += len(g.entries) * g.needs.num_kv_heads * per_head * width
+            total += len(g.entries) * g.needs.num_kv_heads * (per_head * width + (2 if g.needs.eight_bit else 0))
         return total
 
     # ------------------------------------------------------------------ requests

@@ -5,7 +5,7 @@
 ``--temperature`` (0 = greedy), ``--top-p``, ``--top-k`` (0 = disabled); and the engine's
 (``acorninfer/bench.py:107-112``): ``--num-blocks``, ``--page-size``, ``--max-running``,
 ``--watermark-blocks``.  Added: ``--prompt-ids`` (comma-separated ids, no tokenizer
-needed), ``--seed``, ``--dtype``, ``--chunked-budget``.
+needed), ``--seed``, ``--dtype``, ``--kv-dtype``, ``--chunked-budget``.
 ``random-model`` writes a model folder with seeded random weights from a config.json.
 """
 
@@ -20,6 +20,7 @@ import time
 def _add_engine_options(p: argparse.ArgumentParser) -> None:
     p.add_argument("--device", default="cuda:0")
     p.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    p.add_argument("--kv-dtype", default=None, choices=["float8"], help="keep keys and values in 8 bits (default: as --dtype)")
     p.add_argument("--num-blocks", type=int, default=1024)
     p.add_argument("--page-size", type=int, default=16)
     p.add_argument("--max-running", type=int, default=8)
@@ -72,7 +73,8 @@ def main(argv=None) -> int:
     t0 = time.perf_counter()
     engine = build_engine(args.model_dir, dtype=args.dtype, device=args.device, num_blocks=args.num_blocks,
                           page_size=args.page_size, max_running=args.max_running,
-                          watermark_blocks=args.watermark_blocks, chunked_budget=args.chunked_budget)
+                          watermark_blocks=args.watermark_blocks, chunked_budget=args.chunked_budget,
+                          kv_dtype=args.kv_dtype)
     print(f"model loaded in {time.perf_counter() - t0:.1f}s", file=sys.stderr)
     t0 = time.perf_counter()
     ids = generate_with_engine(engine, [prompt_ids], max_new_tokens=args.max_new_tokens,

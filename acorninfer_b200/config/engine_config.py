@@ -5,7 +5,7 @@ Names and meanings follow the reference where it has them
 ``num_blocks`` pages in the pool of every cache group, ``page_size`` tokens a page,
 ``max_running`` requests in a step at most, ``watermark_blocks`` pages that admission
 leaves free, ``chunked_budget`` the most tokens one step may carry (``None``: whole
-prompts).  The reference's back-end switches have no counterpart: there is one back end.
+prompts).  ``kv_dtype`` "float8" keeps keys and values in 8 bits (None: in ``dtype``).  The reference's back-end switches have no counterpart: there is one back end.
 """
 
 from __future__ import annotations
@@ -27,11 +27,16 @@ class EngineConfig:
     chunked_budget: int | None = None
     max_step_tokens: int = 8192      # capacity of the step workspace (tokens in one step)
     decode_graph: bool = True        # replay captured CUDA graphs for all-decode steps
+    kv_dtype: str | None = None      # what the cache keeps keys and values in: None (as ``dtype``) or "float8"
 
     def __post_init__(self) -> None:
         if self.dtype not in DTYPE_NAMES:
             raise ValueError(f"dtype must be one of {sorted(DTYPE_NAMES)}, got {self.dtype!r}")
         object.__setattr__(self, "dtype", DTYPE_NAMES[self.dtype])
+        if self.kv_dtype not in (None, "float8"):
+            raise ValueError(f"kv_dtype must be None or 'float8', got {self.kv_dtype!r}")
+        if self.kv_dtype is not None and self.dtype != "bfloat16":
+            raise ValueError(f"kv_dtype {self.kv_dtype!r} goes with dtype 'bfloat16', not {self.dtype!r}")
         if self.num_blocks < 1:
             raise ValueError(f"num_blocks must be >= 1, got {self.num_blocks}")
         if self.page_size < 1 or self.page_size > 256 or self.page_size & (self.page_size - 1):

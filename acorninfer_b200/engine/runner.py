@@ -36,6 +36,18 @@ from .batch import (PREFILL_GRAPH_MAX_TOKENS, BatchError, StepEntry, StepWorkspa
                     plan_step, prefill_bucket, prefill_buckets, validate_entries)
 
 _DTYPES = {"bfloat16": torch.bfloat16, "float32": torch.float32}
+_KV_DTYPES = {None: None, "float8": torch.float8_e4m3fn}
+
+
+def _dtypes(kw: dict) -> tuple[torch.dtype, torch.dtype | None]:
+    """The activations' and the cache's element type (None: the activations') that a runner's options ask for."""
+    dtype, kv = kw.get("dtype", "bfloat16"), kw.get("kv_dtype")
+    dtype = _DTYPES[dtype] if isinstance(dtype, str) else dtype
+    if kv not in _KV_DTYPES:
+        raise ValueError(f"kv_dtype must be one of {sorted(k for k in _KV_DTYPES if k)} or None, got {kv!r}")
+    if kv is not None and dtype != torch.bfloat16:
+        raise ValueError(f"an 8-bit cache goes with bfloat16 activations, not {dtype}")
+    return dtype, _KV_DTYPES[kv]
 
 
 MAX_GRAPHS = 384
@@ -45,14 +57,16 @@ class ModelRunner:
     def __init__(self, config: ModelConfig, tensors: dict[str, torch.Tensor] | None, *, dtype: str = "bfloat16",
                  device: str = "cuda:0", num_blocks: int = 1024, page_size: int = 16, max_requests: int = 64,
                  max_step_tokens: int = 8192, decoder: Decoder | None = None, decode_graph: bool = True,
-                 workspace_ints: int = 1 << 20):
+                 workspace_ints: int = 1 << 20, kv_dtype: str | None = None):
+        """``kv_dtype``: None keeps keys and values in the activations' type; "float8" keeps them as e4m3 codes with a power of
+        two a row (``ops.qk_rope_kv_f8``), half of bfloat16's bytes, for models whose layers are all of attention."""
         self.config = config
-        self.dtype = _DTYPES[dtype] if isinstance(dtype, str) else dtype
+        self.dtype, self.kv_dtype = _dtypes({"dtype": dtype, "kv_dtype": kv_dtype})
         self.device = torch.device(device)
         ops.lib()      # fails here, loudly, if there is no device or no compiled kernels
         torch.cuda.set_device(self.device)
         self.spec = spec_for(config)
-        self.decoder = decoder or Decoder(self.spec, self.dtype, self.device, page_size)
+        self.decoder = decoder or Decoder(self.spec, self.dtype, self.device, page_size, self.kv_dtype)
         if tensors is not None:
             self.decoder.bind(tensors)
         kv_needs, state_needs = self.decoder.cache_needs()
@@ -80,10 +94,9 @@ class ModelRunner:
     @classmethod
     def from_model_dir(cls, model_dir: str | Path, **kw) -> "ModelRunner":
         config = load_config(model_dir)
-        dtype = kw.get("dtype", "bfloat16")
-        tdtype = _DTYPES[dtype] if isinstance(dtype, str) else dtype
+        tdtype, kv_dtype = _dtypes(kw)
         device = kw.get("device", "cuda:0")
-        probe = Decoder(spec_for(config), tdtype, device, kw.get("page_size", 16))
+        probe = Decoder(spec_for(config), tdtype, device, kw.get("page_size", 16), kv_dtype)
         tensors = load_tensors(model_dir, probe.expected_tensors(), tdtype, device, probe.ignorable_tensors())
         probe.bind(tensors)
         return cls(config, None, decoder=probe, **kw)
@@ -92,10 +105,9 @@ class ModelRunner:
     def from_random(cls, config: ModelConfig, seed: int, sigma: float = 0.02, sigma_norm: float = 0.0,
                     **kw) -> "ModelRunner":
         """Random weights drawn straight on the device (no folder): for benchmarks of large sizes."""
-        dtype = kw.get("dtype", "bfloat16")
-        tdtype = _DTYPES[dtype] if isinstance(dtype, str) else dtype
+        tdtype, kv_dtype = _dtypes(kw)
         device = kw.get("device", "cuda:0")
-        probe = Decoder(spec_for(config), tdtype, device, kw.get("page_size", 16))
+        probe = Decoder(spec_for(config), tdtype, device, kw.get("page_size", 16), kv_dtype)
         tensors = random_state(probe.expected_tensors(), seed, sigma, sigma_norm, torch.bfloat16, device)
         if tdtype == torch.float32:
             tensors = {k: v.float() for k, v in tensors.items()}

@@ -19,12 +19,13 @@ from .sampling.params import SamplingParams
 
 def build_engine(model_dir: str | Path, *, dtype: str = "bfloat16", device: str = "cuda:0", num_blocks: int = 1024,
                  page_size: int = 16, max_running: int = 8, watermark_blocks: int = 8,
-                 chunked_budget: int | None = None, warm_up: bool = False) -> Engine:
+                 chunked_budget: int | None = None, warm_up: bool = False, kv_dtype: str | None = None) -> Engine:
     """``warm_up``: run throw-away steps now (``ModelRunner.warm_up``) so that the first requests do not
-    pay for kernels loaded and graphs captured at first use; worth it for an engine that serves."""
+    pay for kernels loaded and graphs captured at first use; worth it for an engine that serves.  ``kv_dtype`` "float8":
+    keys and values in 8 bits."""
     cfg = EngineConfig(model_dir=str(model_dir), device=device, dtype=dtype, num_blocks=num_blocks,
                        page_size=page_size, max_running=max_running, watermark_blocks=watermark_blocks,
-                       chunked_budget=chunked_budget)
+                       chunked_budget=chunked_budget, kv_dtype=kv_dtype)
     engine = Engine.from_config(cfg)
     if warm_up:
         engine.runner.warm_up()

@@ -56,6 +56,26 @@ STEP_ARRAYS = {
     "attention.q_tiles_small": lambda plan: _tiles(plan, 2, LARGE_MIN, Q_TILE),
 }
 
+# The same for an 8-bit cache (``paged_attention_f8``): single tokens, tiles of the rows of a few tokens (as many tokens a tile as the
+# kernel's sixteen query rows hold), tiles of 128 of the longer ones.
+F8_LARGE_MIN = 32
+
+
+def f8_step_arrays(nq: int, nkv: int) -> dict:
+    step = ops.f8_tile_tokens(nq, nkv)
+
+    def large(plan):
+        t = _tiles(plan, F8_LARGE_MIN, None, ops.F8_PREFILL_TILE)
+        keys = plan.row_pos[t[:, 0]] + np.minimum(t[:, 1] + ops.F8_PREFILL_TILE, np.asarray(plan.row_lens, np.int32)[t[:, 0]])
+        return np.ascontiguousarray(t[np.argsort(-keys, kind="stable")])
+
+    return {
+        "attention.f8_single": lambda plan: _tiles(plan, 1, 2, 1),
+        f"attention.f8_short{step}": lambda plan: _tiles(plan, 2, F8_LARGE_MIN, step),
+        "attention.f8_large": large,
+    }
+
+
 sm_count = ops.device_sms
 
 
@@ -182,6 +202,25 @@ def _decode(qkv, inputs, group, cache, nq, nkv, d, P, scale, window, bound, n, w
     return ops.attention_decode(qkv, qkv.stride(0), cache.k_pages, cache.v_pages, group.block_table, group.page_base, inputs.token_row,
                                 inputs.positions, inputs.num_tokens, nq, nkv, d, scale, window, splits, token_list=token_list, out=out,
                                 **mask)
+
+
+def paged_attention_f8(q: torch.Tensor, inputs, group, cache, nq: int, nkv: int, d: int, scale: float, window: int | None,
+                       chunk: int | None = None, keep_first: int = 0, sink32: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of all tokens of the step over an 8-bit cache; ``q`` [T, >= nq d].  Rows of a few tokens go to the split-K
+    kernel, single ones in a launch of their own, longer rows to the prefill kernel, all into one output."""
+    T, x, hx = inputs.num_tokens, inputs.extra, inputs.plan.extra
+    out = torch.empty((T, nq * d), dtype=q.dtype, device=q.device)
+    args = (q, q.stride(0), cache.k_pages, cache.v_pages, cache.scales, group.block_table, group.page_base, inputs.row_start,
+            inputs.row_pos)
+    rest = (T, nq, nkv, d, scale, window)
+    mask = {"out": out, "chunk": chunk, "keep_first": keep_first, "sink32": sink32}
+    if hx["attention.f8_large"].shape[0]:
+        ops.attention_prefill_f8(*args, x["attention.f8_large"], *rest, **mask)
+    step = ops.f8_tile_tokens(nq, nkv)
+    for name, most in ((f"attention.f8_short{step}", step), ("attention.f8_single", 1)):
+        if hx[name].shape[0]:
+            ops.attention_decode_f8(*args, x[name], *rest, tile_tokens=most, **mask)
+    return out
 
 
 def _key_bound(table_keys: int, window: int | None, chunk: int | None, keep_first: int) -> int:

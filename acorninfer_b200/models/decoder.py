@@ -32,14 +32,15 @@ class EntryCache:
     v_pages: torch.Tensor | None
     write: bool
     state: torch.Tensor | None
+    scales: torch.Tensor | None = None      # an 8-bit cache's powers of two (``CacheManager.kv_scales``)
 
 
 class Decoder:
-    def __init__(self, spec: ModelSpec, dtype: torch.dtype, device, page_size: int = 16):
+    def __init__(self, spec: ModelSpec, dtype: torch.dtype, device, page_size: int = 16, kv_dtype: torch.dtype | None = None):
         self.spec = spec
         self.dtype = dtype
         self.device = torch.device(device)
-        self.ctx = BuildContext(dtype=dtype, device=self.device, page_size=page_size)
+        self.ctx = BuildContext(dtype=dtype, device=self.device, page_size=page_size, kv_dtype=kv_dtype)
         for name, ps in spec.positions.items():
             self.ctx.positions[name] = build_part(POSITION_ENCODINGS, ps, self.ctx)
         self.blocks = []
@@ -139,6 +140,9 @@ class Decoder:
                     kv[e.reads_cache_of] = replace(owner, window=needs.kv.window)
                 continue
             if needs.kv is not None:
+                if self.ctx.kv_dtype is not None and needs.kv.dtype != self.ctx.kv_dtype:
+                    raise ValueError(f"schedule entry {i} ({type(self.blocks[e.layer].mixer).__name__}) keeps keys and values that "
+                                     f"have no form in {self.ctx.kv_dtype}")
                 kv[i] = needs.kv
             if needs.state is not None:
                 state[i] = needs.state
@@ -155,10 +159,10 @@ class Decoder:
             owner = i if e.reads_cache_of is None else e.reads_cache_of
             if owner in manager.entry_group:
                 k, v = manager.kv_pages(owner)
-                group = manager.group_of(owner)
+                group, scales = manager.group_of(owner), manager.kv_scales(owner)
             else:
-                k = v = group = None
-            out.append(EntryCache(i, group, k, v, e.reads_cache_of is None, manager.state.get(i)))
+                k = v = group = scales = None
+            out.append(EntryCache(i, group, k, v, e.reads_cache_of is None, manager.state.get(i), scales))
         for where, stages in self.stages.items():
             for n, st in enumerate(stages):
                 if f"{where}.{n}" in manager.state:

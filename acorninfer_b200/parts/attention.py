@@ -127,6 +127,19 @@ class Attention(Mixer):
         self.plain = (not (values_from_keys or head_gate or bias or conv_taps or self.norm_after or self.sink or softcap
                            or q_temp is not None or self.norm_rows or self.unit_sink)
                       and self.norm_weights and magnitude == 1.0 and self.dv == head_dim)
+        self.eight_bit = ctx.kv_dtype == ops.F8
+        if self.eight_bit:
+            refused = [what for what, has in (
+                ("value heads of another width", self.dv != self.d), ("values taken from the keys", values_from_keys),
+                ("a convolution over time", bool(conv_taps)), ("a distance penalty", slope_exponent is not None),
+                ("capped scores", bool(softcap)), ("a q/k norm after the rotation", self.norm_after),
+                ("a q/k norm over whole rows", self.norm_rows), ("a query temperature", q_temp is not None),
+                (f"heads of {self.d} entries (a multiple of 8, up to {ops.F8_MAX_HEAD})", self.d % 8 != 0 or self.d > ops.F8_MAX_HEAD),
+                (f"{getattr(self.position, 'rotary_dim', 0)} rotated entries (a multiple of 16)", self.position is not None
+                 and not self.position.interleaved and self.position.rotary_dim % 16 != 0)) if has]
+            if refused:
+                raise ValueError(f"attention over an 8-bit cache does not go with {', '.join(refused)}")
+            self.plain = False
         self.gate_col = (self.nq + self.nkv) * self.d + (0 if values_from_keys else self.nkv * self.dv)
         self.w_qkv = self.w_o = self.q_norm32 = self.k_norm32 = None
 
@@ -208,14 +221,14 @@ class Attention(Mixer):
             self.slopes32 = self.slopes32.to(self.w_o.device)
 
     def cache_needs(self):
-        kv = KVNeeds(self.nkv, self.d, self.window, chunk=self.chunk, keep_first=self.keep_first,
+        kv = KVNeeds(self.nkv, self.d, self.window, dtype=self.ctx.kv_dtype, chunk=self.chunk, keep_first=self.keep_first,
                      value_dim=None if self.dv == self.d else self.dv)
         # the convolutions' memory: the last taps - 1 rows as projected (with their biases), float32
         state = StateNeeds(((self.taps - 1) * self.channels,)) if self.taps and self.taps > 1 and self.channels else None
         return CacheNeeds(kv=kv, state=state)
 
     def step_arrays(self):
-        return attn_kernels.STEP_ARRAYS
+        return attn_kernels.f8_step_arrays(self.nq, self.nkv) if self.eight_bit else attn_kernels.STEP_ARRAYS
 
     def fusable(self, num_rows):
         # (the options only change what runs between the two products, which take the fused forms either way)
@@ -259,6 +272,29 @@ class Attention(Mixer):
                                              sink32=self.sink32, softcap=self.softcap)
         return heads if out is None else ops.head_gate(heads, None, self.nq, 1.0, out=out)
 
+    def _inner_f8(self, x, inputs, cache, out_scale, out):
+        """``inner`` over an 8-bit cache."""
+        g, pos = inputs.groups[cache.group], self.position
+        proj = ops.linear(x, self.w_qkv, out_dtype=self.ctx.dtype, inputs=inputs)
+        inv_freq = pos.inv_freq if pos is not None else _no_freq(self.ctx.device)
+        rot, interleaved = (pos.rotary_dim, pos.interleaved) if pos is not None else (0, False)
+        eps, magnitude = self.qk_norm_eps if self.qk_norm_eps is not None else 0.0, getattr(pos, "magnitude", 1.0)
+        if cache.write:
+            q = ops.qk_rope_kv_f8(proj, self.q_norm32, self.k_norm32, inv_freq, inputs.positions, inputs.token_row, g.block_table,
+                                  g.page_base, cache.k_pages, cache.v_pages, cache.scales, self.nq, self.nkv, self.d, rot, interleaved,
+                                  eps, bias32=self.bias32, magnitude=magnitude)
+        else:                                 # another run's cache is read: the queries alone, in place
+            if self.bias:
+                raise ValueError("attention: biased projections need a cache of the run's own")
+            q = proj
+            ops.qk_rope_kv(proj, self.q_norm32, self.k_norm32, inv_freq, inputs.positions, inputs.token_row, g.block_table, g.page_base,
+                           None, None, self.nq, self.nkv, self.d, rot, interleaved, eps, write_kv=False, magnitude=magnitude)
+        heads = attn_kernels.paged_attention_f8(q, inputs, g, cache, self.nq, self.nkv, self.d, self.scale, self.window,
+                                                chunk=self.chunk, keep_first=self.keep_first, sink32=self.sink32)
+        if self.head_gate or out_scale != 1.0 or out is not None:
+            return ops.head_gate(heads, proj[:, self.gate_col:] if self.head_gate else None, self.nq, out_scale, out=out)
+        return heads
+
     state_base = 0
     w_in = None            # the projection of x where its product may be made by the caller (``inner(proj=...)``)
 
@@ -268,6 +304,8 @@ class Attention(Mixer):
         ``fused``: the layer's other products fuse."""
         if self.norm_rows:
             return self._inner_norm_rows(x, inputs, cache, out_scale, out, proj)
+        if self.eight_bit:
+            return self._inner_f8(x, inputs, cache, out_scale, out)
         g = inputs.groups[cache.group]
         pos = self.position
         rows = x.x.shape[0] if isinstance(x, ops.NormedRows) else x.shape[0]

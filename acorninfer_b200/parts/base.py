@@ -118,6 +118,7 @@ class BuildContext:
     device: torch.device
     page_size: int
     positions: dict[str, "PositionEncoding"] = field(default_factory=dict)
+    kv_dtype: torch.dtype | None = None      # element type that keys and values are asked to be kept in (None: ``dtype``)
 
 
 # --------------------------------------------------------------------------- cache needs
@@ -129,7 +130,8 @@ class KVNeeds:
     an integer w: a query at position p reads keys p-w+1 .. p.  ``chunk`` c: a query reads the keys of
     its own block of c positions only (blocks counted from position 0).  ``keep_first`` n: the
     request's first n keys stay readable whatever the window (the pages of such a cache are all kept).
-    ``dtype`` None: the engine's activation dtype.  ``values`` False: one row per token and kv head only
+    ``dtype`` None: the engine's activation dtype; ``torch.float8_e4m3fn``: the 8-bit cache, whose rows have a power of two
+    each beside their codes (``kernels.ops.qk_rope_kv_f8``).  ``values`` False: one row per token and kv head only
     (a mixer whose values are a function of its key rows, such as attention through a cached latent).
     ``value_dim``: width of a value row where it differs from ``head_dim`` (values then lie in a
     tensor of their own)."""
@@ -147,6 +149,10 @@ class KVNeeds:
     def group_key(self) -> tuple:
         return ("kv", self.num_kv_heads, self.head_dim, self.window, self.dtype, self.values, self.chunk,
                 self.keep_first, self.value_width)
+
+    @property
+    def eight_bit(self) -> bool:
+        return self.dtype == torch.float8_e4m3fn
 
     @property
     def value_width(self) -> int:
