@@ -1,6 +1,6 @@
 // Attention of few tokens a row over the pages of the 8-bit cache (f8_cache.cuh), head sizes 64 and 128: split-K flash decoding.
 //
-// One CTA per (tile, kv head, split).  A tile is up to 16 / rep tokens of one row (rep = nq / nkv query heads share a kv head);
+// A tile is up to 16 / rep tokens of one row (rep = nq / nkv query heads share a kv head);
 // its (token, head) pairs are its query rows, so the tokens of a tile read their row's pages together.
 // A producer warp brings the codes by TMA (swizzled; a box is the keys and the values of one page and head, through a map whose
 // third dimension is the distance between the two page tensors) and their exponents by asynchronous copies into a ring of
@@ -20,8 +20,14 @@
 // entries in a product over them is free (Q is laid out the same way), and so is the order of the output's rows.
 // Codes of keys that no query of the tile reads are replaced by zeros (a slot that was never written may hold anything).
 //
-// The warps are merged through shared memory, the splits of a (tile, kv head) by a thread-block cluster through
-// distributed shared memory (2 to 8, or 16 of them), more by a second kernel through scratch.
+// Which keys a CTA takes:
+//   splits         one (tile, kv head, split) a CTA; the splits of a (tile, kv head), 2 to 8 or 16, are a thread-block cluster
+//                  that joins them through distributed shared memory: one launch, for calls of little work;
+//   even shares    as many CTAs as the device holds at once share all the chunks of 64 keys of all (tile, kv head) pairs out evenly,
+//                  in order, so that a CTA walks from pair to pair: nobody waits for the longest row or for a last wave of few CTAs, and
+//                  the codes of the next pair are on their way while the warps finish one (a CTA's start and end cost some 5
+//                  us).  A pair that several CTAs had parts of is joined by a second, small kernel.  64 rows of 4,096 keys: 128 us
+//                  whole, 114 in the best number of splits; figures of the shares below.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
@@ -39,25 +45,33 @@ namespace cg = cooperative_groups;
 
 __device__ int g_attn_dec_f8_error = 0;
 
+#define DF8_SHARE_TILES 256                 // tiles that a CTA keeps the sizes of for the even shares
+#define DF8_SHARE_MIN 4                     // chunks that a share has at least
+
 struct DecodeF8Params {
     F8AttnParams a;
-    int tile_tokens, num_splits, cluster_merge;     // tile_tokens: the most tokens a tile holds
+    int n_tiles, tile_tokens, num_splits;           // tile_tokens: the most tokens a tile holds; num_splits 0: even shares
     int joint, v_first;       // one box brings keys and values (the tensor at the lower address first), else two do
-    float* part_o;            // [n_tiles, nkv, splits, 16, D]  (more splits than a cluster merges)
-    float* part_lse;          // [n_tiles, nkv, splits, 16]
+    // even shares: what the join needs
+    float* part_o;            // [CTAs, 2, 8 NH, D]: the part that a CTA's share begins with, and the one that it ends with
+    float* part_lse;          // [CTAs, 2, 8 NH]
+    int4* plan;               // [n_tiles + 1]: chunks of the tiles before (of one kv head), chunks, first token, tokens; the last: chunks a share
 };
 
 template <int D, int NH> struct DecodeF8 {
-    static constexpr int STAGES = D == 128 ? 4 : 8;
+    static constexpr int ROWS = 8 * NH;
+    static constexpr int STAGES = D == 128 ? 3 : 6;
     static constexpr int ROWS_BYTES = DF8_CHUNK * D;                  // the codes of a stage's keys (or values)
     static constexpr int STAGE_BYTES = 2 * ROWS_BYTES;
     static constexpr int SCALE_BYTES = 2 * DF8_CHUNK;
     static constexpr int RECV_ROW = D + 4;                            // floats a received partial row takes: the output, then its log-sum
     static constexpr int RING = STAGES * STAGE_BYTES;
-    static constexpr int MERGE = DF8_WARPS * 8 * NH * (2 + D) * 4;
-    static constexpr int BARS = RING > MERGE ? RING : MERGE;          // offsets in shared memory
+    static constexpr int MERGE_BYTES = DF8_WARPS * ROWS * (2 + D) * 4;
+    static constexpr int MERGE = RING;                                // offsets in shared memory
+    static constexpr int BARS = MERGE + MERGE_BYTES;
     static constexpr int SCALES = BARS + 2 * STAGES * 8;
-    static constexpr int RECV = SCALES + STAGES * SCALE_BYTES;
+    static constexpr int RECV = SCALES + STAGES * SCALE_BYTES;        // received rows of a cluster, or the sizes of the tiles
+    static constexpr int SHARES = (DF8_SHARE_TILES + 4) * 4 + DF8_SHARE_TILES * 16;       // chunks before a tile; row, first token, tokens, position
     // byte offset of the 16-byte piece `seg` of row `row` of a stage (boxes of 2^log_box keys, then as many values), as the
     // TMA's swizzle places it
     static __device__ __forceinline__ uint32_t at(int row, int seg) {
@@ -97,11 +111,64 @@ __device__ __forceinline__ float column_sum(float v) {
     return v + __shfl_xor_sync(0xffffffffu, v, 16);
 }
 
-template <int D, int NH>
+// What a CTA needs to know of a tile.
+struct F8Tile {
+    int r, tok0, n_q, pos0, hi, lo, base_key, nkb, n_chunks;
+    __device__ __forceinline__ F8Tile(const DecodeF8Params& dp, int ti) {
+        const F8AttnParams& p = dp.a;
+        r = p.tiles[2 * ti];
+        const int q0 = p.tiles[2 * ti + 1];
+        tok0 = p.row_start[r] + q0;
+        n_q = max(0, min(dp.tile_tokens, p.row_start[r + 1] - tok0));
+        pos0 = p.row_pos[r] + q0;
+        keys(p);
+    }
+    __device__ __forceinline__ F8Tile(const F8AttnParams& p, const int4& v) : r(v.x), tok0(v.y), n_q(v.z), pos0(v.w) { keys(p); }
+    __device__ __forceinline__ void keys(const F8AttnParams& p) {
+        hi = pos0 + n_q;                                          // keys < hi are read by the tile
+        lo = mask_lo(p.mask, pos0);                               // the first query's rule starts first
+        base_key = lo & ~(DF8_CHUNK - 1);                         // chunks start at multiples of 64 keys
+        // the kept first keys, where the rule's range starts beyond them, are chunks of their own in front
+        nkb = (p.mask.keep > 0 && base_key > 0) ? min((p.mask.keep + DF8_CHUNK - 1) / DF8_CHUNK, base_key / DF8_CHUNK) : 0;
+        n_chunks = n_q > 0 ? nkb + (hi - base_key + DF8_CHUNK - 1) / DF8_CHUNK : 0;
+    }
+    __device__ __forceinline__ int key0(int c) const { return c < nkb ? c * DF8_CHUNK : base_key + (c - nkb) * DF8_CHUNK; }
+};
+
+// The parts of (tile, kv head) pairs that a CTA takes, one after the other.
+struct F8Walk {
+    const int* before;        // even shares: chunks of the tiles before each, and the tiles (shared memory)
+    const int4* tiles;
+    int n_tiles, nkv, ti, kvh, c0, c1;
+    int64_t at, end;          // of the share, in chunks of all pairs
+    // even shares: units are ordered by tile, then kv head, then chunk
+    __device__ __forceinline__ bool next() {
+        if (at >= end) return false;
+        int a = 0, b = n_tiles;                                   // the last tile that starts at or before `at`
+        while (b - a > 1) {
+            const int m = (a + b) >> 1;
+            if ((int64_t)before[m] * nkv <= at) a = m; else b = m;
+        }
+        ti = a;
+        const int n = before[a + 1] - before[a];                  // > 0: tiles without chunks start where the next one does
+        const int64_t in = at - (int64_t)before[a] * nkv;
+        kvh = (int)(in / n);
+        c0 = (int)(in - (int64_t)kvh * n);
+        c1 = (int)min((int64_t)n, c0 + (end - at));
+        at += c1 - c0;
+        return true;
+    }
+};
+
+// Meets the compute warps.
+__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, %0;" :: "n"(32 * DF8_WARPS) : "memory"); }
+
+template <int D, int NH, bool SHARES>
 __global__ void __launch_bounds__(DF8_THREADS, NH == 1 ? 3 : 2) attention_decode_f8_kernel(const __grid_constant__ CUtensorMap map_k,
                                                                          const __grid_constant__ CUtensorMap map_v,
                                                                          const DecodeF8Params dp) {
     using L = DecodeF8<D, NH>;
+    constexpr int ROWS = L::ROWS;
     constexpr int WORDS = D / 16;                              // 32-bit words of codes a lane holds of a key row; k-steps of a product;
                                                                // row tiles of the output
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -118,68 +185,129 @@ __global__ void __launch_bounds__(DF8_THREADS, NH == 1 ? 3 : 2) attention_decode
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
+    const bool cluster = !SHARES && dp.num_splits > 1;
     // every CTA of the cluster says that it runs; nobody writes into a peer's shared memory before all have
-    if (dp.cluster_merge) cg::this_cluster().barrier_arrive();
+    if (cluster) cg::this_cluster().barrier_arrive();
     pdl_wait();
     pdl_trigger();
 
-    const int kvh = blockIdx.x, split = blockIdx.y, ti = blockIdx.z;
-    const int r = p.tiles[2 * ti], q0 = p.tiles[2 * ti + 1];
+    F8Walk walk;
+    const int split = SHARES ? 0 : blockIdx.y;
+    if constexpr (SHARES) {
+        int* before = reinterpret_cast<int*>(smem + L::RECV);
+        int4* tiles = reinterpret_cast<int4*>(smem + L::RECV + (DF8_SHARE_TILES + 4) * 4);
+        for (int k = threadIdx.x; k < dp.n_tiles; k += DF8_THREADS) {
+            const F8Tile t(dp, k);
+            before[k + 1] = t.n_chunks;
+            tiles[k] = make_int4(t.r, t.tok0, t.n_q, t.pos0);
+        }
+        __syncthreads();
+        if (warp == 0) {
+            int sum = 0;
+            for (int t0 = 0; t0 < dp.n_tiles; t0 += 32) {
+                int v = t0 + lane < dp.n_tiles ? before[t0 + lane + 1] : 0;
+#pragma unroll
+                for (int o = 1; o < 32; o *= 2) {
+                    const int w = __shfl_up_sync(0xffffffffu, v, o);
+                    if (lane >= o) v += w;
+                }
+                if (t0 + lane < dp.n_tiles) before[t0 + lane + 1] = sum + v;
+                sum += __shfl_sync(0xffffffffu, v, 31);
+            }
+            if (lane == 0) before[0] = 0;
+        }
+        __syncthreads();
+        const int64_t total = (int64_t)before[dp.n_tiles] * p.nkv;
+        const int64_t share = max((int64_t)DF8_SHARE_MIN, (total + gridDim.x - 1) / gridDim.x);
+        walk.before = before;
+        walk.tiles = tiles;
+        walk.n_tiles = dp.n_tiles;
+        walk.nkv = p.nkv;
+        walk.at = min(total, blockIdx.x * share);
+        walk.end = min(total, walk.at + share);
+        if (blockIdx.x == 0) {
+            for (int k = threadIdx.x; k < dp.n_tiles; k += DF8_THREADS)
+                dp.plan[k] = make_int4(before[k], before[k + 1] - before[k], tiles[k].y, tiles[k].z);
+            if (threadIdx.x == 0) dp.plan[dp.n_tiles] = make_int4((int)min(share, (int64_t)0x7fffffff), 0, 0, 0);
+        }
+    }
     const int rep = p.nq / p.nkv;
-    const int tok0 = p.row_start[r] + q0;
-    const int n_q = max(0, min(dp.tile_tokens, p.row_start[r + 1] - tok0));
-    const int m_rows = n_q * rep;
-    const int pos0 = p.row_pos[r] + q0;
-    const int hi = pos0 + n_q;                                  // keys < hi are read by the tile
-    const int lo = mask_lo(p.mask, pos0);                       // the first query's rule starts first
-    const int base_key = lo & ~(DF8_CHUNK - 1);                 // chunks start at multiples of 64 keys
-    // the kept first keys, where the rule's range starts beyond them, are chunks of their own in front
-    const int nkb = (p.mask.keep > 0 && base_key > 0) ? min((p.mask.keep + DF8_CHUNK - 1) / DF8_CHUNK, base_key / DF8_CHUNK) : 0;
-    const int n_chunks = n_q > 0 ? nkb + (hi - base_key + DF8_CHUNK - 1) / DF8_CHUNK : 0;
-    const int per = (n_chunks + dp.num_splits - 1) / dp.num_splits;
-    const int c0 = min(n_chunks, split * per), c1 = min(n_chunks, c0 + per);
-    auto key0_of = [&](int c) { return c < nkb ? c * DF8_CHUNK : base_key + (c - nkb) * DF8_CHUNK; };
-
-    float o[NH][WORDS][4];
-    float m_ref[NH][2], l_run[NH][2];
     const int g = lane >> 2, i = lane & 3;
     const int log_box = min(p.logP, 6);
+    // the parts this CTA takes; fn(tile, kv head, first chunk, end, whether the share begins with it)
+    auto parts = [&](auto fn) {
+        if constexpr (SHARES) {
+            for (bool first = true; walk.next(); first = false)
+                if (!fn(F8Tile(p, walk.tiles[walk.ti]), walk.kvh, walk.c0, walk.c1, first)) break;
+        } else {
+            const F8Tile t(dp, blockIdx.z);
+            const int per = (t.n_chunks + dp.num_splits - 1) / dp.num_splits;
+            const int c0 = min(t.n_chunks, split * per);
+            fn(t, (int)blockIdx.x, c0, min(t.n_chunks, c0 + per), true);
+        }
+    };
 
     if (warp == DF8_WARPS) {
         // ---------------------------------------------------------------- producer
         // The whole warp: lane l looks up the cache row of keys 2 l and 2 l + 1 of a chunk, a chunk ahead of the loads, and
         // copies their exponents; an elected lane issues the boxes (one page, or 64 keys of a larger one).
-        const int* table = p.block_table + (int64_t)r * p.table_stride - p.page_base[r];
-        const int box = 1 << log_box, first_key = p.page_base[r] << p.logP;
-        auto row_at = [&](int c) -> int {
-            const int key = key0_of(c) + 2 * lane;
-            int b = key & ~(box - 1);
-            if (b >= hi) b = (hi - 1) & ~(box - 1);               // masked later: any box that exists
-            if (b < first_key) b = first_key;
-            const int page = table[b >> p.logP];
-            return ((page * p.nkv + kvh) << p.logP) + (b & ((1 << p.logP) - 1)) + (key & (box - 1));
-        };
-        int row_next = c0 < c1 ? row_at(c0) : 0;
-        for (int c = c0; c < c1; ++c) {
-            const int row = row_next, n = c - c0, s = n % L::STAGES;
-            if (c + 1 < c1) row_next = row_at(c + 1);
-            const bool got = mbar_wait(empty0 + 8 * s, ((n / L::STAGES) & 1) ^ 1);
-            if (!got && lane == 0) tc_fail(&g_attn_dec_f8_error, 1, ACORN_KERNEL_ATTN_DECODE_F8);
-            if (!__all_sync(0xffffffffu, got)) break;
-            if (elect_one()) mbar_expect_tx(full0 + 8 * s, L::STAGE_BYTES);
-            cp_async_bytes<4>(tc_smem(smem + L::SCALES + s * L::SCALE_BYTES) + 4 * lane, p.scales + 2 * (int64_t)row);
-            cp_async_arrive(full0 + 8 * s);
-            for (int k = 0; k < DF8_CHUNK; k += box) {
-                const int y = __shfl_sync(0xffffffffu, row, k >> 1);
-                if (elect_one()) {
-                    const uint32_t dst = tc_smem(smem + s * L::STAGE_BYTES) + (uint32_t)(2 * k * D);
-                    tma_load_3d(dst, &map_k, full0 + 8 * s, 0, y, 0);
-                    if (!dp.joint) tma_load_3d(dst + box * D, &map_v, full0 + 8 * s, 0, y, 0);
+        const int box = 1 << log_box;
+        int n = 0;                                                // chunks so far
+        parts([&](const F8Tile& t, int kvh, int c0, int c1, bool) -> bool {
+            const int* table = p.block_table + (int64_t)t.r * p.table_stride - p.page_base[t.r];
+            const int first_key = p.page_base[t.r] << p.logP;
+            auto row_at = [&](int c) -> int {
+                const int key = t.key0(c) + 2 * lane;
+                int b = key & ~(box - 1);
+                if (b >= t.hi) b = (t.hi - 1) & ~(box - 1);       // masked later: any box that exists
+                if (b < first_key) b = first_key;
+                const int page = table[b >> p.logP];
+                return ((page * p.nkv + kvh) << p.logP) + (b & ((1 << p.logP) - 1)) + (key & (box - 1));
+            };
+            int row_next = c0 < c1 ? row_at(c0) : 0;
+            for (int c = c0; c < c1; ++c, ++n) {
+                const int row = row_next, s = n % L::STAGES;
+                if (c + 1 < c1) row_next = row_at(c + 1);
+                const bool got = mbar_wait(empty0 + 8 * s, ((n / L::STAGES) & 1) ^ 1);
+                if (!got && lane == 0) tc_fail(&g_attn_dec_f8_error, 1, ACORN_KERNEL_ATTN_DECODE_F8);
+                if (!__all_sync(0xffffffffu, got)) return false;
+                if (elect_one()) mbar_expect_tx(full0 + 8 * s, L::STAGE_BYTES);
+                cp_async_bytes<4>(tc_smem(smem + L::SCALES + s * L::SCALE_BYTES) + 4 * lane, p.scales + 2 * (int64_t)row);
+                cp_async_arrive(full0 + 8 * s);
+                for (int k = 0; k < DF8_CHUNK; k += box) {
+                    const int y = __shfl_sync(0xffffffffu, row, k >> 1);
+                    if (elect_one()) {
+                        const uint32_t dst = tc_smem(smem + s * L::STAGE_BYTES) + (uint32_t)(2 * k * D);
+                        tma_load_3d(dst, &map_k, full0 + 8 * s, 0, y, 0);
+                        if (!dp.joint) tma_load_3d(dst + box * D, &map_v, full0 + 8 * s, 0, y, 0);
+                    }
                 }
             }
+            return true;
+        });
+        if (cluster) {
+            cg::this_cluster().barrier_wait();
+            cg::this_cluster().sync();
         }
-    } else {
-        // ---------------------------------------------------------------- compute warps
+        return;
+    }
+
+    // -------------------------------------------------------------------- compute warps
+    // this lane's pieces of a stage: keys g and g + 8, values of keys 2 i, 2 i + 1, 8 + 2 i, 9 + 2 i of the warp's 16
+    const int k_skip = dp.v_first ? 1 << log_box : 0, v_skip = (1 << log_box) - k_skip;
+    uint32_t k_at[2], v_at[4];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) k_at[k] = L::at(f8_stage_row(warp * 16 + 8 * k + g, log_box) + k_skip, (WORDS / 4) * i);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int row = f8_stage_row(warp * 16 + 2 * i + (k & 1) + 8 * (k >> 1), log_box) + v_skip;
+        v_at[k] = D == 128 ? L::at(row, g) : L::at(row, g >> 1) + 8 * (g & 1);
+    }
+    int n = 0;                                                    // chunks so far
+    parts([&](const F8Tile& t, int kvh, int c0, int c1, bool first) -> bool {
+        const int m_rows = t.n_q * rep, tok0 = t.tok0;
+        float o[NH][WORDS][4];
+        float m_ref[NH][2], l_run[NH][2];
         // queries: this lane holds row g (of each half), entries i * D / 4 .. + D / 4 - 1 of the head, as the B operand
         uint32_t qb[NH][WORDS][2];
         float factor[NH][2];                                      // of query rows 2 i and 2 i + 1: the softmax scale, and what undoes
@@ -215,7 +343,7 @@ __global__ void __launch_bounds__(DF8_THREADS, NH == 1 ? 3 : 2) attention_decode
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
                 factor[h][b] = __shfl_sync(0xffffffffu, back, 4 * (2 * i + b)) * p.scale_log2;
-                qpos[h][b] = pos0 + min((8 * h + 2 * i + b) / rep, max(n_q - 1, 0));
+                qpos[h][b] = t.pos0 + min((8 * h + 2 * i + b) / rep, max(t.n_q - 1, 0));
                 first_seen[h][b] = mask_lo(p.mask, qpos[h][b]);
                 m_ref[h][b] = -INFINITY;
                 l_run[h][b] = 0.f;
@@ -223,28 +351,18 @@ __global__ void __launch_bounds__(DF8_THREADS, NH == 1 ? 3 : 2) attention_decode
 #pragma unroll
             for (int n = 0; n < WORDS; ++n) { o[h][n][0] = o[h][n][1] = o[h][n][2] = o[h][n][3] = 0.f; }
         }
-        const int last_lo = mask_lo(p.mask, hi - 1);              // the last query's rule starts last
-        // this lane's pieces of a stage: keys g and g + 8, values of keys 2 i, 2 i + 1, 8 + 2 i, 9 + 2 i of the warp's 16
-        const int k_skip = dp.v_first ? 1 << log_box : 0, v_skip = (1 << log_box) - k_skip;
-        uint32_t k_at[2], v_at[4];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) k_at[k] = L::at(f8_stage_row(warp * 16 + 8 * k + g, log_box) + k_skip, (WORDS / 4) * i);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int row = f8_stage_row(warp * 16 + 2 * i + (k & 1) + 8 * (k >> 1), log_box) + v_skip;
-            v_at[k] = D == 128 ? L::at(row, g) : L::at(row, g >> 1) + 8 * (g & 1);
-        }
+        const int last_lo = mask_lo(p.mask, t.hi - 1);              // the last query's rule starts last
         bool good = true;
-        for (int c = c0; c < c1; ++c) {
-            const int n = c - c0, s = n % L::STAGES;
+        for (int c = c0; c < c1; ++c, ++n) {
+            const int s = n % L::STAGES;
             if (!mbar_wait(full0 + 8 * s, (n / L::STAGES) & 1)) {
                 tc_fail(&g_attn_dec_f8_error, 2, ACORN_KERNEL_ATTN_DECODE_F8);
                 good = false;
             }
             good = __all_sync(0xffffffffu, good);
             if (!good) break;
-            const int wkey0 = key0_of(c) + warp * 16;             // first key of this warp's 16
-            if (wkey0 < hi && (wkey0 + 15 >= lo || wkey0 < p.mask.keep)) {
+            const int wkey0 = t.key0(c) + warp * 16;             // first key of this warp's 16
+            if (wkey0 < t.hi && (wkey0 + 15 >= t.lo || wkey0 < p.mask.keep)) {
                 const uint8_t* stage = smem + s * L::STAGE_BYTES;
                 float sc[NH][4], sd[NH][4];                       // two chains of products
 #pragma unroll
@@ -270,7 +388,7 @@ __global__ void __launch_bounds__(DF8_THREADS, NH == 1 ? 3 : 2) attention_decode
                     for (int h = 0; h < NH; ++h) mma_f16_16816(k & 1 ? sd[h] : sc[h], a, qb[h][k][0], qb[h][k][1]);
                 }
                 // all of the tile's queries see all 16 keys: no mask
-                const bool whole = wkey0 + 15 <= pos0 && wkey0 >= last_lo;
+                const bool whole = wkey0 + 15 <= t.pos0 && wkey0 >= last_lo;
                 float ve[2], ks[2];
 #pragma unroll
                 for (int r2 = 0; r2 < 2; ++r2) {
@@ -286,12 +404,12 @@ __global__ void __launch_bounds__(DF8_THREADS, NH == 1 ? 3 : 2) attention_decode
                     for (int b = 0; b < 2; ++b) {
 #pragma unroll
                         for (int r2 = 0; r2 < 2; ++r2) {
-                            float t = (sc[h][2 * r2 + b] + sd[h][2 * r2 + b]) * factor[h][b] * ks[r2];
+                            float x = (sc[h][2 * r2 + b] + sd[h][2 * r2 + b]) * factor[h][b] * ks[r2];
                             if (!whole) {
                                 const int key = wkey0 + 8 * r2 + g;
-                                if (!(key <= qpos[h][b] && (key >= first_seen[h][b] || key < p.mask.keep))) t = -INFINITY;
+                                if (!(key <= qpos[h][b] && (key >= first_seen[h][b] || key < p.mask.keep))) x = -INFINITY;
                             }
-                            sc[h][2 * r2 + b] = t;
+                            sc[h][2 * r2 + b] = x;
                         }
                         mx[h][b] = fmaxf(sc[h][b] + ve[0], sc[h][2 + b] + ve[1]);
                         grew = grew || mx[h][b] > m_ref[h][b] + DF8_GROW_LOG2;
@@ -344,7 +462,7 @@ __global__ void __launch_bounds__(DF8_THREADS, NH == 1 ? 3 : 2) attention_decode
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const int key = wkey0 + 2 * i + (k & 1) + 8 * (k >> 1);
-                        if (!(key < hi && (key >= lo || key < p.mask.keep))) {
+                        if (!(key < t.hi && (key >= t.lo || key < p.mask.keep))) {
 #pragma unroll
                             for (int w = 0; w < WORDS / 2; ++w) vw[k][w] = 0u;
                         }
@@ -368,14 +486,11 @@ __global__ void __launch_bounds__(DF8_THREADS, NH == 1 ? 3 : 2) attention_decode
         }
 #pragma unroll
         for (int h = 0; h < NH; ++h) { l_run[h][0] = column_sum(l_run[h][0]); l_run[h][1] = column_sum(l_run[h][1]); }
-    }
-    // every stage has been consumed (the compute warps waited for each); the ring is free for the merge
-    __syncthreads();
-    constexpr int ROWS = 8 * NH;
-    float* sm_m = reinterpret_cast<float*>(smem);                 // [WARPS][ROWS]
-    float* sm_l = sm_m + ROWS * DF8_WARPS;
-    float* sm_o = sm_l + ROWS * DF8_WARPS;                        // [WARPS][ROWS][D]
-    if (warp < DF8_WARPS) {
+        // ---- the warps joined
+        float* sm_m = reinterpret_cast<float*>(smem + L::MERGE);  // [WARPS][ROWS]
+        float* sm_l = sm_m + ROWS * DF8_WARPS;
+        float* sm_o = sm_l + ROWS * DF8_WARPS;                    // [WARPS][ROWS][D]
+        compute_sync();                                           // the part before has been read
 #pragma unroll
         for (int h = 0; h < NH; ++h)
 #pragma unroll
@@ -386,88 +501,130 @@ __global__ void __launch_bounds__(DF8_THREADS, NH == 1 ? 3 : 2) attention_decode
                     sm_l[m] = l_run[h][b];
                 }
 #pragma unroll
-                for (int n = 0; n < WORDS; n += 2)
-                    *reinterpret_cast<float4*>(sm_o + m * D + g * (D / 8) + 2 * n) =
-                        make_float4(o[h][n][b], o[h][n][2 + b], o[h][n + 1][b], o[h][n + 1][2 + b]);
+                for (int n2 = 0; n2 < WORDS; n2 += 2)
+                    *reinterpret_cast<float4*>(sm_o + m * D + g * (D / 8) + 2 * n2) =
+                        make_float4(o[h][n2][b], o[h][n2][2 + b], o[h][n2 + 1][b], o[h][n2 + 1][2 + b]);
             }
-    }
-    __syncthreads();
-    // received partial rows: recv[rank of the sender][slot][RECV_ROW]
-    float* recv = reinterpret_cast<float*>(smem + L::RECV);
-    const int csize = dp.cluster_merge ? dp.num_splits : 1;
-    const int slots = (dp.tile_tokens * rep + csize - 1) / csize;
-    if (dp.cluster_merge) cg::this_cluster().barrier_wait();
-    for (int idx = threadIdx.x; idx < m_rows * D; idx += DF8_THREADS) {
-        const int m = idx / D, e = idx - m * D;
-        const int head = kvh * rep + m % rep;
-        const float sink = p.sink && split == 0 ? p.sink[head] * 1.4426950408889634f : -INFINITY;
-        float mstar = sink;
+        compute_sync();
+        // received partial rows: recv[rank of the sender][slot][RECV_ROW]
+        float* recv = reinterpret_cast<float*>(smem + L::RECV);
+        const int csize = cluster ? dp.num_splits : 1;
+        const int slots = (dp.tile_tokens * rep + csize - 1) / csize;
+        const bool whole_pair = SHARES ? c0 == 0 && c1 == t.n_chunks : !cluster;
+        if (cluster) cg::this_cluster().barrier_wait();
+        for (int idx = threadIdx.x; idx < m_rows * D; idx += 32 * DF8_WARPS) {
+            const int m = idx / D, e = idx - m * D;
+            const int head = kvh * rep + m % rep;
+            const float sink = p.sink && c0 == 0 && split == 0 ? p.sink[head] * 1.4426950408889634f : -INFINITY;
+            float mstar = sink;
 #pragma unroll
-        for (int w = 0; w < DF8_WARPS; ++w) mstar = fmaxf(mstar, sm_m[w * ROWS + m]);
-        float sum = sink == -INFINITY ? 0.f : exp2f(sink - mstar), acc = 0.f;
+            for (int w = 0; w < DF8_WARPS; ++w) mstar = fmaxf(mstar, sm_m[w * ROWS + m]);
+            float sum = sink == -INFINITY ? 0.f : exp2f(sink - mstar), acc = 0.f;
 #pragma unroll
-        for (int w = 0; w < DF8_WARPS; ++w) {
-            // a warp without keys has maximum -inf and sum 0; one whose keys are all NaN a sum that is NaN
-            const float mw = sm_m[w * ROWS + m], lw = sm_l[w * ROWS + m];
-            const float f = mw == -INFINITY ? 0.f : exp2f(mw - mstar);
-            sum += f * lw;
-            acc += f * sm_o[(w * ROWS + m) * D + e];
-        }
-        const bool empty = mstar == -INFINITY && sum == 0.f;      // no key of this split is seen by the query
-        if (dp.num_splits == 1) {
-            p.out[((int64_t)(tok0 + m / rep) * p.nq + head) * D + e] = __float2bfloat16_rn(acc / sum);
-        } else if (dp.cluster_merge) {
-            // to the CTA that finishes this row; a split without keys sends a log-sum of -inf
-            const uint32_t dst = cluster_map(tc_smem(recv + (split * slots + m / csize) * L::RECV_ROW), m % csize);
-            st_cluster_f32(dst + 4 * e, empty ? 0.f : acc / sum);
-            if (e == 0) st_cluster_f32(dst + 4 * D, empty ? -INFINITY : mstar + log2f(sum));
-        } else {
-            const int64_t at = (((int64_t)ti * p.nkv + kvh) * dp.num_splits + split) * 16 + m;
-            dp.part_o[at * D + e] = empty ? 0.f : acc / sum;
-            if (e == 0) dp.part_lse[at] = empty ? -INFINITY : mstar + log2f(sum);
-        }
-    }
-    if (dp.cluster_merge) {
-        cg::this_cluster().sync();                               // all partial rows have arrived
-        for (int idx = threadIdx.x; idx < slots * D; idx += DF8_THREADS) {
-            const int slot = idx / D, e = idx - slot * D;
-            const int m = split + slot * csize;                  // the rows this CTA finishes: rank, rank + csize, ...
-            if (m >= m_rows) break;
-            float mstar = -INFINITY;
-            for (int s = 0; s < csize; ++s) mstar = fmaxf(mstar, recv[(s * slots + slot) * L::RECV_ROW + D]);
-            float sum = 0.f, acc = 0.f;
-            for (int s = 0; s < csize; ++s) {
-                const float lse = recv[(s * slots + slot) * L::RECV_ROW + D];
-                const float f = lse == -INFINITY ? 0.f : exp2f(lse - mstar);
-                sum += f;
-                acc += f * recv[(s * slots + slot) * L::RECV_ROW + e];
+            for (int w = 0; w < DF8_WARPS; ++w) {
+                // a warp without keys has maximum -inf and sum 0; one whose keys are all NaN a sum that is NaN
+                const float mw = sm_m[w * ROWS + m], lw = sm_l[w * ROWS + m];
+                const float f = mw == -INFINITY ? 0.f : exp2f(mw - mstar);
+                sum += f * lw;
+                acc += f * sm_o[(w * ROWS + m) * D + e];
             }
-            p.out[((int64_t)(tok0 + m / rep) * p.nq + kvh * rep + m % rep) * D + e] = __float2bfloat16_rn(acc / sum);
+            const bool empty = mstar == -INFINITY && sum == 0.f;  // no key of this part is seen by the query
+            if (whole_pair) {
+                p.out[((int64_t)(tok0 + m / rep) * p.nq + head) * D + e] = __float2bfloat16_rn(acc / sum);
+            } else if (cluster) {
+                // to the CTA that finishes this row; a split without keys sends a log-sum of -inf
+                const uint32_t dst = cluster_map(tc_smem(recv + (split * slots + m / csize) * L::RECV_ROW), m % csize);
+                st_cluster_f32(dst + 4 * e, empty ? 0.f : acc / sum);
+                if (e == 0) st_cluster_f32(dst + 4 * D, empty ? -INFINITY : mstar + log2f(sum));
+            } else {
+                const int64_t at = ((int64_t)blockIdx.x * 2 + (first ? 0 : 1)) * ROWS + m;
+                dp.part_o[at * D + e] = empty ? 0.f : acc / sum;
+                if (e == 0) dp.part_lse[at] = empty ? -INFINITY : mstar + log2f(sum);
+            }
         }
-    }
+        if (cluster) {
+            cg::this_cluster().sync();                            // all partial rows have arrived
+            for (int idx = threadIdx.x; idx < slots * D; idx += 32 * DF8_WARPS) {
+                const int slot = idx / D, e = idx - slot * D;
+                const int m = split + slot * csize;               // the rows this CTA finishes: rank, rank + csize, ...
+                if (m >= m_rows) break;
+                float mstar = -INFINITY;
+                for (int s = 0; s < csize; ++s) mstar = fmaxf(mstar, recv[(s * slots + slot) * L::RECV_ROW + D]);
+                float sum = 0.f, acc = 0.f;
+                for (int s = 0; s < csize; ++s) {
+                    const float lse = recv[(s * slots + slot) * L::RECV_ROW + D];
+                    const float f = lse == -INFINITY ? 0.f : exp2f(lse - mstar);
+                    sum += f;
+                    acc += f * recv[(s * slots + slot) * L::RECV_ROW + e];
+                }
+                p.out[((int64_t)(tok0 + m / rep) * p.nq + kvh * rep + m % rep) * D + e] = __float2bfloat16_rn(acc / sum);
+            }
+        }
+        return good;
+    });
 }
 
-// The splits of a (tile, kv head) from scratch: one CTA per (tile, kv head, row of the tile), a thread an entry.
-template <int D>
-__global__ void attention_decode_f8_merge_kernel(const DecodeF8Params dp) {
+// Even shares: the pairs that several CTAs had parts of.  One CTA per (tile, kv head, query row); its four warps take every
+// fourth part, D / 32 entries a lane.
+template <int D, int NH>
+__global__ void __launch_bounds__(128) attention_decode_f8_join_kernel(const DecodeF8Params dp) {
+    constexpr int ROWS = 8 * NH, E = D / 32;
+    __shared__ float so[4][D], sl[4], sm[4];
     pdl_wait();
     pdl_trigger();
     const F8AttnParams& p = dp.a;
-    const int kvh = blockIdx.x, m = blockIdx.y, ti = blockIdx.z, e = threadIdx.x;
-    const int r = p.tiles[2 * ti], q0 = p.tiles[2 * ti + 1], rep = p.nq / p.nkv;
-    const int tok = p.row_start[r] + q0 + m / rep;
-    if (tok >= p.row_start[r + 1]) return;
-    const int64_t at0 = ((int64_t)ti * p.nkv + kvh) * dp.num_splits * 16 + m;
-    float mstar = -INFINITY;
-    for (int s = 0; s < dp.num_splits; ++s) mstar = fmaxf(mstar, dp.part_lse[at0 + 16 * s]);
-    float sum = 0.f, acc = 0.f;
-    for (int s = 0; s < dp.num_splits; ++s) {
-        const float lse = dp.part_lse[at0 + 16 * s];
-        const float f = lse == -INFINITY ? 0.f : exp2f(lse - mstar);
-        sum += f;
-        acc += f * dp.part_o[(at0 + 16 * s) * D + e];
+    const int kvh = blockIdx.x, m = blockIdx.y, rep = p.nq / p.nkv;
+    const int4 t = dp.plan[blockIdx.z];                            // chunks before, chunks, first token, tokens
+    const int share = dp.plan[dp.n_tiles].x;
+    const int64_t u0 = (int64_t)t.x * p.nkv + (int64_t)kvh * t.y;
+    if (t.y == 0 || m >= t.w * rep) return;
+    const int b0 = (int)(u0 / share), b1 = (int)((u0 + t.y - 1) / share);
+    if (b0 == b1) return;                                         // one CTA had it all
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // the first CTA's part is the last of its share, unless its share begins with the pair
+    auto at = [&](int b) { return ((int64_t)b * 2 + (b * (int64_t)share >= u0 ? 0 : 1)) * ROWS + m; };
+    float top = -INFINITY, sum = 0.f, acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    for (int c = b0 + warp; c <= b1; c += 4 * 8) {                // eight parts at a time, all on their way together
+        float lse[8], v[8][E];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const bool live = c + 4 * k <= b1;
+            lse[k] = live ? dp.part_lse[at(c + 4 * k)] : -INFINITY;
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[k][e] = live ? dp.part_o[at(c + 4 * k) * D + lane * E + e] : 0.f;
+        }
+        float mx = top;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) mx = fmaxf(mx, lse[k]);
+        const float corr = top == -INFINITY ? 0.f : exp2f(top - mx);
+        top = mx;
+        sum *= corr;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] *= corr;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float f = lse[k] == -INFINITY ? 0.f : exp2f(lse[k] - top);
+            sum += f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] = fmaf(f, v[k][e], acc[e]);
+        }
     }
-    p.out[((int64_t)tok * p.nq + kvh * rep + m % rep) * D + e] = __float2bfloat16_rn(acc / sum);
+    if (lane == 0) { sm[warp] = top; sl[warp] = sum; }
+#pragma unroll
+    for (int e = 0; e < E; ++e) so[warp][lane * E + e] = acc[e];
+    __syncthreads();
+    const float all = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+    float f[4], total = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        f[w] = sm[w] == -INFINITY ? 0.f : exp2f(sm[w] - all);
+        total += f[w] * sl[w];                                    // (a part whose logarithm is NaN left a sum that is NaN)
+    }
+    for (int e = threadIdx.x; e < D; e += 128)
+        p.out[((int64_t)(t.z + m / rep) * p.nq + kvh * rep + m % rep) * D + e] =
+            __float2bfloat16_rn((f[0] * so[0][e] + f[1] * so[1][e] + f[2] * so[2][e] + f[3] * so[3][e]) / total);
 }
 
 // What this kernel takes.
@@ -475,11 +632,44 @@ extern "C" int acorn_attention_decode_f8_supported(int nq, int nkv, int d, int P
     return nkv > 0 && nq % nkv == 0 && nq / nkv <= 16 && (d == 64 || d == 128) && P >= 8 && P <= 4096 && (P & (P - 1)) == 0;
 }
 
-// Whether this many splits are merged inside the kernel (by a cluster, without scratch).
-extern "C" int acorn_attention_decode_f8_merges(int num_splits) { return num_splits <= 8 || num_splits == DF8_CLUSTER_MAX; }
+template <int D, int NH, bool SHARES>
+static cudaError_t configure_decode_f8(size_t smem) {
+    static AcornPerDevice configured;
+    if (configured.seen()) return cudaSuccess;
+    cudaError_t e = cudaFuncSetAttribute(attention_decode_f8_kernel<D, NH, SHARES>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess && !SHARES)
+        e = cudaFuncSetAttribute(attention_decode_f8_kernel<D, NH, SHARES>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess) configured.mark();
+    return e;
+}
+
+// CTAs of the even shares: as many as the device holds at once.
+template <int D, int NH> static int share_ctas() {
+    static int ctas[64] = {};
+    const int dev = AcornPerDevice::current();
+    if (dev < 0) return 0;
+    if (ctas[dev] == 0) {
+        int per_sm = 0;
+        const size_t smem = DecodeF8<D, NH>::RECV + DecodeF8<D, NH>::SHARES;
+        if (configure_decode_f8<D, NH, true>(smem) != cudaSuccess ||
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, attention_decode_f8_kernel<D, NH, true>, DF8_THREADS, smem) != cudaSuccess)
+            return 0;
+        ctas[dev] = per_sm * acorn_sms();
+    }
+    return ctas[dev];
+}
+
+// CTAs that share the work of a call with num_splits 0 (its scratch: part_o [CTAs, 2, rows, d], part_lse [CTAs, 2, rows] float32,
+// plan [n_tiles + 1, 4] int32, with rows = 8 up to 8 query rows a tile, else 16); 0 where there are too many tiles for that.
+extern "C" int acorn_attention_decode_f8_shares(int nq, int nkv, int d, int tile_tokens, int n_tiles) {
+    if (n_tiles > DF8_SHARE_TILES || nkv < 1 || nq % nkv) return 0;
+    const bool one = tile_tokens * (nq / nkv) <= 8;
+    if (d == 128) return one ? share_ctas<128, 1>() : share_ctas<128, 2>();
+    return one ? share_ctas<64, 1>() : share_ctas<64, 2>();
+}
 
 template <int D, int NH>
-static int launch_decode_f8(DecodeF8Params dp, int64_t num_pages, int n_tiles, cudaStream_t stream) {
+static int launch_decode_f8(DecodeF8Params dp, int64_t num_pages, cudaStream_t stream) {
     using L = DecodeF8<D, NH>;
     const F8AttnParams& p = dp.a;
     CUtensorMap mk, mv;
@@ -487,46 +677,48 @@ static int launch_decode_f8(DecodeF8Params dp, int64_t num_pages, int n_tiles, c
     const int rc = make_code_maps(&mk, &mv, p, num_pages, D, box_rows,
                                   D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, &dp.joint, &dp.v_first);
     if (rc) return rc;
-    const int rows = dp.tile_tokens * (p.nq / p.nkv);
-    const size_t recv = dp.cluster_merge ? (size_t)dp.num_splits * ((rows + dp.num_splits - 1) / dp.num_splits) * L::RECV_ROW * 4 : 0;
-    const size_t smem = L::RECV + recv, smem_max = L::RECV + (size_t)32 * L::RECV_ROW * 4;
-    static AcornPerDevice configured;
-    if (!configured.seen()) {
-        cudaError_t e = cudaFuncSetAttribute(attention_decode_f8_kernel<D, NH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_max);
-        if (e != cudaSuccess) return (int)e;
-        e = cudaFuncSetAttribute(attention_decode_f8_kernel<D, NH>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e != cudaSuccess) return (int)e;
-        configured.mark();
+    if (dp.num_splits == 0) {
+        const int ctas = share_ctas<D, NH>();
+        if (ctas < 1) return ACORN_ERR_UNSUPPORTED;
+        const int e = acorn_launch(attention_decode_f8_kernel<D, NH, true>, dim3(ctas), dim3(DF8_THREADS), (size_t)(L::RECV + L::SHARES), stream,
+                                   mk, mv, dp);
+        return e ? e : acorn_launch(attention_decode_f8_join_kernel<D, NH>, dim3(p.nkv, dp.tile_tokens * (p.nq / p.nkv), dp.n_tiles), dim3(128), 0, stream,
+                                    dp);
     }
+    const int rows = dp.tile_tokens * (p.nq / p.nkv), splits = dp.num_splits;
+    const size_t recv = splits > 1 ? (size_t)splits * ((rows + splits - 1) / splits) * L::RECV_ROW * 4 : 0;
+    cudaError_t e = configure_decode_f8<D, NH, false>(L::RECV + (size_t)32 * L::RECV_ROW * 4);
+    if (e != cudaSuccess) return (int)e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.nkv, dp.num_splits, n_tiles);
+    cfg.gridDim = dim3(p.nkv, splits, dp.n_tiles);
     cfg.blockDim = dim3(DF8_THREADS);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = L::RECV + recv;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 1;
-    attr[0].val.clusterDim.y = dp.cluster_merge ? dp.num_splits : 1;
+    attr[0].val.clusterDim.y = splits;
     attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = acorn_pdl_enabled() ? 2 : 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, attention_decode_f8_kernel<D, NH>, mk, mv, dp);
-    if (e == cudaSuccess) e = cudaGetLastError();
-    if (e != cudaSuccess || dp.num_splits == 1 || dp.cluster_merge) return (int)e;
-    return acorn_launch(attention_decode_f8_merge_kernel<D>, dim3(p.nkv, rows, n_tiles), dim3(D), 0, stream, dp);
+    e = cudaLaunchKernelEx(&cfg, attention_decode_f8_kernel<D, NH, false>, mk, mv, dp);
+    return e != cudaSuccess ? (int)e : acorn_launch_status();
 }
 
+// num_splits: 1 to 8 or 16 (a cluster joins them), or 0: even shares, which need the scratch of acorn_attention_decode_f8_shares.
 extern "C" int acorn_attention_decode_f8(const void* q, int64_t q_stride, void* out, const void* k_pages, const void* v_pages,
                                          const void* scales, int64_t num_pages, const int* block_table, const int* page_base,
                                          int table_stride, const int* row_start, const int* row_pos, const int* tiles, int n_tiles,
                                          int nq, int nkv, int d, int P, float scale, int window, int chunk, int keep,
-                                         const float* sink, int tile_tokens, int num_splits, float* part_o, float* part_lse,
+                                         const float* sink, int tile_tokens, int num_splits, float* part_o, float* part_lse, void* plan,
                                          cudaStream_t stream) {
     if (n_tiles <= 0) return 0;
-    if (!acorn_attention_decode_f8_supported(nq, nkv, d, P) || n_tiles > 65535 || num_splits < 1 || num_splits > 65535 || q_stride % 8 ||
-        tile_tokens < 1 || tile_tokens > 16 / (nq / nkv))
+    if (!acorn_attention_decode_f8_supported(nq, nkv, d, P) || n_tiles > 65535 || q_stride % 8 || num_splits < 0 ||
+        (num_splits > 8 && num_splits != DF8_CLUSTER_MAX) || tile_tokens < 1 || tile_tokens > 16 / (nq / nkv) || nkv > 65535)
+        return ACORN_ERR_UNSUPPORTED;
+    if (num_splits == 0 && (n_tiles > DF8_SHARE_TILES || part_o == nullptr || part_lse == nullptr || plan == nullptr))
         return ACORN_ERR_UNSUPPORTED;
     DecodeF8Params dp;
     F8AttnParams& p = dp.a;
@@ -535,15 +727,11 @@ extern "C" int acorn_attention_decode_f8(const void* q, int64_t q_stride, void* 
     p.row_start = row_start; p.row_pos = row_pos; p.tiles = tiles; p.sink = sink; p.table_stride = table_stride;
     p.nq = nq; p.nkv = nkv; p.mask = {window, chunk, keep}; p.scale_log2 = scale * 1.4426950408889634f;
     p.logP = acorn_log2_exact_tc(P);
-    dp.tile_tokens = tile_tokens;
-    dp.num_splits = num_splits;
-    dp.cluster_merge = num_splits > 1 && acorn_attention_decode_f8_merges(num_splits);
-    dp.part_o = part_o; dp.part_lse = part_lse;
-    if (num_splits > 1 && !dp.cluster_merge && (part_o == nullptr || part_lse == nullptr)) return ACORN_ERR_UNSUPPORTED;
+    dp.n_tiles = n_tiles; dp.tile_tokens = tile_tokens; dp.num_splits = num_splits;
+    dp.part_o = part_o; dp.part_lse = part_lse; dp.plan = (int4*)plan;
     const bool one = tile_tokens * (nq / nkv) <= 8;
-    if (d == 128)
-        return one ? launch_decode_f8<128, 1>(dp, num_pages, n_tiles, stream) : launch_decode_f8<128, 2>(dp, num_pages, n_tiles, stream);
-    return one ? launch_decode_f8<64, 1>(dp, num_pages, n_tiles, stream) : launch_decode_f8<64, 2>(dp, num_pages, n_tiles, stream);
+    if (d == 128) return one ? launch_decode_f8<128, 1>(dp, num_pages, stream) : launch_decode_f8<128, 2>(dp, num_pages, stream);
+    return one ? launch_decode_f8<64, 1>(dp, num_pages, stream) : launch_decode_f8<64, 2>(dp, num_pages, stream);
 }
 
 extern "C" int acorn_attention_decode_f8_error() {

@@ -150,7 +150,7 @@ class _Sigs:
                                 c_void_p, c_void_p]
     acorn_attention_decode_f8 = [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p,
                                  c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p, c_int,
-                                 c_int, c_void_p, c_void_p, c_void_p]
+                                 c_int, c_void_p, c_void_p, c_void_p, c_void_p]
     acorn_attention_prefill_f8 = [c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
                                   c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int,
                                   c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]
@@ -158,7 +158,7 @@ class _Sigs:
     acorn_attention_prefill_f8_error = []
     acorn_attention_prefill_f8_set_error_word = [c_void_p]
     acorn_attention_decode_f8_supported = [c_int, c_int, c_int, c_int]
-    acorn_attention_decode_f8_merges = [c_int]
+    acorn_attention_decode_f8_shares = [c_int, c_int, c_int, c_int, c_int]
     acorn_attention_decode_f8_error = []
     acorn_attention_decode_f8_set_error_word = [c_void_p]
     acorn_scan_chunk = [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
@@ -438,7 +438,7 @@ class _TimedLib:
 
     def __getattr__(self, name):
         fn = getattr(self._library, name)
-        if not name.startswith("acorn_") or name.endswith(("_supported", "_error", "_merges", "_scratch", "_ids")):
+        if not name.startswith("acorn_") or name.endswith(("_supported", "_error", "_merges", "_scratch", "_ids", "_shares")):
             return fn
 
         def timed(*args):
@@ -1104,7 +1104,8 @@ def f8_tile_tokens(num_heads: int, num_kv_heads: int) -> int:
     return max(1, 16 // (num_heads // num_kv_heads))
 
 
-F8_MAX_SPLITS = 64
+F8_MAX_SPLITS = 16
+F8_SPLITS = (0, 1, 2, 3, 4, 5, 6, 7, 8, 16)       # of ``attention_decode_f8``: even shares, or so many parts a row
 
 
 F8_PREFILL_SCRATCH = 1 << 30      # bytes of bfloat16 keys and values that a call of ``attention_prefill_f8`` makes at a time
@@ -1123,12 +1124,15 @@ def prefill_f8_splits(ctas: int, blocks: int, num_sms: int = 148) -> int:
 
 
 @lru_cache(maxsize=4096)
-def decode_f8_splits(tiles: int, num_kv_heads: int, key_bound: int, head_dim: int, num_sms: int = 148) -> int:
-    """Splits of the key range for ``attention_decode_f8``."""
-    pairs = max(1, tiles * num_kv_heads)
+def decode_f8_splits(tiles: int, num_kv_heads: int, key_bound: int, head_dim: int, shares: int) -> int:
+    """How ``attention_decode_f8`` cuts its work: into even shares (0) for ``shares`` CTAs, or into so many parts a (tile, kv
+    head)."""
+    pairs, chunks = max(1, tiles * num_kv_heads), -(-key_bound // 64)
+    if shares and pairs * chunks > 2 * shares:
+        return 0
     best = 1
     for s in (2, 3, 4, 5, 6, 7, 8, 16):
-        if pairs * s <= 2 * num_sms and key_bound >= 128 * s:
+        if pairs * s <= max(shares, 148) and chunks >= s:
             best = s
     return best
 
@@ -1189,7 +1193,7 @@ def attention_decode_f8(q: torch.Tensor, q_stride: int, k_pages: torch.Tensor, v
     ``row_pos[r] + i`` and reads the keys up to its own.  ``out`` is [all tokens of the step, nq * d]; rows of tokens in no tile
     are left as they are.  No token is in two tiles, and no tile is empty.  ``tile_tokens``: the most tokens a tile holds, where
     that is less than ``f8_tile_tokens`` (tiles of single tokens among longer rows).  ``num_splits``: into how many parts a row's
-    keys are cut (None: by a rule).  ``window`` / ``chunk`` / ``keep_first`` / ``sink32``: as for ``attention_plain``."""
+    keys are cut (1 to 8, 16), or 0: all tiles' keys in even shares for as many CTAs as the device holds (None: by a rule).  ``window`` / ``chunk`` / ``keep_first`` / ``sink32``: as for ``attention_plain``."""
     what = "attention_decode_f8"
     P, out, stream = _check_f8_attention(what, q, q_stride, k_pages, v_pages, scales, block_table, page_base, row_start, row_pos, tiles,
                                          num_tokens, num_heads, num_kv_heads, head_dim, window, out, chunk, keep_first, sink32)
@@ -1202,21 +1206,24 @@ def attention_decode_f8(q: torch.Tensor, q_stride: int, k_pages: torch.Tensor, v
         return _attention_f8_plain(q, q_stride, out, k_pages, v_pages, scales, block_table, page_base, row_start, row_pos, tiles,
                                    tile_tokens, num_heads, num_kv_heads, head_dim, P, scale, window, chunk,
                                    keep_first, sink32, stream)
+    shares = lib().acorn_attention_decode_f8_shares(num_heads, num_kv_heads, head_dim, tile_tokens, n)
     if num_splits is None:
         spans = [v for v in (window, chunk) if v]
         bound = block_table.shape[1] * P
-        num_splits = decode_f8_splits(n, num_kv_heads, min([bound] + [v + (keep_first or 0) for v in spans]), head_dim, device_sms(q.device))
-    if not 1 <= num_splits <= F8_MAX_SPLITS:
-        raise KernelError(f"{what}: num_splits must be in 1..{F8_MAX_SPLITS}, got {num_splits}")
-    part_o = part_lse = None
-    if n and not lib().acorn_attention_decode_f8_merges(num_splits):
-        part_o = torch.empty((n, num_kv_heads, num_splits, 16, head_dim), dtype=torch.float32, device=q.device)
-        part_lse = torch.empty((n, num_kv_heads, num_splits, 16), dtype=torch.float32, device=q.device)
+        num_splits = decode_f8_splits(n, num_kv_heads, min([bound] + [v + (keep_first or 0) for v in spans]), head_dim, shares)
+    if num_splits not in F8_SPLITS or (num_splits == 0 and not shares):
+        raise KernelError(f"{what}: num_splits must be one of {F8_SPLITS} (0: even shares, of up to 256 tiles), got {num_splits}")
+    part_o = part_lse = plan = None
+    if num_splits == 0:
+        rows = 8 if tile_tokens * (num_heads // num_kv_heads) <= 8 else 16
+        part_o = torch.empty((shares, 2, rows, head_dim + 1), dtype=torch.float32, device=q.device)      # and the sums' logarithms
+        part_lse = part_o.data_ptr() + shares * 2 * rows * head_dim * 4
+        plan = torch.empty((n + 1, 4), dtype=torch.int32, device=q.device)
     _ok(lib().acorn_attention_decode_f8(q.data_ptr(), q_stride, out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
                                         scales.data_ptr(), k_pages.shape[0], block_table.data_ptr(), page_base.data_ptr(),
                                         block_table.stride(0), row_start.data_ptr(), row_pos.data_ptr(), tiles.data_ptr(), n, num_heads,
                                         num_kv_heads, head_dim, P, float(scale), int(window or 0), int(chunk or 0), int(keep_first or 0),
-                                        _ptr(sink32), tile_tokens, num_splits, _ptr(part_o), _ptr(part_lse), stream), what)
+                                        _ptr(sink32), tile_tokens, num_splits, _ptr(part_o), part_lse, _ptr(plan), stream), what)
     return out
 
 

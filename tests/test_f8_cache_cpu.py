@@ -147,11 +147,12 @@ def test_tokens_a_tile(nq, nkv, tokens):
 def test_splits_are_within_the_kernels_limits():
     for tiles in (1, 2, 7, 41, 148, 500):
         for bound in (16, 300, 1000, 4096, 40000, 1 << 20):
-            s = ops.decode_f8_splits(tiles, 8, bound, 128)
-            assert 1 <= s <= ops.F8_MAX_SPLITS
-            assert ops.decode_f8_splits(tiles, 8, bound, 128) == s
-            assert 1 <= ops.prefill_f8_splits(tiles * 16, -(-bound // 128)) <= min(16, -(-bound // 128))
-    assert ops.decode_f8_splits(1, 8, 16, 128) == 1 and ops.prefill_f8_splits(2000, 64) == 1
+            for shares in (0, 444):
+                s = ops.decode_f8_splits(tiles, 8, bound, 128, shares)
+                assert s in ops.F8_SPLITS and (shares or s)             # without CTAs to share there are no shares
+            assert 1 <= ops.prefill_f8_splits(tiles * 16, -(-bound // 128)) <= min(ops.F8_MAX_SPLITS, -(-bound // 128))
+    assert ops.decode_f8_splits(1, 8, 16, 128, 444) == 1 and ops.prefill_f8_splits(2000, 64) == 1
+    assert ops.decode_f8_splits(64, 8, 4096, 128, 444) == 0
 
 
 def test_generation_and_command_line_take_the_option():
