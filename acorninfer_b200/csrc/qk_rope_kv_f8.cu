@@ -9,10 +9,13 @@
 //   q heads are rounded to bfloat16 into q_out; k and v heads become e4m3 codes and an exponent, straight from float32.
 //
 // A CTA takes one token, or a share of its heads where tokens are few: the token's angles are made once, in shared memory, and
-// a lane takes eight neighbouring entries of a head (16 bytes in; 16 or 8 out), LPH lanes a head, so that the sum of squares,
-// the largest magnitude and the other half of a rotated pair are shuffles among them.  The angle is formed and brought to
-// [-pi, pi] in 64 bits: in 32 its error is 2^-24 of the angle itself, 0.008 radians at position 131,072, against 2^-9 of a
-// rounding to bfloat16.
+// a lane takes eight entries of a head (16 bytes in; 16 or 8 out), LPH lanes a head, so that the sum of squares and the
+// largest magnitude are shuffles among them.  Heads rotated whole in pairs (j, j + d/2) give a lane four entries of each half, so
+// that it holds whole pairs (PAIRED); otherwise the eight are neighbours, and the other half of a pair is a shuffle more.
+// What bounds it: its instructions, not its bytes; so only the key and value heads look for their largest magnitude, as an
+// integer maximum over the bits, which also tells infinities and NaN.
+// The angle is formed and brought to [-pi, pi] in 64 bits: in 32 its error is 2^-24 of the angle itself, 0.008 radians at
+// position 131,072, against 2^-9 of a rounding to bfloat16.
 #include "f8_cache.cuh"
 
 #define KVF8_THREADS 256
@@ -46,48 +49,88 @@ __device__ __forceinline__ void kvf8_unpack(const uint4& raw, float (&x)[8]) {
     }
 }
 
-template <int LPH>
+__device__ __forceinline__ uint2 kvf8_pack4(float a, float b, float c, float d) {
+    const __nv_bfloat162 x = __floats2bfloat162_rn(a, b), y = __floats2bfloat162_rn(c, d);
+    return make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+}
+
+// Eight entries as codes: times inv, or zeros.
+__device__ __forceinline__ uint2 kvf8_codes(const float (&x)[8], float inv, float limit) {
+    float z[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) z[i] = fminf(fmaxf(x[i] * inv, -limit), limit);
+    return make_uint2(f8_pack2(z[0], z[1]) | f8_pack2(z[2], z[3]) << 16, f8_pack2(z[4], z[5]) | f8_pack2(z[6], z[7]) << 16);
+}
+
+template <int LPH, bool PAIRED>
 __global__ void __launch_bounds__(KVF8_THREADS) qk_rope_kv_f8_kernel(const KvF8Params p) {
-    extern __shared__ float2 turn[];                          // cos and sin of the token's angles
+    extern __shared__ __align__(16) float2 turn[];            // cos and sin of the token's angles
     pdl_wait();
     pdl_trigger();
     const int t = blockIdx.x;
-    const int pos = p.positions[t];
+    const int pos = p.positions[t], r = p.token_row[t];
     const int half = p.rot >> 1;
-    for (int j = threadIdx.x; j < half; j += KVF8_THREADS) {
-        const double a = (double)pos * (double)p.inv_freq[j];
-        const double r = fma(-rint(a * 0.15915494309189535), 6.283185307179586, a);
-        float s, c;
-        sincosf((float)r, &s, &c);
-        turn[j] = make_float2(c * p.magnitude, s * p.magnitude);
-    }
-    __syncthreads();
     const int heads = p.nq + 2 * p.nkv;
     const int l = threadIdx.x & (LPH - 1);
     const bool on = 8 * l < p.d;                              // lanes beyond a head whose size is no power of two
-    const int per_pass = KVF8_THREADS / LPH * gridDim.y;
-    for (int h0 = blockIdx.y * (KVF8_THREADS / LPH); h0 < heads; h0 += per_pass) {       // the same trips for all lanes of a warp
-        const int h = h0 + threadIdx.x / LPH;
+    // this lane's entries: at0 .. at0 + 3 and at1 .. at1 + 3
+    const int at0 = PAIRED ? 4 * l : 8 * l, at1 = PAIRED ? (p.d >> 1) + 4 * l : 8 * l + 4;
+    const bf16* row = p.qkv + (int64_t)t * p.ld;
+    auto fetch = [&](int h) {
+        if (!on || h >= heads) return make_uint4(0u, 0u, 0u, 0u);
+        const bf16* src = row + (int64_t)h * p.d;
+        const uint2 a = *reinterpret_cast<const uint2*>(src + at0), b = *reinterpret_cast<const uint2*>(src + at1);
+        return make_uint4(a.x, a.y, b.x, b.y);
+    };
+    const int per_pass = KVF8_THREADS / LPH * gridDim.y, in_pass = threadIdx.x / LPH;
+    int h0 = blockIdx.y * (KVF8_THREADS / LPH);
+    uint4 raw = fetch(h0 + in_pass);                          // on its way while the angles are made
+    const int page = p.block_table[(int64_t)r * p.table_stride + (pos / p.P - p.page_base[r])];
+    for (int j = threadIdx.x; j < half; j += KVF8_THREADS) {
+        const double a = (double)pos * (double)p.inv_freq[j];
+        const double z = fma(-rint(a * 0.15915494309189535), 6.283185307179586, a);
+        float s, c;
+        sincosf((float)z, &s, &c);
+        turn[j] = make_float2(c * p.magnitude, s * p.magnitude);
+    }
+    __syncthreads();
+    const int64_t slot0 = (int64_t)page * p.nkv * p.P + pos % p.P;
+    for (; h0 < heads; h0 += per_pass) {                      // the same trips for all lanes of a warp
+        const int h = h0 + in_pass;
         const bool live = on && h < heads;
-        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (live) kvf8_unpack(*reinterpret_cast<const uint4*>(p.qkv + (int64_t)t * p.ld + (int64_t)h * p.d + 8 * l), x);
+        float x[8];
+        kvf8_unpack(raw, x);
+        raw = fetch(h + per_pass);
         if (p.bias && live) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] += p.bias[h * p.d + 8 * l + i];
+            for (int i = 0; i < 8; ++i) x[i] += p.bias[h * p.d + (i < 4 ? at0 + i : at1 + i - 4)];
         }
         const bool is_v = h >= p.nq + p.nkv;
         const float* w = is_v ? nullptr : h < p.nq ? p.q_w : p.k_w;
-        float ss = 0.f;
+        if (p.q_w || p.k_w) {
+            float ss = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+            for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
 #pragma unroll
-        for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (w && live) {
-            const float inv = rsqrtf(ss / (float)p.d + p.eps);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * w[8 * l + i];
+            for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            if (w && live) {
+                const float inv = rsqrtf(ss / (float)p.d + p.eps);
+                const float4 wa = *reinterpret_cast<const float4*>(w + at0), wb = *reinterpret_cast<const float4*>(w + at1);
+                x[0] *= inv * wa.x; x[1] *= inv * wa.y; x[2] *= inv * wa.z; x[3] *= inv * wa.w;
+                x[4] *= inv * wb.x; x[5] *= inv * wb.y; x[6] *= inv * wb.z; x[7] *= inv * wb.w;
+            }
         }
-        if (p.interleaved) {
+        if constexpr (PAIRED) {
+            if (!is_v && live) {
+#pragma unroll
+                for (int i = 0; i < 4; i += 2) {
+                    const float4 cs = *reinterpret_cast<const float4*>(turn + at0 + i);
+                    const float a0 = x[i], b0 = x[4 + i], a1 = x[i + 1], b1 = x[5 + i];
+                    x[i] = a0 * cs.x - b0 * cs.y; x[4 + i] = b0 * cs.x + a0 * cs.y;
+                    x[i + 1] = a1 * cs.z - b1 * cs.w; x[5 + i] = b1 * cs.z + a1 * cs.w;
+                }
+            }
+        } else if (p.interleaved) {
             if (live && !is_v && 8 * l < p.rot) {
 #pragma unroll
                 for (int i = 0; i < 8; i += 2) {
@@ -101,60 +144,63 @@ __global__ void __launch_bounds__(KVF8_THREADS) qk_rope_kv_f8_kernel(const KvF8P
                 }
             }
         } else if (half > 0) {                                // half is a multiple of 8: the partner is another lane's entry
-            const int step = half >> 3;
-            const bool first = l < step, second = !first && l < 2 * step;
-            const int from = (threadIdx.x & 31 & ~(LPH - 1)) + (first ? l + step : second ? l - step : l);
+            const int away = half >> 3;
+            const bool first = l < away, second = !first && l < 2 * away;
+            const int from = (threadIdx.x & 31 & ~(LPH - 1)) + (first ? l + away : second ? l - away : l);
             float y[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(0xffffffffu, x[i], from);
             if (!is_v && (first || second) && live) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float2 cs = turn[8 * (first ? l : l - step) + i];
+                    const float2 cs = turn[8 * (first ? l : l - away) + i];
                     x[i] = x[i] * cs.x + (first ? -y[i] : y[i]) * cs.y;
                 }
             }
         }
-        float most = 0.f;
-        bool finite = true;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            most = fmaxf(most, fabsf(x[i]));
-            finite = finite && fabsf(x[i]) <= 3.402823466e38f;
-        }
-#pragma unroll
-        for (int o = LPH / 2; o > 0; o >>= 1) {
-            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-            finite = __shfl_xor_sync(0xffffffffu, (int)finite, o) && finite;
-        }
-        if (!live) continue;
-        if (h < p.nq) {
-            uint32_t v[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const __nv_bfloat162 b = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-                v[i] = *reinterpret_cast<const uint32_t*>(&b);
+        if (__all_sync(0xffffffffu, h < p.nq)) {              // queries throughout the warp
+            if (live) {
+                bf16* dst = p.q_out + (int64_t)t * p.ld_q + (int64_t)h * p.d;
+                *reinterpret_cast<uint2*>(dst + at0) = kvf8_pack4(x[0], x[1], x[2], x[3]);
+                *reinterpret_cast<uint2*>(dst + at1) = kvf8_pack4(x[4], x[5], x[6], x[7]);
             }
-            *reinterpret_cast<uint4*>(p.q_out + (int64_t)t * p.ld_q + (int64_t)h * p.d + 8 * l) = make_uint4(v[0], v[1], v[2], v[3]);
             continue;
         }
-        const int r = p.token_row[t], kvh = (h - p.nq) % p.nkv;
-        const int page = p.block_table[(int64_t)r * p.table_stride + (pos / p.P - p.page_base[r])];
-        const int64_t slot = ((int64_t)page * p.nkv + kvh) * p.P + pos % p.P;
-        const int e = f8_row_exponent(most);
-        // at the largest exponent a code above 240 would stand for more than the largest float
-        const float inv = finite ? f8_pow2(-e) : 0.f, limit = e == F8_MAX_EXP ? 240.f : 448.f;
-        uint32_t c[2];
+        uint32_t most = 0u;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            float z[4];
+        for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) z[k] = finite ? fminf(fmaxf(x[4 * i + k] * inv, -limit), limit) : 0.f;
-            c[i] = f8_pack2(z[0], z[1]) | f8_pack2(z[2], z[3]) << 16;
+        for (int o = LPH / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+        if (!live) continue;
+        if (h < p.nq) {
+            bf16* dst = p.q_out + (int64_t)t * p.ld_q + (int64_t)h * p.d;
+            *reinterpret_cast<uint2*>(dst + at0) = kvf8_pack4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<uint2*>(dst + at1) = kvf8_pack4(x[4], x[5], x[6], x[7]);
+            continue;
         }
-        *reinterpret_cast<uint2*>((is_v ? p.v_pages : p.k_pages) + slot * p.d + 8 * l) = make_uint2(c[0], c[1]);
+        const int64_t slot = slot0 + (int64_t)((h - p.nq) % p.nkv) * p.P;
+        const bool finite = most < 0x7f800000u;
+        const int e = f8_row_exponent(__uint_as_float(most));
+        // at the largest exponent a code above 240 would stand for more than the largest float
+        const uint2 c = finite ? kvf8_codes(x, f8_pow2(-e), e == F8_MAX_EXP ? 240.f : 448.f) : make_uint2(0u, 0u);
+        uint8_t* dst = (is_v ? p.v_pages : p.k_pages) + slot * p.d;
+        if constexpr (PAIRED) {
+            *reinterpret_cast<uint32_t*>(dst + at0) = c.x;
+            *reinterpret_cast<uint32_t*>(dst + at1) = c.y;
+        } else {
+            *reinterpret_cast<uint2*>(dst + at0) = c;
+        }
         if (l == 0) p.scales[2 * slot + (is_v ? 1 : 0)] = (uint8_t)(finite ? e + 127 : F8_NAN_BYTE);
     }
+}
+
+template <int LPH>
+static int launch_kv_f8(const KvF8Params& p, int tokens, cudaStream_t stream) {
+    const int per_cta = KVF8_THREADS / LPH, passes = (p.nq + 2 * p.nkv + per_cta - 1) / per_cta;
+    const size_t smem = (size_t)(p.rot / 2) * sizeof(float2);
+    const dim3 grid(tokens, tokens < 2 * acorn_sms() ? passes : 1);          // few tokens: a CTA for every pass over a token's heads
+    if (p.rot == p.d && !p.interleaved) return acorn_launch(qk_rope_kv_f8_kernel<LPH, true>, grid, dim3(KVF8_THREADS), smem, stream, p);
+    return acorn_launch(qk_rope_kv_f8_kernel<LPH, false>, grid, dim3(KVF8_THREADS), smem, stream, p);
 }
 
 extern "C" int acorn_qk_rope_kv_f8(const void* qkv, int64_t ld, const float* q_w, const float* k_w, const float* bias,
@@ -173,15 +219,12 @@ extern "C" int acorn_qk_rope_kv_f8(const void* qkv, int64_t ld, const float* q_w
     p.nq = nq; p.nkv = nkv; p.d = d; p.rot = rot; p.interleaved = interleaved; p.P = P; p.eps = eps; p.magnitude = magnitude;
     int lph = 1;
     while (8 * lph < d) lph *= 2;
-    const int passes = (nq + 2 * nkv + KVF8_THREADS / lph - 1) / (KVF8_THREADS / lph);
-    const dim3 grid(tokens, tokens < 2 * acorn_sms() ? passes : 1);
-    const size_t smem = (size_t)(rot / 2) * sizeof(float2);
     switch (lph) {
-        case 1: return acorn_launch(qk_rope_kv_f8_kernel<1>, grid, dim3(KVF8_THREADS), smem, stream, p);
-        case 2: return acorn_launch(qk_rope_kv_f8_kernel<2>, grid, dim3(KVF8_THREADS), smem, stream, p);
-        case 4: return acorn_launch(qk_rope_kv_f8_kernel<4>, grid, dim3(KVF8_THREADS), smem, stream, p);
-        case 8: return acorn_launch(qk_rope_kv_f8_kernel<8>, grid, dim3(KVF8_THREADS), smem, stream, p);
-        case 16: return acorn_launch(qk_rope_kv_f8_kernel<16>, grid, dim3(KVF8_THREADS), smem, stream, p);
-        default: return acorn_launch(qk_rope_kv_f8_kernel<32>, grid, dim3(KVF8_THREADS), smem, stream, p);
+        case 1: return launch_kv_f8<1>(p, tokens, stream);
+        case 2: return launch_kv_f8<2>(p, tokens, stream);
+        case 4: return launch_kv_f8<4>(p, tokens, stream);
+        case 8: return launch_kv_f8<8>(p, tokens, stream);
+        case 16: return launch_kv_f8<16>(p, tokens, stream);
+        default: return launch_kv_f8<32>(p, tokens, stream);
     }
 }

@@ -1126,14 +1126,24 @@ def prefill_f8_splits(ctas: int, blocks: int, num_sms: int = 148) -> int:
 @lru_cache(maxsize=4096)
 def decode_f8_splits(tiles: int, num_kv_heads: int, key_bound: int, head_dim: int, shares: int) -> int:
     """How ``attention_decode_f8`` cuts its work: into even shares (0) for ``shares`` CTAs, or into so many parts a (tile, kv
-    head)."""
+    head).  By estimates in us, fitted to 1 to 128 rows of 8 kv heads with 300 to 131,072 keys, which they meet to some 20 %: a
+    CTA's start and end take 6, a chunk of 64 keys 0.8 in a CTA (its warps' latencies), all of them together 6.1 TB/s; clusters run in
+    one wave up to 400 CTAs, of sixteen up to 256 (8 rows of 4,000 keys: 6 parts, 384 CTAs, 18.9, 7 parts 28.4); shares take 12
+    and 3 a pair that a CTA comes to (64 rows of 4,096 keys: 101, whole 124, in 3 parts 114; 41 of 600 to 1,700: 34.5, whole 30;
+    one of 131,072: 61, in 16 parts 105)."""
     pairs, chunks = max(1, tiles * num_kv_heads), -(-key_bound // 64)
-    if shares and pairs * chunks > 2 * shares:
+    at_once = shares or 444
+    stream_us = pairs * chunks * (128 * head_dim + 128) / 6.1e6
+    best, best_us = 1, None
+    for s in (1, 2, 3, 4, 5, 6, 7, 8, 16):
+        if s > chunks or (s > 1 and pairs * s > (256 if s == 16 else 400)):
+            continue
+        us = -(-pairs * s // at_once) * (6.0 + -(-chunks // s) * 0.8) + (0.5 if s > 1 else 0.0)
+        us = max(us, 6.0 + stream_us)
+        if best_us is None or us <= best_us:
+            best, best_us = s, us
+    if shares and 12.0 + 3.0 * (pairs / at_once + 1) + max(stream_us, max(pairs * chunks / at_once, 4) * 0.8) < best_us:
         return 0
-    best = 1
-    for s in (2, 3, 4, 5, 6, 7, 8, 16):
-        if pairs * s <= max(shares, 148) and chunks >= s:
-            best = s
     return best
 
 
