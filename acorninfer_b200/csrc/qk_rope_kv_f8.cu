@@ -12,8 +12,8 @@
 // a lane takes eight entries of a head (16 bytes in; 16 or 8 out), LPH lanes a head, so that the sum of squares and the
 // largest magnitude are shuffles among them.  Heads rotated whole in pairs (j, j + d/2) give a lane four entries of each half, so
 // that it holds whole pairs (PAIRED); otherwise the eight are neighbours, and the other half of a pair is a shuffle more.
-// What bounds it: its instructions, not its bytes; so only the key and value heads look for their largest magnitude, as an
-// integer maximum over the bits, which also tells infinities and NaN.
+// What bounds it: its instructions, not its bytes; so only the key and value heads look for their largest magnitude, by a
+// maximum that hands NaN on, which tells infinities and NaN as well.
 // The angle is formed and brought to [-pi, pi] in 64 bits: in 32 its error is 2^-24 of the angle itself, 0.008 radians at
 // position 131,072, against 2^-9 of a rounding to bfloat16.
 #include "f8_cache.cuh"
@@ -36,8 +36,8 @@ struct KvF8Params {
     uint8_t* scales;
     bf16* q_out;
     int64_t ld_q;
-    int table_stride, nq, nkv, d, rot, interleaved, P;
-    float eps, magnitude;
+    int tokens, table_stride, nq, nkv, d, rot, interleaved, logP;
+    float inv_d, eps, magnitude;
 };
 
 __device__ __forceinline__ void kvf8_unpack(const uint4& raw, float (&x)[8]) {
@@ -54,16 +54,27 @@ __device__ __forceinline__ uint2 kvf8_pack4(float a, float b, float c, float d) 
     return make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
 }
 
-// Eight entries as codes: times inv, or zeros.
-__device__ __forceinline__ uint2 kvf8_codes(const float (&x)[8], float inv, float limit) {
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// Eight entries times 2^-e as codes.  At the largest exponent a code above 240 would stand for more than the largest float.
+__device__ __forceinline__ uint2 kvf8_codes(const float (&x)[8], int e) {
     float z[8];
+    const float inv = f8_pow2(-e);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) z[i] = fminf(fmaxf(x[i] * inv, -limit), limit);
+    for (int i = 0; i < 8; ++i) z[i] = x[i] * inv;
+    if (e == F8_MAX_EXP) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[i] = fminf(fmaxf(z[i], -240.f), 240.f);
+    }
     return make_uint2(f8_pack2(z[0], z[1]) | f8_pack2(z[2], z[3]) << 16, f8_pack2(z[4], z[5]) | f8_pack2(z[6], z[7]) << 16);
 }
 
 template <int LPH, bool PAIRED>
-__global__ void __launch_bounds__(KVF8_THREADS) qk_rope_kv_f8_kernel(const KvF8Params p) {
+__global__ void __launch_bounds__(KVF8_THREADS, 8) qk_rope_kv_f8_kernel(const KvF8Params p) {
     extern __shared__ __align__(16) float2 turn[];            // cos and sin of the token's angles
     pdl_wait();
     pdl_trigger();
@@ -78,15 +89,15 @@ __global__ void __launch_bounds__(KVF8_THREADS) qk_rope_kv_f8_kernel(const KvF8P
     const bf16* row = p.qkv + (int64_t)t * p.ld;
     auto fetch = [&](int h) {
         if (!on || h >= heads) return make_uint4(0u, 0u, 0u, 0u);
-        const bf16* src = row + (int64_t)h * p.d;
+        const bf16* src = row + h * p.d;
         const uint2 a = *reinterpret_cast<const uint2*>(src + at0), b = *reinterpret_cast<const uint2*>(src + at1);
         return make_uint4(a.x, a.y, b.x, b.y);
     };
-    const int per_pass = KVF8_THREADS / LPH * gridDim.y, in_pass = threadIdx.x / LPH;
-    int h0 = blockIdx.y * (KVF8_THREADS / LPH);
+    const int in_pass = threadIdx.x / LPH, per_cta = blockDim.x / LPH, per_pass = per_cta * gridDim.y;
+    int h0 = blockIdx.y * per_cta;
     uint4 raw = fetch(h0 + in_pass);                          // on its way while the angles are made
-    const int page = p.block_table[(int64_t)r * p.table_stride + (pos / p.P - p.page_base[r])];
-    for (int j = threadIdx.x; j < half; j += KVF8_THREADS) {
+    const int page = p.block_table[(int64_t)r * p.table_stride + ((pos >> p.logP) - p.page_base[r])];
+    for (int j = threadIdx.x; j < half; j += blockDim.x) {
         const double a = (double)pos * (double)p.inv_freq[j];
         const double z = fma(-rint(a * 0.15915494309189535), 6.283185307179586, a);
         float s, c;
@@ -94,7 +105,7 @@ __global__ void __launch_bounds__(KVF8_THREADS) qk_rope_kv_f8_kernel(const KvF8P
         turn[j] = make_float2(c * p.magnitude, s * p.magnitude);
     }
     __syncthreads();
-    const int64_t slot0 = (int64_t)page * p.nkv * p.P + pos % p.P;
+    const int64_t slot0 = (((int64_t)page * p.nkv) << p.logP) + (pos & ((1 << p.logP) - 1));
     for (; h0 < heads; h0 += per_pass) {                      // the same trips for all lanes of a warp
         const int h = h0 + in_pass;
         const bool live = on && h < heads;
@@ -114,7 +125,7 @@ __global__ void __launch_bounds__(KVF8_THREADS) qk_rope_kv_f8_kernel(const KvF8P
 #pragma unroll
             for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
             if (w && live) {
-                const float inv = rsqrtf(ss / (float)p.d + p.eps);
+                const float inv = rsqrtf(fmaf(ss, p.inv_d, p.eps));
                 const float4 wa = *reinterpret_cast<const float4*>(w + at0), wb = *reinterpret_cast<const float4*>(w + at1);
                 x[0] *= inv * wa.x; x[1] *= inv * wa.y; x[2] *= inv * wa.z; x[3] *= inv * wa.w;
                 x[4] *= inv * wb.x; x[5] *= inv * wb.y; x[6] *= inv * wb.z; x[7] *= inv * wb.w;
@@ -166,11 +177,11 @@ __global__ void __launch_bounds__(KVF8_THREADS) qk_rope_kv_f8_kernel(const KvF8P
             }
             continue;
         }
-        uint32_t most = 0u;
+        float most = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
+        for (int i = 0; i < 8; ++i) most = max_nan(most, fabsf(x[i]));
 #pragma unroll
-        for (int o = LPH / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+        for (int o = LPH / 2; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
         if (!live) continue;
         if (h < p.nq) {
             bf16* dst = p.q_out + (int64_t)t * p.ld_q + (int64_t)h * p.d;
@@ -178,11 +189,10 @@ __global__ void __launch_bounds__(KVF8_THREADS) qk_rope_kv_f8_kernel(const KvF8P
             *reinterpret_cast<uint2*>(dst + at1) = kvf8_pack4(x[4], x[5], x[6], x[7]);
             continue;
         }
-        const int64_t slot = slot0 + (int64_t)((h - p.nq) % p.nkv) * p.P;
-        const bool finite = most < 0x7f800000u;
-        const int e = f8_row_exponent(__uint_as_float(most));
-        // at the largest exponent a code above 240 would stand for more than the largest float
-        const uint2 c = finite ? kvf8_codes(x, f8_pow2(-e), e == F8_MAX_EXP ? 240.f : 448.f) : make_uint2(0u, 0u);
+        const int64_t slot = slot0 + ((h - p.nq - (is_v ? p.nkv : 0)) << p.logP);
+        const bool finite = most <= 3.402823466e38f;
+        const int e = f8_row_exponent(most);
+        const uint2 c = finite ? kvf8_codes(x, e) : make_uint2(0u, 0u);
         uint8_t* dst = (is_v ? p.v_pages : p.k_pages) + slot * p.d;
         if constexpr (PAIRED) {
             *reinterpret_cast<uint32_t*>(dst + at0) = c.x;
@@ -194,13 +204,18 @@ __global__ void __launch_bounds__(KVF8_THREADS) qk_rope_kv_f8_kernel(const KvF8P
     }
 }
 
+template <int LPH, bool PAIRED>
+static int launch_kv_f8(const KvF8Params& p, cudaStream_t stream) {
+    // as few passes as 256 threads need, and as many threads as those passes leave no idle ones; few tokens: a CTA a pass
+    const int lanes = (p.nq + 2 * p.nkv) * LPH, passes = (lanes + KVF8_THREADS - 1) / KVF8_THREADS;
+    const int threads = ((lanes + passes - 1) / passes + 31) / 32 * 32;
+    return acorn_launch(qk_rope_kv_f8_kernel<LPH, PAIRED>, dim3(p.tokens, p.tokens < 2 * acorn_sms() ? passes : 1), dim3(threads),
+                        (size_t)(p.rot / 2) * sizeof(float2), stream, p);
+}
+
 template <int LPH>
-static int launch_kv_f8(const KvF8Params& p, int tokens, cudaStream_t stream) {
-    const int per_cta = KVF8_THREADS / LPH, passes = (p.nq + 2 * p.nkv + per_cta - 1) / per_cta;
-    const size_t smem = (size_t)(p.rot / 2) * sizeof(float2);
-    const dim3 grid(tokens, tokens < 2 * acorn_sms() ? passes : 1);          // few tokens: a CTA for every pass over a token's heads
-    if (p.rot == p.d && !p.interleaved) return acorn_launch(qk_rope_kv_f8_kernel<LPH, true>, grid, dim3(KVF8_THREADS), smem, stream, p);
-    return acorn_launch(qk_rope_kv_f8_kernel<LPH, false>, grid, dim3(KVF8_THREADS), smem, stream, p);
+static int launch_kv_f8(const KvF8Params& p, cudaStream_t stream) {
+    return p.rot == p.d && !p.interleaved ? launch_kv_f8<LPH, true>(p, stream) : launch_kv_f8<LPH, false>(p, stream);
 }
 
 extern "C" int acorn_qk_rope_kv_f8(const void* qkv, int64_t ld, const float* q_w, const float* k_w, const float* bias,
@@ -209,22 +224,25 @@ extern "C" int acorn_qk_rope_kv_f8(const void* qkv, int64_t ld, const float* q_w
                                    void* q_out, int64_t ld_q, int tokens, int nq, int nkv, int d, int rot, int interleaved,
                                    int P, float eps, float magnitude, cudaStream_t stream) {
     if (tokens <= 0) return 0;
-    if (d < 8 || d % 8 || d > 256 || rot < 0 || rot > d || rot % (interleaved ? 2 : 16) || P < 1 || nq < 1 || nkv < 1 ||
+    if (d < 8 || d % 8 || d > 256 || rot < 0 || rot > d || rot % (interleaved ? 2 : 16) || P < 1 || (P & (P - 1)) || nq < 1 || nkv < 1 ||
         ld % 8 || ld_q % 8)
         return ACORN_ERR_UNSUPPORTED;
     KvF8Params p;
     p.qkv = (const bf16*)qkv; p.ld = ld; p.q_w = q_w; p.k_w = k_w; p.bias = bias; p.inv_freq = inv_freq; p.positions = positions;
     p.token_row = token_row; p.block_table = block_table; p.page_base = page_base; p.k_pages = (uint8_t*)k_pages;
     p.v_pages = (uint8_t*)v_pages; p.scales = (uint8_t*)scales; p.q_out = (bf16*)q_out; p.ld_q = ld_q; p.table_stride = table_stride;
-    p.nq = nq; p.nkv = nkv; p.d = d; p.rot = rot; p.interleaved = interleaved; p.P = P; p.eps = eps; p.magnitude = magnitude;
+    p.tokens = tokens; p.nq = nq; p.nkv = nkv; p.d = d; p.rot = rot; p.interleaved = interleaved; p.eps = eps; p.inv_d = 1.f / (float)d;
+    p.logP = 0;
+    while ((1 << p.logP) < P) ++p.logP;
+    p.magnitude = magnitude;
     int lph = 1;
     while (8 * lph < d) lph *= 2;
     switch (lph) {
-        case 1: return launch_kv_f8<1>(p, tokens, stream);
-        case 2: return launch_kv_f8<2>(p, tokens, stream);
-        case 4: return launch_kv_f8<4>(p, tokens, stream);
-        case 8: return launch_kv_f8<8>(p, tokens, stream);
-        case 16: return launch_kv_f8<16>(p, tokens, stream);
-        default: return launch_kv_f8<32>(p, tokens, stream);
+        case 1: return launch_kv_f8<1>(p, stream);
+        case 2: return launch_kv_f8<2>(p, stream);
+        case 4: return launch_kv_f8<4>(p, stream);
+        case 8: return launch_kv_f8<8>(p, stream);
+        case 16: return launch_kv_f8<16>(p, stream);
+        default: return launch_kv_f8<32>(p, stream);
     }
 }

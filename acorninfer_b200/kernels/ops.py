@@ -713,8 +713,8 @@ def qk_rope_kv_f8(qkv: torch.Tensor, q_weight32: torch.Tensor | None, k_weight32
     for w, n in ((q_weight32, "q_norm weight"), (k_weight32, "k_norm weight")):
         if w is not None:
             _check(w, n, torch.float32, 1)
-            if w.numel() != head_dim:
-                raise KernelError(f"{n} must have head_dim entries")
+            if w.numel() != head_dim or w.data_ptr() % 16:
+                raise KernelError(f"{n} must have head_dim entries, from a 16-byte boundary on")
     if bias32 is not None:
         _check(bias32, "bias", torch.float32, 1)
         if bias32.numel() != channels:
