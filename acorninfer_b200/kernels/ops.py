@@ -647,33 +647,36 @@ F8_SCALE = torch.float8_e8m0fnu     # its powers of two, a byte each
 F8_MAX_HEAD = 256
 
 
-def _check_f8_pages(what: str, k_pages: torch.Tensor, v_pages: torch.Tensor, scales: torch.Tensor, num_kv_heads: int,
+def _check_tensors(what: str, device: int, *tensors) -> None:
+    """``(tensor or None, name, dtype, dimensions)`` each: contiguous, and on the device of that index."""
+    for t, name, dtype, dims in tensors:
+        if t is not None and (t.get_device() != device or t.dtype is not dtype or t.dim() != dims or not t.is_contiguous()):
+            _check(t, name, dtype, dims)
+            raise KernelError(f"{what}: {name} is on {t.device}, other tensors on cuda:{device}")
+
+
+def _check_f8_pages(what: str, device: int, k_pages: torch.Tensor, v_pages: torch.Tensor, scales: torch.Tensor, num_kv_heads: int,
                     head_dim: int) -> int:
     """Checks the pages of an 8-bit cache and returns the page size."""
-    _check(k_pages, "k_pages", F8, 4)
-    _check(v_pages, "v_pages", F8, 4)
-    _check(scales, "scales", F8_SCALE, 4)
+    _check_tensors(what, device, (k_pages, "k_pages", F8, 4), (v_pages, "v_pages", F8, 4), (scales, "scales", F8_SCALE, 4))
     n, heads, P, d = k_pages.shape
-    if heads != num_kv_heads or d != head_dim or v_pages.shape != k_pages.shape or tuple(scales.shape) != (n, heads, P, 2):
+    if heads != num_kv_heads or d != head_dim or v_pages.shape != k_pages.shape or scales.shape != (n, heads, P, 2):
         raise KernelError(f"{what}: cache pages {tuple(k_pages.shape)} / {tuple(v_pages.shape)} / {tuple(scales.shape)} do not fit "
                           f"nkv={num_kv_heads}, d={head_dim} (scales: [pages, nkv, page, 2])")
     if P & (P - 1):
         raise KernelError(f"{what}: the page size must be a power of two, got {P}")
     if head_dim % 8 or not 8 <= head_dim <= F8_MAX_HEAD:
         raise KernelError(f"{what}: head sizes are multiples of 8 up to {F8_MAX_HEAD}, got {head_dim}")
-    if k_pages.data_ptr() % 16 or v_pages.data_ptr() % 16 or scales.data_ptr() % 16:
+    if (k_pages.data_ptr() | v_pages.data_ptr() | scales.data_ptr()) % 16:
         raise KernelError(f"{what}: the cache pages must start on 16-byte boundaries")
     return P
 
 
-def _stream_of(what: str, first: torch.Tensor, *others) -> int:
-    """The current stream's handle on the device of the given tensors, which must be one, and the current one."""
-    for t in others:
-        if t is not None and t.device != first.device:
-            raise KernelError(f"{what}: tensors on {first.device} and {t.device}")
-    if first.device.index != torch.cuda.current_device():
-        raise KernelError(f"{what}: tensors on {first.device}, the current device is cuda:{torch.cuda.current_device()}")
-    return torch.cuda.current_stream().cuda_stream if _raw_stream is None else _raw_stream(first.device.index)
+def _stream_of(what: str, device: int) -> int:
+    """The current stream's handle on the tensors' device, which must be the current one."""
+    if device != torch.cuda.current_device():
+        raise KernelError(f"{what}: tensors on cuda:{device}, the current device is cuda:{torch.cuda.current_device()}")
+    return torch.cuda.current_stream().cuda_stream if _raw_stream is None else _raw_stream(device)
 
 
 def qk_rope_kv_f8(qkv: torch.Tensor, q_weight32: torch.Tensor | None, k_weight32: torch.Tensor | None, inv_freq: torch.Tensor,
@@ -695,42 +698,38 @@ def qk_rope_kv_f8(qkv: torch.Tensor, q_weight32: torch.Tensor | None, k_weight32
     are multiples of 8 up to 256; ``rotary_dim`` is a multiple of 16 (of 2 with ``interleaved`` pairs)."""
     what = "qk_rope_kv_f8"
     _check(qkv, "qkv", torch.bfloat16, 2)
-    P = _check_f8_pages(what, k_pages, v_pages, scales, num_kv_heads, head_dim)
-    T, channels = qkv.shape[0], (num_heads + 2 * num_kv_heads) * head_dim
-    if num_heads < 1 or num_kv_heads < 1 or qkv.shape[1] < channels or qkv.shape[1] % 8 or qkv.data_ptr() % 16:
-        raise KernelError(f"{what}: rows of {qkv.shape[1]} for {channels} channels (a multiple of 8, on 16-byte boundaries)")
+    device = qkv.get_device()
+    P = _check_f8_pages(what, device, k_pages, v_pages, scales, num_kv_heads, head_dim)
+    (T, width), channels = qkv.shape, (num_heads + 2 * num_kv_heads) * head_dim
+    if num_heads < 1 or num_kv_heads < 1 or width < channels or width % 8 or qkv.data_ptr() % 16:
+        raise KernelError(f"{what}: rows of {width} for {channels} channels (a multiple of 8, on 16-byte boundaries)")
     if not 0 <= rotary_dim <= head_dim or rotary_dim % (2 if interleaved else 16):
         raise KernelError(f"{what}: rotary_dim {rotary_dim} must be at most head_dim and a multiple of "
                           f"{2 if interleaved else 16}")
-    _check(inv_freq, "inv_freq", torch.float32, 1)
+    if out is None:
+        out = qkv.new_empty((T, num_heads * head_dim))
+    i32, f32 = torch.int32, torch.float32
+    _check_tensors(what, device, (inv_freq, "inv_freq", f32, 1), (positions, "positions", i32, 1), (token_row, "token_row", i32, 1),
+                   (page_base, "page_base", i32, 1), (block_table, "block_table", i32, 2), (q_weight32, "q_norm weight", f32, 1),
+                   (k_weight32, "k_norm weight", f32, 1), (bias32, "bias", f32, 1), (out, "out", torch.bfloat16, 2))
     if inv_freq.numel() != rotary_dim // 2:
         raise KernelError("inv_freq must have rotary_dim / 2 entries")
-    for t, n in ((positions, "positions"), (token_row, "token_row"), (page_base, "page_base")):
-        _check(t, n, torch.int32, 1)
-    _check(block_table, "block_table", torch.int32, 2)
-    if positions.numel() < T or token_row.numel() < T or page_base.numel() < block_table.shape[0]:
+    rows, table_stride = block_table.shape
+    if positions.numel() < T or token_row.numel() < T or page_base.numel() < rows:
         raise KernelError(f"{what}: positions and token_row need an entry per token, page_base one per row")
-    for w, n in ((q_weight32, "q_norm weight"), (k_weight32, "k_norm weight")):
-        if w is not None:
-            _check(w, n, torch.float32, 1)
-            if w.numel() != head_dim or w.data_ptr() % 16:
-                raise KernelError(f"{n} must have head_dim entries, from a 16-byte boundary on")
-    if bias32 is not None:
-        _check(bias32, "bias", torch.float32, 1)
-        if bias32.numel() != channels:
-            raise KernelError(f"{what}: bias has {bias32.numel()} entries for {channels} channels")
-    if out is None:
-        out = torch.empty((T, num_heads * head_dim), dtype=qkv.dtype, device=qkv.device)
-    _check(out, "out", torch.bfloat16, 2)
-    if out.shape[0] != T or out.shape[1] < num_heads * head_dim or out.shape[1] % 8 or out.data_ptr() % 16:
+    for w in (q_weight32, k_weight32):
+        if w is not None and (w.numel() != head_dim or w.data_ptr() % 16):
+            raise KernelError(f"{what}: a norm weight must have head_dim entries, from a 16-byte boundary on")
+    if bias32 is not None and bias32.numel() != channels:
+        raise KernelError(f"{what}: bias has {bias32.numel()} entries for {channels} channels")
+    out_rows, out_width = out.shape
+    if out_rows != T or out_width < num_heads * head_dim or out_width % 8 or out.data_ptr() % 16:
         raise KernelError(f"{what}: out {tuple(out.shape)} does not hold [{T}, {num_heads * head_dim}] in rows of a multiple of 8")
-    stream = _stream_of(what, qkv, q_weight32, k_weight32, inv_freq, positions, token_row, block_table, page_base, k_pages, v_pages,
-                        scales, bias32, out)
-    _ok(lib().acorn_qk_rope_kv_f8(qkv.data_ptr(), qkv.stride(0), _ptr(q_weight32), _ptr(k_weight32), _ptr(bias32),
-                                  inv_freq.data_ptr(), positions.data_ptr(), token_row.data_ptr(), block_table.data_ptr(),
-                                  page_base.data_ptr(), block_table.stride(0), k_pages.data_ptr(), v_pages.data_ptr(),
-                                  scales.data_ptr(), out.data_ptr(), out.stride(0), T, num_heads, num_kv_heads, head_dim,
-                                  rotary_dim, 1 if interleaved else 0, P, float(eps), float(magnitude), stream), what)
+    _ok(lib().acorn_qk_rope_kv_f8(qkv.data_ptr(), width, _ptr(q_weight32), _ptr(k_weight32), _ptr(bias32), inv_freq.data_ptr(),
+                                  positions.data_ptr(), token_row.data_ptr(), block_table.data_ptr(), page_base.data_ptr(), table_stride,
+                                  k_pages.data_ptr(), v_pages.data_ptr(), scales.data_ptr(), out.data_ptr(), out_width, T, num_heads,
+                                  num_kv_heads, head_dim, rotary_dim, 1 if interleaved else 0, P, float(eps), float(magnitude),
+                                  _stream_of(what, device)), what)
     return out
 
 
@@ -1150,33 +1149,34 @@ def decode_f8_splits(tiles: int, num_kv_heads: int, key_bound: int, head_dim: in
 def _check_f8_attention(what: str, q, q_stride, k_pages, v_pages, scales, block_table, page_base, row_start, row_pos, tiles, num_tokens,
                         num_heads, num_kv_heads, head_dim, window, out, chunk, keep_first, sink32):
     """Checks the arguments that the attention kernels over an 8-bit cache share; returns (page size, out, stream)."""
-    if q.dtype != torch.bfloat16 or not q.is_cuda or q.stride(-1) != 1:
+    device = q.get_device()
+    if q.dtype is not torch.bfloat16 or device < 0 or q.stride(-1) != 1:
         raise KernelError(f"{what} takes bfloat16 queries on the device, rows of neighbouring entries")
     if num_kv_heads < 1 or num_heads < 1 or num_heads % num_kv_heads:
         raise KernelError("num_heads must be a multiple of num_kv_heads")
-    P = _check_f8_pages(what, k_pages, v_pages, scales, num_kv_heads, head_dim)
+    P = _check_f8_pages(what, device, k_pages, v_pages, scales, num_kv_heads, head_dim)
     width = num_heads * head_dim
-    if q_stride < width or q_stride % 8 or q.data_ptr() % 16 or (num_tokens > 0 and q.untyped_storage().nbytes() // 2 <
-                                                                 q.storage_offset() + (num_tokens - 1) * q_stride + width):
+    if q_stride < width or q_stride % 8 or q.data_ptr() % 16 or num_tokens < 0 or (num_tokens > 0 and q.untyped_storage().nbytes() // 2 <
+                                                                                   q.storage_offset() + (num_tokens - 1) * q_stride + width):
         raise KernelError(f"{what}: q must hold {num_tokens} rows of {width} entries, a multiple of 8 entries apart, from a 16-byte "
                           "boundary on")
-    for t, n in ((page_base, "page_base"), (row_start, "row_start"), (row_pos, "row_pos")):
-        _check(t, n, torch.int32, 1)
-    _check(block_table, "block_table", torch.int32, 2)
-    _check(tiles, "tiles", torch.int32, 2)
+    if out is None:
+        out = q.new_empty((num_tokens, width))
+    i32 = torch.int32
+    _check_tensors(what, device, (page_base, "page_base", i32, 1), (row_start, "row_start", i32, 1), (row_pos, "row_pos", i32, 1),
+                   (block_table, "block_table", i32, 2), (tiles, "tiles", i32, 2), (out, "out", torch.bfloat16, 2),
+                   (sink32, "sink", torch.float32, 1))
     rows = block_table.shape[0]
     if page_base.numel() < rows or row_pos.numel() < rows or row_start.numel() < rows + 1 or tiles.shape[1] != 2:
         raise KernelError(f"{what}: page_base and row_pos need an entry per row, row_start one more, tiles two columns")
-    for v, n in ((window, "window"), (chunk, "chunk"), (keep_first, "keep_first")):
-        if v is not None and v < 0:
-            raise KernelError(f"{what}: {n} must not be negative, got {v}")
-    _check_sink(sink32, num_heads)
-    if out is None:
-        out = torch.empty((num_tokens, width), dtype=q.dtype, device=q.device)
-    _check(out, "out", torch.bfloat16, 2)
-    if out.shape[0] < num_tokens or out.shape[1] != width or out.data_ptr() % 16:
+    if (window or 0) < 0 or (chunk or 0) < 0 or (keep_first or 0) < 0:
+        raise KernelError(f"{what}: window, chunk and keep_first must not be negative, got {window}, {chunk}, {keep_first}")
+    if sink32 is not None and sink32.numel() != num_heads:
+        raise KernelError("sink must have one entry per query head")
+    out_rows, out_width = out.shape
+    if out_rows < num_tokens or out_width != width or out.data_ptr() % 16:
         raise KernelError(f"{what}: out {tuple(out.shape)} does not hold [{num_tokens}, {width}]")
-    return P, out, _stream_of(what, q, k_pages, v_pages, scales, block_table, page_base, row_start, row_pos, tiles, out, sink32)
+    return P, out, _stream_of(what, device)
 
 
 def _attention_f8_plain(q, q_stride, out, k_pages, v_pages, scales, block_table, page_base, row_start, row_pos, tiles, tile_tokens,
