@@ -1127,7 +1127,8 @@ def decode_f8_splits(tiles: int, num_kv_heads: int, key_bound: int, head_dim: in
     """How ``attention_decode_f8`` cuts its work: into even shares (0) for ``shares`` CTAs, or into so many parts a (tile, kv
     head).  By estimates in us, fitted to 1 to 128 rows of 8 kv heads with 300 to 131,072 keys, which they meet to some 20 %: a
     CTA's start and end take 6, a chunk of 64 keys 0.8 in a CTA (its warps' latencies), all of them together 6.1 TB/s; clusters run in
-    one wave up to 400 CTAs, of sixteen up to 256 (8 rows of 4,000 keys: 6 parts, 384 CTAs, 18.9, 7 parts 28.4); shares take 12
+    one wave up to 0.9 of the CTAs that the device holds, of sixteen up to 0.57 (444 of them, 8 rows of 4,000 keys: 6 parts, 384 CTAs,
+    18.9, 7 parts 28.4; 4 rows of 300: 8 parts 7.4, 16 14.4); shares take 12
     and 3 a pair that a CTA comes to (64 rows of 4,096 keys: 101, whole 124, in 3 parts 114; 41 of 600 to 1,700: 34.5, whole 30;
     one of 131,072: 61, in 16 parts 105)."""
     pairs, chunks = max(1, tiles * num_kv_heads), -(-key_bound // 64)
@@ -1135,7 +1136,7 @@ def decode_f8_splits(tiles: int, num_kv_heads: int, key_bound: int, head_dim: in
     stream_us = pairs * chunks * (128 * head_dim + 128) / 6.1e6
     best, best_us = 1, None
     for s in (1, 2, 3, 4, 5, 6, 7, 8, 16):
-        if s > chunks or (s > 1 and pairs * s > (256 if s == 16 else 400)):
+        if s > chunks or (s > 1 and pairs * s > (0.57 if s == 16 else 0.9) * at_once):
             continue
         us = -(-pairs * s // at_once) * (6.0 + -(-chunks // s) * 0.8) + (0.5 if s > 1 else 0.0)
         us = max(us, 6.0 + stream_us)
