@@ -100,9 +100,10 @@ __global__ void __launch_bounds__(KVF8_THREADS, 8) qk_rope_kv_f8_kernel(const Kv
     for (int j = threadIdx.x; j < half; j += blockDim.x) {
         const double a = (double)pos * (double)p.inv_freq[j];
         const double z = fma(-rint(a * 0.15915494309189535), 6.283185307179586, a);
+        const float zh = (float)z, zl = (float)(z - (double)zh);         // sin(zh + zl) = sin zh + zl cos zh, zl < 2^-23
         float s, c;
-        sincosf((float)z, &s, &c);
-        turn[j] = make_float2(c * p.magnitude, s * p.magnitude);
+        sincosf(zh, &s, &c);
+        turn[j] = make_float2(fmaf(-s, zl, c) * p.magnitude, fmaf(c, zl, s) * p.magnitude);
     }
     __syncthreads();
     const int64_t slot0 = (((int64_t)page * p.nkv) << p.logP) + (pos & ((1 << p.logP) - 1));
@@ -125,7 +126,9 @@ __global__ void __launch_bounds__(KVF8_THREADS, 8) qk_rope_kv_f8_kernel(const Kv
 #pragma unroll
             for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
             if (w && live) {
-                const float inv = rsqrtf(fmaf(ss, p.inv_d, p.eps));
+                const float mean = fmaf(ss, p.inv_d, p.eps), guess = rsqrtf(mean);
+                // a Newton step: codes flip where an entry lies near the middle of two, so that every bit counts
+                const float inv = mean > 1e-30f ? fmaf(0.5f * guess, fmaf(-mean * guess, guess, 1.f), guess) : guess;
                 const float4 wa = *reinterpret_cast<const float4*>(w + at0), wb = *reinterpret_cast<const float4*>(w + at1);
                 x[0] *= inv * wa.x; x[1] *= inv * wa.y; x[2] *= inv * wa.z; x[3] *= inv * wa.w;
                 x[4] *= inv * wb.x; x[5] *= inv * wb.y; x[6] *= inv * wb.z; x[7] *= inv * wb.w;
