@@ -84,7 +84,9 @@ __device__ __forceinline__ int f8_slot_key(const F8AttnParams& p, int r) { retur
 
 #define RB_THREADS 256
 
-// One CTA per (block of 128 keys, kv head of the pass, slot); 16 codes a thread at a time.
+// A CTA takes a part of a block of 128 keys, 16 codes of a key and of its value a thread, of one kv head of the pass and one
+// slot: a call of 2,048 tokens has some hundreds of CTAs then, whose chains of lookups overlap (a whole block a CTA: 10.9 us, 3 of
+// them the bytes).
 template <int D>
 __global__ void __launch_bounds__(RB_THREADS) read_pages_f8_kernel(const PrefillF8Params pp) {
     const F8AttnParams& p = pp.a;
@@ -99,39 +101,36 @@ __global__ void __launch_bounds__(RB_THREADS) read_pages_f8_kernel(const Prefill
     const F8Blocks b(p.mask, p.row_pos[r], p.row_start[r + 1] - p.row_start[r]);
     const int* table = p.block_table + (int64_t)r * p.table_stride - p.page_base[r];
     const int first_key = p.page_base[r] << p.logP, slot_key = f8_slot_key(p, r), pmask = (1 << p.logP) - 1;
-    constexpr int PIECES = D / 16;
-    for (int j = blockIdx.x; j < b.n; j += gridDim.x) {
-        const int key0 = b.key0(j);
+    constexpr int PIECES = D / 16, KEYS = RB_THREADS / PIECES, PARTS = PF8_BN / KEYS;
+    const int piece = threadIdx.x % PIECES;
+    for (int part = blockIdx.x; part < b.n * PARTS; part += gridDim.x) {
+        const int key0 = b.key0(part / PARTS), key = key0 + part % PARTS * KEYS + threadIdx.x / PIECES;
         if (key0 < slot_key) continue;                               // (a kept block whose pages are gone)
-        const int64_t out0 = ((int64_t)(slot * pp.kvhs + blockIdx.y) * pp.cap + (key0 - slot_key)) * D;
-#pragma unroll 2
-        for (int idx = threadIdx.x; idx < PF8_BN * PIECES; idx += RB_THREADS) {
-            const int row = idx / PIECES, piece = idx % PIECES, key = key0 + row;
-            uint4 kc = make_uint4(0u, 0u, 0u, 0u), vc = kc;
-            float ks = 0.f, vs = 0.f;
-            if (key >= first_key && key < b.hi) {
-                const int64_t at = (((int64_t)table[key >> p.logP] * p.nkv + kvh) << p.logP) + (key & pmask);
-                kc = *reinterpret_cast<const uint4*>(p.k_pages + at * D + 16 * piece);
-                vc = *reinterpret_cast<const uint4*>(p.v_pages + at * D + 16 * piece);
-                const uint32_t bytes = *reinterpret_cast<const uint16_t*>(p.scales + 2 * at);
-                ks = f8_scale(bytes & 255u);
-                vs = f8_scale(bytes >> 8);
-                if (isnan(ks) || isnan(vs)) { ks = __uint_as_float(0x7fc00000u); vs = 0.f; }
-            }
-            const uint32_t kw[4] = {kc.x, kc.y, kc.z, kc.w}, vw[4] = {vc.x, vc.y, vc.z, vc.w};
-            uint32_t ko[8], vo[8];
-#pragma unroll
-            for (int q = 0; q < 8; ++q) {
-                const float2 a = f8_codes2(kw[q >> 1] >> (16 * (q & 1))), c = f8_codes2(vw[q >> 1] >> (16 * (q & 1)));
-                const __nv_bfloat162 ab = __floats2bfloat162_rn(a.x * ks, a.y * ks), cb = __floats2bfloat162_rn(c.x * vs, c.y * vs);
-                ko[q] = *reinterpret_cast<const uint32_t*>(&ab);
-                vo[q] = *reinterpret_cast<const uint32_t*>(&cb);
-            }
-            uint4* kd = reinterpret_cast<uint4*>(pp.k_rows + out0 + (int64_t)row * D + 16 * piece);
-            uint4* vd = reinterpret_cast<uint4*>(pp.v_rows + out0 + (int64_t)row * D + 16 * piece);
-            kd[0] = make_uint4(ko[0], ko[1], ko[2], ko[3]); kd[1] = make_uint4(ko[4], ko[5], ko[6], ko[7]);
-            vd[0] = make_uint4(vo[0], vo[1], vo[2], vo[3]); vd[1] = make_uint4(vo[4], vo[5], vo[6], vo[7]);
+        uint4 kc = make_uint4(0u, 0u, 0u, 0u), vc = kc;
+        float ks = 0.f, vs = 0.f;
+        if (key >= first_key && key < b.hi) {
+            const int64_t at = (((int64_t)table[key >> p.logP] * p.nkv + kvh) << p.logP) + (key & pmask);
+            kc = *reinterpret_cast<const uint4*>(p.k_pages + at * D + 16 * piece);
+            vc = *reinterpret_cast<const uint4*>(p.v_pages + at * D + 16 * piece);
+            const uint32_t bytes = *reinterpret_cast<const uint16_t*>(p.scales + 2 * at);
+            ks = f8_scale(bytes & 255u);
+            vs = f8_scale(bytes >> 8);
+            if (isnan(ks) || isnan(vs)) { ks = __uint_as_float(0x7fc00000u); vs = 0.f; }
         }
+        const uint32_t kw[4] = {kc.x, kc.y, kc.z, kc.w}, vw[4] = {vc.x, vc.y, vc.z, vc.w};
+        uint32_t ko[8], vo[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            const float2 a = f8_codes2(kw[q >> 1] >> (16 * (q & 1))), c = f8_codes2(vw[q >> 1] >> (16 * (q & 1)));
+            const __nv_bfloat162 ab = __floats2bfloat162_rn(a.x * ks, a.y * ks), cb = __floats2bfloat162_rn(c.x * vs, c.y * vs);
+            ko[q] = *reinterpret_cast<const uint32_t*>(&ab);
+            vo[q] = *reinterpret_cast<const uint32_t*>(&cb);
+        }
+        const int64_t out = ((int64_t)(slot * pp.kvhs + blockIdx.y) * pp.cap + (key - slot_key)) * D + 16 * piece;
+        uint4* kd = reinterpret_cast<uint4*>(pp.k_rows + out);
+        uint4* vd = reinterpret_cast<uint4*>(pp.v_rows + out);
+        kd[0] = make_uint4(ko[0], ko[1], ko[2], ko[3]); kd[1] = make_uint4(ko[4], ko[5], ko[6], ko[7]);
+        vd[0] = make_uint4(vo[0], vo[1], vo[2], vo[3]); vd[1] = make_uint4(vo[4], vo[5], vo[6], vo[7]);
     }
 }
 
@@ -563,7 +562,7 @@ static int launch_prefill_f8(const PrefillF8Params& pp, int tokens, int slots, i
 }
 
 // `slots`: min(rows of the table, tiles); k_rows / v_rows: [slots, kvhs, cap, d] bfloat16 for the kv heads kvh0 .. kvh0 + kvhs - 1
-// of this pass; blocks: CTAs along a row's blocks of 128 keys.
+// of this pass; blocks: CTAs along a row's keys.
 extern "C" int acorn_attention_prefill_f8(const void* q, int64_t q_stride, int tokens, void* out, const void* k_pages,
                                           const void* v_pages, const void* scales, const int* block_table, const int* page_base,
                                           int table_stride, int rows, const int* row_start, const int* row_pos, const int* tiles,

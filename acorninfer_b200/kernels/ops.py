@@ -1284,7 +1284,7 @@ def attention_prefill_f8(q: torch.Tensor, q_stride: int, k_pages: torch.Tensor, 
                                              rows, row_start.data_ptr(), row_pos.data_ptr(), tiles.data_ptr(), n, num_heads,
                                              num_kv_heads, head_dim, P, float(scale), int(window or 0), int(chunk or 0),
                                              int(keep_first or 0), _ptr(sink32), first, min(kvhs, num_kv_heads - first),
-                                             scratch[0].data_ptr(), scratch[1].data_ptr(), slots, cap, min(cap // 128, 1024), num_splits,
+                                             scratch[0].data_ptr(), scratch[1].data_ptr(), slots, cap, min(cap // 32, 4096), num_splits,
                                              _ptr(part_o), _ptr(part_lse), stream), what)
     return out
 
