@@ -22,6 +22,7 @@
 // g_gemm_tc_error, skips the rest of its work, still frees its tensor memory and returns.
 #include <cooperative_groups.h>
 
+#include "f8_cache.cuh"
 #include "tcgen05_helpers.cuh"
 
 namespace cg = cooperative_groups;
@@ -71,6 +72,7 @@ struct TcParams {
     const float* inv_freq;   // [64]
     bf16* k_pages;
     bf16* v_pages;           // nullptr: keys and values are not written (a layer that reads another's cache)
+    uint8_t* scales;         // [page, nkv, P, 2]: the pages hold e4m3 codes and these their rows' powers of two (f8_cache.cuh); or nullptr
     int table_stride, nq, nkv, logP;
     float rope_eps;
     // TC_MODE_GELU_ROWS: row gate_ids[m] of gate_rows ([rows, gate_ld] bf16), columns from gate_col0
@@ -377,11 +379,30 @@ __global__ void __launch_bounds__(TC_THREADS) gemm_tcgen05_kernel(const __grid_c
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     float sn, cs;
-                    sincosf((float)pos_s[m] * freq[j], &sn, &cs);
+                    float angle = (float)pos_s[m] * freq[j];
+                    if (p.scales != nullptr) {               // an 8-bit cache: as qk_rope_kv_f8.cu makes it, right at far positions too
+                        const double far = (double)pos_s[m] * (double)freq[j];
+                        angle = (float)fma(-rint(far * 0.15915494309189535), 6.283185307179586, far);
+                    }
+                    sincosf(angle, &sn, &cs);
                     const float a = v[j], b = v[j + 2];
                     v[j] = a * cs - b * sn;
                     v[j + 2] = b * cs + a * sn;
                 }
+            }
+            if (!is_q && p.scales != nullptr) {              // a key or value row of an 8-bit cache
+                const int64_t slot = (((int64_t)slot_s[2 * m] * p.nkv + kvh) << p.logP) + slot_s[2 * m + 1];
+                const uint32_t most = __reduce_max_sync(0xffffffffu, max(max(__float_as_uint(v[0]) & 0x7fffffffu, __float_as_uint(v[1]) & 0x7fffffffu),
+                                                                         max(__float_as_uint(v[2]) & 0x7fffffffu, __float_as_uint(v[3]) & 0x7fffffffu)));
+                const bool finite = most < 0x7f800000u;
+                const int e = f8_row_exponent(__uint_as_float(most));
+                const float down = f8_pow2(-e), limit = e == F8_MAX_EXP ? 240.f : 448.f;
+                uint8_t* codes = reinterpret_cast<uint8_t*>(is_k ? p.k_pages : p.v_pages) + slot * TC_BM + lane;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    codes[32 * j] = finite ? (uint8_t)f8_pack2(fminf(fmaxf(v[j] * down, -limit), limit), 0.f) : 0;
+                if (lane == 0) p.scales[2 * slot + (is_k ? 0 : 1)] = (uint8_t)(finite ? e + 127 : F8_NAN_BYTE);
+                continue;
             }
             bf16* dst = nullptr;
             if (is_q) dst = reinterpret_cast<bf16*>(p.out) + (int64_t)t * p.ldo + head * TC_BM;
@@ -544,14 +565,16 @@ extern "C" int acorn_gemm_tc_gelu_rows(const void* x, int64_t ldx, const void* w
 
 // The q/k/v product of an attention layer with head size 128 (TC_MODE_QKV_ROPE): w is [(nq + 2 nkv)
 // * 128, K]; out [M, ldo] takes the query heads; k_pages / v_pages ([pages, nkv, P, 128], P a power
-// of two) the keys and values, or nothing when they are nullptr.
+// of two) the keys and values, or nothing when they are nullptr.  With scales ([pages, nkv, P, 2]) the pages are those of an 8-bit
+// cache: e4m3 codes, and their rows' powers of two.
 extern "C" int acorn_gemm_tc_qkv_rope(const void* x, int64_t ldx, const void* w, int64_t ldw, void* out, int64_t ldo,
                                       int M, int K, int splits, int per_sm, const float* ss_in, int ss_parts,
                                       int norm_width, float eps, const int* positions, const int* token_row,
                                       const int* block_table, const int* page_base, int table_stride, void* k_pages,
-                                      void* v_pages, const float* q_w, const float* k_w, const float* inv_freq, int nq,
+                                      void* v_pages, void* scales, const float* q_w, const float* k_w, const float* inv_freq, int nq,
                                       int nkv, int P, float rope_eps, cudaStream_t stream) {
     const int logP = acorn_log2_exact_tc(P);
+    if (scales != nullptr && v_pages == nullptr) return ACORN_ERR_UNSUPPORTED;
     if (nq < 1 || nkv < 1 || logP < 0 || positions == nullptr || inv_freq == nullptr) return ACORN_ERR_UNSUPPORTED;
     if ((k_pages == nullptr) != (v_pages == nullptr)) return ACORN_ERR_UNSUPPORTED;
     if (k_pages != nullptr && (token_row == nullptr || block_table == nullptr || page_base == nullptr)) return ACORN_ERR_UNSUPPORTED;
@@ -560,7 +583,7 @@ extern "C" int acorn_gemm_tc_qkv_rope(const void* x, int64_t ldx, const void* w,
     p.mode = TC_MODE_QKV_ROPE; p.ss_in = ss_in; p.ss_parts = ss_parts; p.norm_width = norm_width; p.eps = eps;
     p.positions = positions; p.token_row = token_row; p.block_table = block_table; p.page_base = page_base;
     p.table_stride = table_stride; p.k_pages = (bf16*)k_pages; p.v_pages = (bf16*)v_pages; p.q_w = q_w; p.k_w = k_w;
-    p.inv_freq = inv_freq; p.nq = nq; p.nkv = nkv; p.logP = logP; p.rope_eps = rope_eps;
+    p.scales = (uint8_t*)scales; p.inv_freq = inv_freq; p.nq = nq; p.nkv = nkv; p.logP = logP; p.rope_eps = rope_eps;
     return run_tc(x, ldx, w, ldw, p, splits, per_sm, stream);
 }
 

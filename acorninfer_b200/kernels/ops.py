@@ -283,7 +283,7 @@ class _Sigs:
                                c_void_p, c_void_p, c_int64, c_int, c_void_p]
     acorn_gemm_tc_qkv_rope = [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int, c_int,
                               c_void_p, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
-                              c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_void_p]
+                              c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_void_p]
     acorn_gemm_tc_supported = [c_int64, c_int64, c_int64, c_int64, c_int64]
     acorn_gemm_tc_pair = [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int,
                           c_int, c_void_p, c_int, c_int, c_float, c_void_p, c_int64, c_void_p, c_void_p, c_void_p]
@@ -1499,6 +1499,7 @@ class RopeKvEpilogue:
     num_kv_heads: int
     eps: float
     cos_sin: torch.Tensor | None = None      # [M, 128] float32 from ``rope_table``: spares the epilogue its sincosf
+    scales: torch.Tensor | None = None       # the pages are an 8-bit cache's, and these its rows' powers of two (``qk_rope_kv_f8``)
 
 
 def rope_table(positions: torch.Tensor, inv_freq: torch.Tensor) -> torch.Tensor:
@@ -1527,9 +1528,13 @@ def gemm_tc_qkv_rope(x, w: torch.Tensor, ep: RopeKvEpilogue, out: torch.Tensor |
     if ep.inv_freq.numel() != 64 or ep.positions.numel() < M:
         raise KernelError("gemm_tc_qkv_rope: inv_freq must have 64 entries and positions one per row")
     P = 1
+    if ep.scales is not None:
+        if M > GEMM_TC_FUSED_MAX_ROWS or ep.k_pages is None:
+            raise KernelError(f"gemm_tc_qkv_rope: up to {GEMM_TC_FUSED_MAX_ROWS} rows are written into an 8-bit cache, got {M}")
+        _check_f8_pages("gemm_tc_qkv_rope", xt.get_device(), ep.k_pages, ep.v_pages, ep.scales, nkv, 128)
     if ep.k_pages is not None:
-        _check(ep.k_pages, "k_pages", torch.bfloat16, 4)
-        _check(ep.v_pages, "v_pages", torch.bfloat16, 4)
+        _check(ep.k_pages, "k_pages", F8 if ep.scales is not None else torch.bfloat16, 4)
+        _check(ep.v_pages, "v_pages", F8 if ep.scales is not None else torch.bfloat16, 4)
         _check(ep.block_table, "block_table", torch.int32, 2)
         if tuple(ep.k_pages.shape[1:]) != (nkv, ep.k_pages.shape[2], 128) or ep.v_pages.shape != ep.k_pages.shape:
             raise KernelError("gemm_tc_qkv_rope: cache pages must be [pages, nkv, P, 128]")
@@ -1561,7 +1566,7 @@ def gemm_tc_qkv_rope(x, w: torch.Tensor, ep: RopeKvEpilogue, out: torch.Tensor |
         rows.ss.data_ptr() if rows is not None else None, rows.ss.shape[0] if rows is not None else 0,
         rows.width if rows is not None else 0, float(rows.eps) if rows is not None else 0.0,
         ep.positions.data_ptr(), _ptr(ep.token_row), _ptr(ep.block_table), _ptr(ep.page_base),
-        ep.block_table.stride(0) if ep.block_table is not None else 0, _ptr(ep.k_pages), _ptr(ep.v_pages),
+        ep.block_table.stride(0) if ep.block_table is not None else 0, _ptr(ep.k_pages), _ptr(ep.v_pages), _ptr(ep.scales),
         _ptr(ep.q_weight32), _ptr(ep.k_weight32), ep.inv_freq.data_ptr(), nq, nkv, P, float(ep.eps), _stream()),
         "gemm_tc_qkv_rope", f"{M}x{N}x{K}")
     return out

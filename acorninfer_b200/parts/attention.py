@@ -139,7 +139,6 @@ class Attention(Mixer):
                  and not self.position.interleaved and self.position.rotary_dim % 16 != 0)) if has]
             if refused:
                 raise ValueError(f"attention over an 8-bit cache does not go with {', '.join(refused)}")
-            self.plain = False
         self.gate_col = (self.nq + self.nkv) * self.d + (0 if values_from_keys else self.nkv * self.dv)
         self.w_qkv = self.w_o = self.q_norm32 = self.k_norm32 = None
 
@@ -241,6 +240,8 @@ class Attention(Mixer):
 
     def _rope_fuses(self, num_rows):
         pos = self.position
+        if self.eight_bit and num_rows > ops.GEMM_TC_FUSED_MAX_ROWS:       # the product of many rows writes bfloat16 pages only
+            return False
         return self.plain and pos is not None and ops.rope_kv_fusable(num_rows, self.ctx.dtype, self.d, pos.rotary_dim, pos.interleaved)
 
     def _tile_fuses(self, num_rows):
@@ -272,14 +273,16 @@ class Attention(Mixer):
                                              sink32=self.sink32, softcap=self.softcap)
         return heads if out is None else ops.head_gate(heads, None, self.nq, 1.0, out=out)
 
-    def _inner_f8(self, x, inputs, cache, out_scale, out):
-        """``inner`` over an 8-bit cache."""
+    def _inner_f8(self, x, inputs, cache, out_scale, out, qkv=None):
+        """``inner`` over an 8-bit cache; ``qkv``: rows whose queries are finished, their keys and values written."""
         g, pos = inputs.groups[cache.group], self.position
-        proj = ops.linear(x, self.w_qkv, out_dtype=self.ctx.dtype, inputs=inputs)
+        proj = None if qkv is not None else ops.linear(x, self.w_qkv, out_dtype=self.ctx.dtype, inputs=inputs)
         inv_freq = pos.inv_freq if pos is not None else _no_freq(self.ctx.device)
         rot, interleaved = (pos.rotary_dim, pos.interleaved) if pos is not None else (0, False)
         eps, magnitude = self.qk_norm_eps if self.qk_norm_eps is not None else 0.0, getattr(pos, "magnitude", 1.0)
-        if cache.write:
+        if qkv is not None:                   # the product's epilogue has done it
+            q = qkv
+        elif cache.write:
             q = ops.qk_rope_kv_f8(proj, self.q_norm32, self.k_norm32, inv_freq, inputs.positions, inputs.token_row, g.block_table,
                                   g.page_base, cache.k_pages, cache.v_pages, cache.scales, self.nq, self.nkv, self.d, rot, interleaved,
                                   eps, bias32=self.bias32, magnitude=magnitude)
@@ -304,8 +307,6 @@ class Attention(Mixer):
         ``fused``: the layer's other products fuse."""
         if self.norm_rows:
             return self._inner_norm_rows(x, inputs, cache, out_scale, out, proj)
-        if self.eight_bit:
-            return self._inner_f8(x, inputs, cache, out_scale, out)
         g = inputs.groups[cache.group]
         pos = self.position
         rows = x.x.shape[0] if isinstance(x, ops.NormedRows) else x.shape[0]
@@ -320,7 +321,12 @@ class Attention(Mixer):
                 cache.k_pages if cache.write else None, cache.v_pages if cache.write else None,
                 self.q_norm32, self.k_norm32, pos.inv_freq, self.nq, self.nkv,
                 self.qk_norm_eps if self.qk_norm_eps is not None else 0.0,
-                cos_sin=pos.table(inputs) if rows > ops.GEMM_TC_FUSED_MAX_ROWS and hasattr(pos, "table") else None))
+                cos_sin=pos.table(inputs) if rows > ops.GEMM_TC_FUSED_MAX_ROWS and hasattr(pos, "table") else None,
+                scales=cache.scales if cache.write else None))
+            if self.eight_bit:
+                return self._inner_f8(x, inputs, cache, out_scale, out, qkv)
+        elif self.eight_bit:
+            return self._inner_f8(x, inputs, cache, out_scale, out)
         elif self.bias or self.taps:
             if not cache.write:
                 raise ValueError("attention: biased or convolved projections need a cache of the run's own")

@@ -497,3 +497,70 @@ def test_attention_does_not_depend_on_the_other_rows(which, nq, nkv, d):
                  "row_start": torch.tensor([0, b - a], dtype=torch.int32, device=DEV), "row_pos": lay["row_pos"][r:r + 1],
                  "num_tokens": b - a}
         assert torch.equal(attend(which, q[a:b].contiguous(), cache, alone, [b - a], nq, nkv, d, 0.1, **kw), whole[a:b])
+
+
+@pytest.mark.parametrize("nq,nkv,K,qlens,norm,P", [(4, 2, 256, [7, 1, 5], True, 16), (6, 1, 520, [1, 1, 1, 1], False, 8), (2, 2, 2048, [30], True, 32),
+                                                   (8, 4, 1024, [3, 20], True, 16), (4, 2, 1024, [41, 1], True, 16), (1, 1, 64, [1], True, 1)])
+def test_write_as_the_epilogue_of_the_projection(nq, nkv, K, qlens, norm, P):
+    """The q/k/v product of few rows that norms, rotates, quantises and writes.  Its sums of K float32 terms are off by less than
+    K 2^-24 of the sum of their magnitudes; a key's norm divides by the row's own size, so that share of a row stays."""
+    o, d, eps = ops(), 128, 3e-6
+    befores = [0, 37, 131000, 15][:len(qlens)]
+    pages = sum(-(-(b + n) // P) for b, n in zip(befores, qlens)) + 5
+    lay = rows_layout(befores, qlens, P, pages, seed=2)
+    T = lay["num_tokens"]
+    g = torch.Generator().manual_seed(K)
+    x = torch.randn(T, K, generator=g).to(torch.bfloat16).to(DEV)
+    w = (torch.randn((nq + 2 * nkv) * d, K, generator=g) / K ** 0.5).to(torch.bfloat16).to(DEV)
+    norms = [(1 + 0.2 * torch.randn(d, generator=g)).to(DEV) if norm else None for _ in range(2)]
+    inv = (1.0 / (1e6 ** (torch.arange(0, d, 2, dtype=torch.float32) / d))).to(DEV)
+    cache = empty_cache(pages, nkv, P, d, byte=99)
+    out = o.gemm_tc_qkv_rope(x, w, o.RopeKvEpilogue(lay["positions"], lay["token_row"], lay["block_table"], lay["page_base"], cache[0], cache[1],
+                                                    norms[0], norms[1], inv, nq, nkv, eps, scales=cache[2]))
+    assert o.gemm_tc_error() == 0
+    proj = x.double() @ w.double().T
+    off = float((x.double().abs() @ w.double().abs().T).amax() * K * 2.0 ** -24)            # of an entry of the product
+    wq, wk, wv = write_wanted(proj, norms, None, inv, lay["positions"], nq, nkv, d, d, False, eps, 1.0)
+    # 1.6: the largest norm weight; a rotation adds two entries; a norm divides by the row's root mean square
+    size = proj.view(T, -1, d).square().mean(-1).sqrt().cpu()
+    move = 1.6 * 2 * off / (size if norm else torch.ones_like(size))
+    got = out[:, :nq * d].double().cpu().view(T, nq, d)
+    assert bool(((got - wq).abs() <= 2.0 ** -8 * wq.abs() + move[:, :nq, None] + 2.0 ** -19 * wq.abs().amax(-1, keepdim=True)).all())
+    at, used = 0, torch.zeros(pages, P, dtype=torch.bool)
+    for r, (held, n) in enumerate(zip(befores, qlens)):
+        kc, vc, kb, vb = rows_of(cache, lay["tables"][r], held + n, P)
+        for codes, byte, want, slack in ((kc, kb, wk, move[:, nq:nq + nkv]), (vc, vb, wv, torch.full((T, nkv), off))):
+            want, slack = want[at:at + n], slack[at:at + n]
+            codes, byte = codes[held:], byte[held:]
+            e, most = byte.double() - 127, want.abs().amax(-1)
+            assert bool((448 * torch.exp2(e) >= most - slack).all()) and bool((448 * torch.exp2(e - 1) < most + slack).all())
+            spacing = torch.exp2(torch.floor(torch.log2((want.abs() * torch.exp2(-e)[..., None]).clamp(min=2.0 ** -6))) - 3 + e[..., None])
+            assert bool(((f8.dequantise(codes, byte) - want).abs() <= spacing / 2 + 2 * slack[..., None]).all())
+        for p in range(held, held + n):
+            used[lay["tables"][r][p // P], p % P] = True
+        at += n
+    for t in cache[:2]:
+        assert int(t.view(torch.uint8).cpu().transpose(1, 2)[~used].sum()) == 0
+    assert bool((cache[2].view(torch.uint8).cpu().transpose(1, 2)[~used] == 99).all())
+
+
+def test_the_epilogue_writes_rows_that_are_no_numbers_as_such():
+    o, nq, nkv, d, K, T, P = ops(), 2, 2, 128, 256, 4, 16
+    x = torch.randn(T, K).to(torch.bfloat16).to(DEV)
+    w = (torch.randn((nq + 2 * nkv) * d, K) / 16).to(torch.bfloat16).to(DEV)
+    inv = (1.0 / (1e6 ** (torch.arange(0, d, 2, dtype=torch.float32) / d))).to(DEV)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    x[2, 5] = float("inf")
+    cache = empty_cache(1, nkv, P, d)
+    o.gemm_tc_qkv_rope(x, w, o.RopeKvEpilogue(torch.arange(T, **i32), torch.zeros(T, **i32), torch.zeros(1, 1, **i32), torch.zeros(1, **i32), cache[0],
+                                              cache[1], None, None, inv, nq, nkv, 0.0, scales=cache[2]))
+    s = cache[2].view(torch.uint8)[0, :, :T].cpu()
+    assert bool((s[:, 2] == 255).all()) and bool((s[:, [0, 1, 3]] < 255).all())
+    assert int(cache[0].view(torch.uint8)[0, :, 2].sum()) == int(cache[1].view(torch.uint8)[0, :, 2].sum()) == 0
+    with raises("8-bit"):                                                   # more rows than the kernel of few rows takes
+        many = torch.zeros(64, K, dtype=torch.bfloat16, device=DEV)
+        o.gemm_tc_qkv_rope(many, w, o.RopeKvEpilogue(torch.arange(64, **i32), torch.zeros(64, **i32), torch.zeros(1, 4, **i32), torch.zeros(1, **i32),
+                                                     cache[0], cache[1], None, None, inv, nq, nkv, 0.0, scales=cache[2]))
+    with raises():                                                          # bfloat16 pages with scales
+        o.gemm_tc_qkv_rope(x, w, o.RopeKvEpilogue(torch.arange(T, **i32), torch.zeros(T, **i32), torch.zeros(1, 1, **i32), torch.zeros(1, **i32),
+                                                  cache[0].bfloat16(), cache[1].bfloat16(), None, None, inv, nq, nkv, 0.0, scales=cache[2]))

@@ -124,8 +124,9 @@ def test_which_kernels_run(folders):
     a, b, c = runner.open("a"), runner.open("b"), runner.open("c")
     n = counts_of(lambda: runner.step([StepEntry(a, random_tokens(40, V, 1), [39]), StepEntry(b, random_tokens(5, V, 2), [4])]))
     assert n["qk_rope_kv_f8"] == n["attention_prefill_f8"] == n["attention_decode_f8"] == L
+    # two decoded tokens: norm, rotation and the cache write ride on the q/k/v product
     n = counts_of(lambda: runner.step([StepEntry(a, [3], [0]), StepEntry(b, [4], [0])]))
-    assert n["qk_rope_kv_f8"] == n["attention_decode_f8"] == L and "attention_prefill_f8" not in n
+    assert n["gemm_tc_qkv_rope"] == n["attention_decode_f8"] == L and "attention_prefill_f8" not in n and "qk_rope_kv_f8" not in n
     n = counts_of(lambda: runner.step([StepEntry(a, [3], [0]), StepEntry(b, [4, 5], [1]), StepEntry(c, random_tokens(33, V, 3), [])]))
     assert n["attention_decode_f8"] == 2 * L and n["attention_prefill_f8"] == L
     assert not any(k.startswith("attention_") and not k.endswith("_f8") for k in n) and "gemm_tc_qkv_rope" not in n
