@@ -72,6 +72,7 @@ template <int D, int NH> struct DecodeF8 {
     static constexpr int SCALES = BARS + 2 * STAGES * 8;
     static constexpr int RECV = SCALES + STAGES * SCALE_BYTES;        // received rows of a cluster, or the sizes of the tiles
     static constexpr int SHARES = (DF8_SHARE_TILES + 4) * 4 + DF8_SHARE_TILES * 16;       // chunks before a tile; row, first token, tokens, position
+    static_assert(RECV % 16 == 0 && MERGE % 16 == 0, "float4 and int4 accesses");
     // byte offset of the 16-byte piece `seg` of row `row` of a stage (boxes of 2^log_box keys, then as many values), as the
     // TMA's swizzle places it
     static __device__ __forceinline__ uint32_t at(int row, int seg) {
@@ -160,8 +161,13 @@ struct F8Walk {
     }
 };
 
-// Meets the compute warps.
-__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, %0;" :: "n"(32 * DF8_WARPS) : "memory"); }
+// Meets the compute warps; whether `v` holds for all of them.
+__device__ __forceinline__ bool compute_all(bool v) {
+    uint32_t r;
+    asm volatile("{\n .reg .pred a, b;\n setp.ne.u32 a, %1, 0;\n barrier.cta.red.and.pred b, 1, %2, a;\n selp.u32 %0, 1, 0, b;\n}\n"
+                 : "=r"(r) : "r"((uint32_t)v), "n"(32 * DF8_WARPS) : "memory");
+    return r != 0;
+}
 
 template <int D, int NH, bool SHARES>
 __global__ void __launch_bounds__(DF8_THREADS, NH == 1 ? 3 : 2) attention_decode_f8_kernel(const __grid_constant__ CUtensorMap map_k,
@@ -490,7 +496,7 @@ __global__ void __launch_bounds__(DF8_THREADS, NH == 1 ? 3 : 2) attention_decode
         float* sm_m = reinterpret_cast<float*>(smem + L::MERGE);  // [WARPS][ROWS]
         float* sm_l = sm_m + ROWS * DF8_WARPS;
         float* sm_o = sm_l + ROWS * DF8_WARPS;                    // [WARPS][ROWS][D]
-        compute_sync();                                           // the part before has been read
+        good = compute_all(good);                                 // the part before has been read; a wait that gave up ends the walk of all
 #pragma unroll
         for (int h = 0; h < NH; ++h)
 #pragma unroll
@@ -505,7 +511,7 @@ __global__ void __launch_bounds__(DF8_THREADS, NH == 1 ? 3 : 2) attention_decode
                     *reinterpret_cast<float4*>(sm_o + m * D + g * (D / 8) + 2 * n2) =
                         make_float4(o[h][n2][b], o[h][n2][2 + b], o[h][n2 + 1][b], o[h][n2 + 1][2 + b]);
             }
-        compute_sync();
+        compute_all(true);
         // received partial rows: recv[rank of the sender][slot][RECV_ROW]
         float* recv = reinterpret_cast<float*>(smem + L::RECV);
         const int csize = cluster ? dp.num_splits : 1;

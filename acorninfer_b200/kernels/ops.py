@@ -691,7 +691,8 @@ def qk_rope_kv_f8(qkv: torch.Tensor, q_weight32: torch.Tensor | None, k_weight32
     A key or value row of ``head_dim`` entries becomes e4m3 codes and a power of two 2^e, ``row = code * 2^e``: e is the
     smallest integer in -120..120 for which 448 * 2^e is not below the row's largest magnitude, a code the nearest e4m3
     number (ties to even; at e = 120 codes end at 240, so that every row stands for finite numbers).  A row with an
-    infinity or a NaN is stored as zeros with the scale NaN.  ``k_pages`` / ``v_pages``: float8_e4m3fn [pages, nkv, page, d];
+    infinity or a NaN is stored as zeros with the scale NaN, and whoever reads it gets NaN; the codes themselves are always
+    numbers (the attention kernels do not expect e4m3's two codes of NaN).  ``k_pages`` / ``v_pages``: float8_e4m3fn [pages, nkv, page, d];
     ``scales``: float8_e8m0fnu [pages, nkv, page, 2], a token's key scale and value scale.
 
     ``bias32`` (float32, an entry per channel of a row) is added first; ``magnitude``: a factor on cos and sin.  Head sizes

@@ -564,3 +564,57 @@ def test_the_epilogue_writes_rows_that_are_no_numbers_as_such():
     with raises():                                                          # bfloat16 pages with scales
         o.gemm_tc_qkv_rope(x, w, o.RopeKvEpilogue(torch.arange(T, **i32), torch.zeros(T, **i32), torch.zeros(1, 1, **i32), torch.zeros(1, **i32),
                                                   cache[0].bfloat16(), cache[1].bfloat16(), None, None, inv, nq, nkv, 0.0, scales=cache[2]))
+
+
+@pytest.mark.parametrize("which", ["decode", "prefill"])
+@pytest.mark.parametrize("d", [128, 64, 32])
+def test_attention_wherever_the_pages_lie(which, d):
+    """Value pages before the key pages in memory, far from them, and the key pages themselves as values."""
+    nq, nkv, P = 8, 2, 16
+    befores, qlens = [77, 500], [3, 40]
+    lay, (k, v, s), keys, values = random_cache(befores, qlens, nkv, d, P, 14)
+    q = torch.randn(43, nq * d).to(torch.bfloat16).to(DEV)
+    n = k.numel()
+    room = torch.zeros(3 * n, dtype=torch.uint8, device=DEV)
+    lower, upper = (room[i * n:(i + 1) * n].view(E4M3).view(k.shape) for i in (0, 2))
+    want = attend(which, q, (k, v, s), lay, qlens, nq, nkv, d, 0.1)
+    for kk, vv in ((lower, upper), (upper, lower)):
+        kk.view(torch.uint8).copy_(k.view(torch.uint8))
+        vv.view(torch.uint8).copy_(v.view(torch.uint8))
+        assert torch.equal(attend(which, q, (kk, vv, s), lay, qlens, nq, nkv, d, 0.1), want)
+    same = s.view(torch.uint8).clone()
+    same[..., 1] = same[..., 0]
+    got = attend(which, q, (k, k, same.view(E8M0)), lay, qlens, nq, nkv, d, 0.1)
+    check_attention(got, q, keys, keys, befores, qlens, nq, d, 0.1)
+
+
+def test_pools_beyond_4_gib():
+    """Rows whose bytes lie beyond 2^32 of their tensor: written, read by every kernel."""
+    nq, nkv, d, P = 4, 2, 128, 16
+    pages = (1 << 32) // (nkv * P * d) + 40
+    k = torch.empty((pages, nkv, P, d), dtype=torch.uint8, device=DEV).view(E4M3)
+    v = torch.empty((pages, nkv, P, d), dtype=torch.uint8, device=DEV).view(E4M3)
+    s = torch.empty((pages, nkv, P, 2), dtype=torch.uint8, device=DEV).view(E8M0)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    T = 200
+    table = torch.arange(pages - 1, pages - 15, -1, **i32)[None]
+    qkv, w, _, inv = write_inputs(T, nq, nkv, d, d, True, False, 5)
+    pos, row, base = torch.arange(T, **i32), torch.zeros(T, **i32), torch.zeros(1, **i32)
+    q = ops().qk_rope_kv_f8(qkv, w[0], w[1], inv, pos, row, table, base, k, v, s, nq, nkv, d, d, False, 1e-6)
+    small = empty_cache(14, nkv, P, d)
+    near = torch.arange(13, -1, -1, **i32)[None]
+    q2 = ops().qk_rope_kv_f8(qkv, w[0], w[1], inv, pos, row, near, base, *small, nq, nkv, d, d, False, 1e-6)
+    assert torch.equal(q, q2)
+    for far, close in zip((k, v, s), small):
+        assert torch.equal(far.view(torch.uint8)[pages - 12:, :, :8], close.view(torch.uint8)[2:, :, :8])
+    lay = {"page_base": base, "row_start": torch.tensor([0, T], **i32), "row_pos": torch.zeros(1, **i32), "num_tokens": T}
+    for which in ("decode", "prefill"):
+        far = attend(which, q, (k, v, s), {**lay, "block_table": table}, [T], nq, nkv, d, 0.1)
+        assert torch.equal(far, attend(which, q, small, {**lay, "block_table": near}, [T], nq, nkv, d, 0.1))
+    narrow = [t.view(torch.uint8).view(pages, nkv, 2 * P, -1) for t in (k, v)]                  # the same bytes as heads of 64 on the way to the
+    far32 = ops().attention_decode_f8(q[:, :nq * 64].contiguous(), nq * 64, *(t.view(E4M3) for t in narrow),      # general kernel: pages of 32
+                                      torch.full((pages, nkv, 2 * P, 2), 127, dtype=torch.uint8, device=DEV).view(E8M0), table, base,
+                                      lay["row_start"], lay["row_pos"], tiles_of([4], 4), T, nq, nkv, 64, 0.1, None)
+    assert bool(torch.isfinite(far32[:4]).all())
+    del k, v, s, narrow
+    torch.cuda.empty_cache()
