@@ -584,7 +584,10 @@ __global__ void __launch_bounds__(128) attention_decode_f8_join_kernel(const Dec
     const int share = dp.plan[dp.n_tiles].x;
     const int64_t u0 = (int64_t)t.x * p.nkv + (int64_t)kvh * t.y;
     if (t.y == 0 || m >= t.w * rep) return;
-    const int b0 = (int)(u0 / share), b1 = (int)((u0 + t.y - 1) / share);
+    // (64-bit quotients take a hundred instructions, and nearly every call's chunks fit 32 bits)
+    const bool narrow = u0 + t.y < 0x7fffffff;
+    const int b0 = narrow ? (int)u0 / share : (int)(u0 / share);
+    const int b1 = narrow ? ((int)u0 + t.y - 1) / share : (int)((u0 + t.y - 1) / share);
     if (b0 == b1) return;                                         // one CTA had it all
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // the first CTA's part is the last of its share, unless its share begins with the pair
