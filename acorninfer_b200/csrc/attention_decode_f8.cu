@@ -26,8 +26,13 @@
 //   even shares    as many CTAs as the device holds at once share all the chunks of 64 keys of all (tile, kv head) pairs out evenly,
 //                  in order, so that a CTA walks from pair to pair: nobody waits for the longest row or for a last wave of few CTAs, and
 //                  the codes of the next pair are on their way while the warps finish one (a CTA's start and end cost some 5
-//                  us).  A pair that several CTAs had parts of is joined by a second, small kernel.  64 rows of 4,096 keys: 128 us
-//                  whole, 114 in the best number of splits; figures of the shares below.
+//                  us).  A pair that several CTAs had parts of is joined by a second, small kernel (some 4 us).  64 rows of 4,096
+//                  keys of 8 kv heads of 128: 124 us whole, 114 in 3 splits, 99 in shares, 545 MB at 5.5 TB/s.
+// What bounds it: memory where there is enough of it (that case's main kernel moves its bytes at 0.85 of the copy rate), else
+// a warp's chain of some 290 instructions a chunk, 0.6 us (0.8 with the copies of pages of 16), and the start and the end.
+// Tried and taken back: the next chunk's scores formed among this one's weights (44 bytes spilled; 10 to 15 % slower at head size
+// 128), four CTAs an SM at 96 registers (20 % slower a chunk), more than 16 splits through scratch (59 us for one row of 131,072
+// keys in 48, as the shares).
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
@@ -590,15 +595,16 @@ __global__ void __launch_bounds__(128) attention_decode_f8_join_kernel(const Dec
     const int b1 = narrow ? ((int)u0 + t.y - 1) / share : (int)((u0 + t.y - 1) / share);
     if (b0 == b1) return;                                         // one CTA had it all
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // the first CTA's part is the last of its share, unless its share begins with the pair
-    auto at = [&](int b) { return ((int64_t)b * 2 + (b * (int64_t)share >= u0 ? 0 : 1)) * ROWS + m; };
+    // the first CTA's part is the last of its share, unless its share begins with the pair; the others begin theirs with it
+    const int begun = (int64_t)b0 * share < u0 ? 1 : 0;
+    auto at = [&](int b) { return (b * 2 + (b == b0 ? begun : 0)) * ROWS + m; };
     float top = -INFINITY, sum = 0.f, acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    for (int c = b0 + warp; c <= b1; c += 4 * 8) {                // eight parts at a time, all on their way together
-        float lse[8], v[8][E];
+    for (int c = b0 + warp; c <= b1; c += 4 * 4) {                // four parts at a time, all on their way together
+        float lse[4], v[4][E];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < 4; ++k) {
             const bool live = c + 4 * k <= b1;
             lse[k] = live ? dp.part_lse[at(c + 4 * k)] : -INFINITY;
 #pragma unroll
@@ -606,14 +612,14 @@ __global__ void __launch_bounds__(128) attention_decode_f8_join_kernel(const Dec
         }
         float mx = top;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) mx = fmaxf(mx, lse[k]);
+        for (int k = 0; k < 4; ++k) mx = fmaxf(mx, lse[k]);
         const float corr = top == -INFINITY ? 0.f : exp2f(top - mx);
         top = mx;
         sum *= corr;
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] *= corr;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < 4; ++k) {
             const float f = lse[k] == -INFINITY ? 0.f : exp2f(lse[k] - top);
             sum += f;
 #pragma unroll

@@ -1130,7 +1130,7 @@ def decode_f8_splits(tiles: int, num_kv_heads: int, key_bound: int, head_dim: in
     CTA's start and end take 6, a chunk of 64 keys 0.8 in a CTA (its warps' latencies), all of them together 6.1 TB/s; clusters run in
     one wave up to 0.9 of the CTAs that the device holds, of sixteen up to 0.57 (444 of them, 8 rows of 4,000 keys: 6 parts, 384 CTAs,
     18.9, 7 parts 28.4; 4 rows of 300: 8 parts 7.4, 16 14.4); shares take 12
-    and 3 a pair that a CTA comes to (64 rows of 4,096 keys: 101, whole 124, in 3 parts 114; 41 of 600 to 1,700: 34.5, whole 30;
+    and 3 a pair that a CTA comes to (64 rows of 4,096 keys: 99, whole 124, in 3 parts 114; 41 of 600 to 1,700: 33, whole 30;
     one of 131,072: 61, in 16 parts 105)."""
     pairs, chunks = max(1, tiles * num_kv_heads), -(-key_bound // 64)
     at_once = shares or 444
