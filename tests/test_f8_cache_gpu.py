@@ -618,3 +618,47 @@ def test_pools_beyond_4_gib():
     assert bool(torch.isfinite(far32[:4]).all())
     del k, v, s, narrow
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("which,splits", [("decode", s) for s in (0, 1, 2, 3, 5, 7, 8, 16)] + [("prefill", s) for s in (1, 2, 3, 7, 16)])
+@pytest.mark.parametrize("nq,nkv,d,P", [(8, 2, 128, 16), (8, 1, 64, 8), (3, 1, 128, 32)])
+def test_attention_in_parts(which, splits, nq, nkv, d, P):
+    """Keys cut into more and fewer parts than there are blocks, parts that a mask leaves empty, rows that are no number."""
+    spoil = [(0, 70, 0, 0), (1, 3, 0, 1), (5, 1100, 0, 0)]
+    lay, cache, keys, values = random_cache(BEFORES, QLENS, nkv, d, P, 31, spoil)
+    g = torch.Generator().manual_seed(32)
+    q = torch.randn(lay["num_tokens"], nq * d, generator=g).to(torch.bfloat16).to(DEV)
+    sink = (3 * torch.randn(nq, generator=g)).to(DEV)
+    for mask in (dict(), dict(window=1), dict(window=70, keep_first=5, sink32=sink), dict(chunk=256)):
+        got = attend(which, q, cache, lay, QLENS, nq, nkv, d, d ** -0.5, num_splits=splits, **mask)
+        check_attention(got, q, keys, values, BEFORES, QLENS, nq, d, d ** -0.5, **mask)
+
+
+@pytest.mark.parametrize("heads_at_once", [1, 2])
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("d", [64, 128])
+def test_prompts_whose_keys_are_made_a_few_heads_at_a_time(monkeypatch, heads_at_once, splits, d):
+    """Scratch for one kv head, and for two of three: the same bits as from all heads at once."""
+    nq, nkv, P = 6, 3, 16
+    lay, cache, keys, values = random_cache(BEFORES, QLENS, nkv, d, P, 33)
+    g = torch.Generator().manual_seed(34)
+    q = torch.randn(lay["num_tokens"], nq * d, generator=g).to(torch.bfloat16).to(DEV)
+    mask = dict(window=300, keep_first=4, sink32=torch.randn(nq, generator=g).to(DEV))
+    whole = attend("prefill", q, cache, lay, QLENS, nq, nkv, d, d ** -0.5, num_splits=splits, **mask)
+    cap = (-(-lay["block_table"].shape[1] * P // 128) + 1) * 128
+    monkeypatch.setattr(ops(), "F8_PREFILL_SCRATCH", heads_at_once * min(len(QLENS), len(tiles_of(QLENS, 128))) * cap * d * 4)
+    got = attend("prefill", q, cache, lay, QLENS, nq, nkv, d, d ** -0.5, num_splits=splits, **mask)
+    assert torch.equal(got, whole)
+    check_attention(got, q, keys, values, BEFORES, QLENS, nq, d, d ** -0.5, **mask)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_single_tokens_of_more_rows_than_are_shared_out(d):
+    nq, nkv, P, rows = 4, 2, 16, 300
+    befores, qlens = [(7 * r) % 150 for r in range(rows)], [1] * rows
+    lay, cache, keys, values = random_cache(befores, qlens, nkv, d, P, 35)
+    q = torch.randn(rows, nq * d, generator=torch.Generator().manual_seed(36)).to(torch.bfloat16).to(DEV)
+    got = attend("decode", q, cache, lay, qlens, nq, nkv, d, d ** -0.5, tiles=tiles_of(qlens, 1))
+    check_attention(got, q, keys, values, befores, qlens, nq, d, d ** -0.5)
+    with raises("num_splits"):
+        attend("decode", q, cache, lay, qlens, nq, nkv, d, d ** -0.5, tiles=tiles_of(qlens, 1), num_splits=0)
