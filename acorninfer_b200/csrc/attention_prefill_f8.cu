@@ -440,16 +440,21 @@ __global__ void __launch_bounds__(PF8_THREADS, 1) attention_prefill_f8_kernel(co
             if (good) {
                 tc_fence_after();
                 float total = l_run + *other;
-                // a sink is one more term of the denominator, against the same reference maximum as the keys' terms; the first
-                // split has it
+                // a sink is one more term of the denominator, in the first split; the denominator is taken against the larger of the
+                // reference and the sink, so that neither overflows
                 const float sink = p.sink && row_ok && split == 0 ? p.sink[head] * 1.4426950408889634f : -INFINITY;
                 // (a split that holds no key of the row: the sink alone; NaN keys leave no maximum, but a NaN sum)
                 const bool empty = m_ref == -INFINITY && total == 0.f;
-                if (sink != -INFINITY && !empty) total += exp2f(sink - m_ref);
-                const float inv = row_ok ? 1.f / total : 0.f;
+                float against = m_ref, shrink = 1.f;
+                if (sink != -INFINITY && !empty) {
+                    against = fmaxf(m_ref, sink);
+                    shrink = exp2f(m_ref - against);
+                    total = total * shrink + exp2f(sink - against);
+                }
+                const float inv = row_ok ? shrink / total : 0.f;
                 const int64_t out_row = (int64_t)(tok0 + row) * p.nq + head;
                 const int64_t part_row = (((int64_t)split * pp.n_tiles + tile) * PF8_BM + row) * p.nq + head;
-                if (pp.num_splits > 1 && row_ok && half == 0) pp.part_lse[part_row] = empty ? sink : m_ref + log2f(total);
+                if (pp.num_splits > 1 && row_ok && half == 0) pp.part_lse[part_row] = empty ? sink : against + log2f(total);
 #pragma unroll 1
                 for (int c = 0; c < D / 2; c += 32) {
                     float part[32];

@@ -662,3 +662,24 @@ def test_single_tokens_of_more_rows_than_are_shared_out(d):
     check_attention(got, q, keys, values, befores, qlens, nq, d, d ** -0.5)
     with raises("num_splits"):
         attend("decode", q, cache, lay, qlens, nq, nkv, d, d ** -0.5, tiles=tiles_of(qlens, 1), num_splits=0)
+
+
+@pytest.mark.parametrize("which,splits", [("decode", 0), ("decode", 1), ("decode", 3), ("prefill", 1), ("prefill", 3), ("plain", None)])
+def test_sinks_far_above_and_below_the_scores(which, splits):
+    """A sink of exp(200) leaves next to nothing of the keys, one of exp(-200) all of it, however the keys are cut.  Sizes below
+    2^-126 (float32's smallest normal number) may become zero."""
+    nq, nkv, P, d = 6, 2, 16, 128 if which != "plain" else 48
+    befores, qlens = [300, 0], [3, 130]
+    lay, cache, keys, values = random_cache(befores, qlens, nkv, d, P, 41)
+    q = torch.randn(lay["num_tokens"], nq * d, generator=torch.Generator().manual_seed(42)).to(torch.bfloat16).to(DEV)
+    sink = torch.tensor([200.0, 60.0, 0.0, -200.0, 100.0, 5.0], device=DEV)
+    kw = {} if splits is None else dict(num_splits=splits)
+    got = attend("prefill" if which == "plain" else which, q, cache, lay, qlens, nq, nkv, d, d ** -0.5, sink32=sink, **kw).double().cpu()
+    at = 0
+    for r, (held, n) in enumerate(zip(befores, qlens)):
+        want, spread, size = f8.attention(q[at:at + n].double().cpu().view(n, nq, d), keys[r], values[r], d ** -0.5, held, sink=sink.cpu())
+        off = (got[at:at + n].view(n, nq, d) - want).abs()
+        share = 2.0 ** -8 + 2 * (2.0 ** -18 + d * 2.0 ** -24 * size)[..., None]
+        most = torch.tensor([float(values[r].abs().max())]).double()
+        assert bool((off <= 2.0 ** -8 * want.abs() + share * spread + 2.0 ** -126 * (1 + most)).all())
+        at += n
