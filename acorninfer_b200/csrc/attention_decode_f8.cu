@@ -296,6 +296,8 @@ __global__ void __launch_bounds__(DF8_THREADS, NH == 1 ? 3 : 2) attention_decode
             }
             return true;
         });
+        // the last stages' copies have landed before the CTA ends, also where the compute warps gave up
+        for (int k = max(0, n - L::STAGES); k < n; ++k) mbar_wait(full0 + 8 * (k % L::STAGES), (k / L::STAGES) & 1);
         if (cluster) {
             cg::this_cluster().barrier_wait();
             cg::this_cluster().sync();
