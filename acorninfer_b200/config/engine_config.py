@@ -5,7 +5,8 @@ Names and meanings follow the reference where it has them
 ``num_blocks`` pages in the pool of every cache group, ``page_size`` tokens a page,
 ``max_running`` requests in a step at most, ``watermark_blocks`` pages that admission
 leaves free, ``chunked_budget`` the most tokens one step may carry (``None``: whole
-prompts).  ``kv_dtype`` "float8" keeps keys and values in 8 bits (None: in ``dtype``).  The reference's back-end switches have no counterpart: there is one back end.
+prompts).  ``kv_dtype`` "float8" keeps keys and values in 8 bits (None: in ``dtype``).  The
+reference's back-end switches have no counterpart: there is one back end.
 """
 
 from __future__ import annotations

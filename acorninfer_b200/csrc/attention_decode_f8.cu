@@ -4,9 +4,9 @@
 // its (token, head) pairs are its query rows, so the tokens of a tile read their row's pages together.
 // A producer warp brings the codes by TMA (swizzled; a box is the keys and the values of one page and head, through a map whose
 // third dimension is the distance between the two page tensors) and their exponents by asynchronous copies into a ring of
-// stages of 64 keys: an issued copy costs the warp some 130 clocks, which is what bounds a CTA at small pages.  Each of the four other warps takes 16 keys of a stage through m16n8k16 products whose sixteen rows are the
-// keys (then the entries of the values) and whose eight columns are query rows; more than eight query rows are NH = 2 products on
-// the same operands:
+// stages of 64 keys: an issued copy costs the warp some 130 clocks, which is what bounds a CTA at small pages.  Each of the four
+// other warps takes 16 keys of a stage through m16n8k16 products whose sixteen rows are the keys (then the entries of the values) and
+// whose eight columns are query rows; more than eight query rows are NH = 2 products on the same operands:
 //   S' = K Q'   codes become half-precision numbers by one conversion a pair (e4m3 is exact in it); the queries are
 //               brought to half precision by a power of two per row (their largest entry to 2^14 .. 2^15, so that a bfloat16
 //               entry is exact unless it is 2^-28 of the largest), and both powers of two meet the score in float32.
@@ -387,7 +387,8 @@ __global__ void __launch_bounds__(DF8_THREADS, NH == 1 ? 3 : 2) attention_decode
                 for (int r2 = 0; r2 < 2; ++r2)
 #pragma unroll
                     for (int q = 0; q < WORDS / 4; ++q) {
-                        const uint4 v = *reinterpret_cast<const uint4*>(stage + (k_at[r2] ^ (16 * q)));          // pieces 2 i and 2 i + 1 differ in one bit, swizzled or not
+                        // pieces 2 i and 2 i + 1 differ in one bit, swizzled or not
+                        const uint4 v = *reinterpret_cast<const uint4*>(stage + (k_at[r2] ^ (16 * q)));
                         kw[r2][4 * q] = v.x; kw[r2][4 * q + 1] = v.y; kw[r2][4 * q + 2] = v.z; kw[r2][4 * q + 3] = v.w;
                     }
                 // exponents of keys g and g + 8: key byte, value byte
@@ -699,8 +700,8 @@ static int launch_decode_f8(DecodeF8Params dp, int64_t num_pages, cudaStream_t s
         if (ctas < 1) return ACORN_ERR_UNSUPPORTED;
         const int e = acorn_launch(attention_decode_f8_kernel<D, NH, true>, dim3(ctas), dim3(DF8_THREADS), (size_t)(L::RECV + L::SHARES), stream,
                                    mk, mv, dp);
-        return e ? e : acorn_launch(attention_decode_f8_join_kernel<D, NH>, dim3(p.nkv, dp.tile_tokens * (p.nq / p.nkv), dp.n_tiles), dim3(128), 0, stream,
-                                    dp);
+        return e ? e : acorn_launch(attention_decode_f8_join_kernel<D, NH>, dim3(p.nkv, dp.tile_tokens * (p.nq / p.nkv), dp.n_tiles),
+                                    dim3(128), 0, stream, dp);
     }
     const int rows = dp.tile_tokens * (p.nq / p.nkv), splits = dp.num_splits;
     const size_t recv = splits > 1 ? (size_t)splits * ((rows + splits - 1) / splits) * L::RECV_ROW * 4 : 0;
