@@ -174,8 +174,11 @@ __device__ __forceinline__ bool compute_all(bool v) {
     return r != 0;
 }
 
+// CTAs an SM: three, but two where sixteen rows of 128 entries need more than 128 registers a thread.  (Sixteen rows of 64, three
+// against two: 24 rows of 3 new tokens over a window of 1,024 19.1 us against 20.7, 41 of 2 over up to 1,700 22.9 against 28.0, 64
+// over 4,096 at sixteen heads a group 62.8 against 68.1.)
 template <int D, int NH, bool SHARES>
-__global__ void __launch_bounds__(DF8_THREADS, NH == 1 ? 3 : 2) attention_decode_f8_kernel(const __grid_constant__ CUtensorMap map_k,
+__global__ void __launch_bounds__(DF8_THREADS, NH == 1 || D == 64 ? 3 : 2) attention_decode_f8_kernel(const __grid_constant__ CUtensorMap map_k,
                                                                          const __grid_constant__ CUtensorMap map_v,
                                                                          const DecodeF8Params dp) {
     using L = DecodeF8<D, NH>;
