@@ -14,8 +14,10 @@
 //               t + e_v so far: the value's power of two rides in the exponent, so that a weight is at most 2^14 (the reference
 //               moves when it is outgrown by more) in half precision, with 11 bits where bfloat16 would keep 8, whatever the
 //               sizes of the value rows.  Against the reference the common step needs no maximum across lanes, only a vote.
-//   O' += V' P' on value codes as half-precision numbers (a weight's transpose within the warp is one movmatrix); the
-//               denominator sums 2^(t - m) in float32.
+//   O' += V' P' on value codes as half-precision numbers (a weight's transpose within the warp is one movmatrix);
+//   L += 2^(t - r)  the denominator in float32, r a reference near the largest t alone: m lies up to 120 to either side of the
+//               scores (a row of zeros has e_v = -120), and 2^(t - m) summed would be infinite after 256 such keys.  The result is
+//               O' / L 2^(m - r).
 // The layouts of the fragments are chosen so that a lane's codes are whole 16-byte pieces of rows: the order of the head's
 // entries in a product over them is free (Q is laid out the same way), and so is the order of the output's rows.
 // Codes of keys that no query of the tile reads are replaced by zeros (a slot that was never written may hold anything).
@@ -47,6 +49,9 @@ namespace cg = cooperative_groups;
 #define DF8_CLUSTER_MAX 16
 #define DF8_GROW_LOG2 14.f                  // the reference maximum moves when a row's maximum outgrew it by more than this
                                             // (half-precision weights end at 2^16)
+#define DF8_SUM_LOG2 64.f                           // and the denominator's by more than this (float32: room for 2^63 keys)
+#define DF8_NONE (-3.402823466e38f)                 // a reference that no score has moved: every finite one is at least as large, and
+                                                    // -infinity less it is -infinity, a weight of 0
 
 __device__ int g_attn_dec_f8_error = 0;
 
@@ -71,7 +76,7 @@ template <int D, int NH> struct DecodeF8 {
     static constexpr int SCALE_BYTES = 2 * DF8_CHUNK;
     static constexpr int RECV_ROW = D + 4;                            // floats a received partial row takes: the output, then its log-sum
     static constexpr int RING = STAGES * STAGE_BYTES;
-    static constexpr int MERGE_BYTES = DF8_WARPS * ROWS * (2 + D) * 4;
+    static constexpr int MERGE_BYTES = DF8_WARPS * ROWS * (3 + D) * 4;
     static constexpr int MERGE = RING;                                // offsets in shared memory
     static constexpr int BARS = MERGE + MERGE_BYTES;
     static constexpr int SCALES = BARS + 2 * STAGES * 8;
@@ -323,7 +328,7 @@ __global__ void __launch_bounds__(DF8_THREADS, NH == 1 || D == 64 ? 3 : 2) atten
     parts([&](const F8Tile& t, int kvh, int c0, int c1, bool first) -> bool {
         const int m_rows = t.n_q * rep, tok0 = t.tok0;
         float o[NH][WORDS][4];
-        float m_ref[NH][2], l_run[NH][2];
+        float m_ref[NH][2], t_ref[NH][2], l_run[NH][2];
         // queries: this lane holds row g (of each half), entries i * D / 4 .. + D / 4 - 1 of the head, as the B operand
         uint32_t qb[NH][WORDS][2];
         float factor[NH][2];                                      // of query rows 2 i and 2 i + 1: the softmax scale, and what undoes
@@ -361,7 +366,7 @@ __global__ void __launch_bounds__(DF8_THREADS, NH == 1 || D == 64 ? 3 : 2) atten
                 factor[h][b] = __shfl_sync(0xffffffffu, back, 4 * (2 * i + b)) * p.scale_log2;
                 qpos[h][b] = t.pos0 + min((8 * h + 2 * i + b) / rep, max(t.n_q - 1, 0));
                 first_seen[h][b] = mask_lo(p.mask, qpos[h][b]);
-                m_ref[h][b] = -INFINITY;
+                m_ref[h][b] = t_ref[h][b] = DF8_NONE;
                 l_run[h][b] = 0.f;
             }
 #pragma unroll
@@ -414,7 +419,7 @@ __global__ void __launch_bounds__(DF8_THREADS, NH == 1 || D == 64 ? 3 : 2) atten
                     ve[r2] = (float)((int)vbyte - 127);
                 }
                 bool grew = false;
-                float mx[NH][2];
+                float mx[NH][2], tx[NH][2];
 #pragma unroll
                 for (int h = 0; h < NH; ++h)
 #pragma unroll
@@ -429,7 +434,8 @@ __global__ void __launch_bounds__(DF8_THREADS, NH == 1 || D == 64 ? 3 : 2) atten
                             sc[h][2 * r2 + b] = x;
                         }
                         mx[h][b] = fmaxf(sc[h][b] + ve[0], sc[h][2 + b] + ve[1]);
-                        grew = grew || mx[h][b] > m_ref[h][b] + DF8_GROW_LOG2;
+                        tx[h][b] = fmaxf(sc[h][b], sc[h][2 + b]);
+                        grew = grew || mx[h][b] > m_ref[h][b] + DF8_GROW_LOG2 || tx[h][b] > t_ref[h][b] + DF8_SUM_LOG2;
                     }
                 if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
@@ -438,11 +444,15 @@ __global__ void __launch_bounds__(DF8_THREADS, NH == 1 || D == 64 ? 3 : 2) atten
                         for (int b = 0; b < 2; ++b) {
                             const float top = column_max(mx[h][b]);
                             if (top > m_ref[h][b]) {
-                                const float corr = fast_exp2(m_ref[h][b] - top);          // from -inf: 0
+                                const float corr = fast_exp2(m_ref[h][b] - top);          // from DF8_NONE: 0
                                 m_ref[h][b] = top;
-                                l_run[h][b] *= corr;
 #pragma unroll
                                 for (int n2 = 0; n2 < WORDS; ++n2) { o[h][n2][b] *= corr; o[h][n2][2 + b] *= corr; }
+                            }
+                            const float most = column_max(tx[h][b]);
+                            if (most > t_ref[h][b]) {
+                                l_run[h][b] *= fast_exp2(t_ref[h][b] - most);
+                                t_ref[h][b] = most;
                             }
                         }
                 }
@@ -451,15 +461,12 @@ __global__ void __launch_bounds__(DF8_THREADS, NH == 1 || D == 64 ? 3 : 2) atten
                 for (int h = 0; h < NH; ++h) {
                     float w[4];
 #pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        const float neg = m_ref[h][b] == -INFINITY ? 0.f : -m_ref[h][b];
+                    for (int b = 0; b < 2; ++b)
 #pragma unroll
                         for (int r2 = 0; r2 < 2; ++r2) {
-                            const float a = sc[h][2 * r2 + b] + neg;
-                            l_run[h][b] += fast_exp2(a);
-                            w[2 * r2 + b] = fast_exp2(a + ve[r2]);
+                            l_run[h][b] += fast_exp2(sc[h][2 * r2 + b] - t_ref[h][b]);
+                            w[2 * r2 + b] = fast_exp2(sc[h][2 * r2 + b] - m_ref[h][b] + ve[r2]);
                         }
-                    }
                     pb[h][0] = movmatrix_trans(pack_f16(w[0], w[1]));
                     pb[h][1] = movmatrix_trans(pack_f16(w[2], w[3]));
                 }
@@ -505,7 +512,8 @@ __global__ void __launch_bounds__(DF8_THREADS, NH == 1 || D == 64 ? 3 : 2) atten
         for (int h = 0; h < NH; ++h) { l_run[h][0] = column_sum(l_run[h][0]); l_run[h][1] = column_sum(l_run[h][1]); }
         // ---- the warps joined
         float* sm_m = reinterpret_cast<float*>(smem + L::MERGE);  // [WARPS][ROWS]
-        float* sm_l = sm_m + ROWS * DF8_WARPS;
+        float* sm_t = sm_m + ROWS * DF8_WARPS;
+        float* sm_l = sm_t + ROWS * DF8_WARPS;
         float* sm_o = sm_l + ROWS * DF8_WARPS;                    // [WARPS][ROWS][D]
         good = compute_all(good);                                 // the part before has been read; a wait that gave up ends the walk of all
 #pragma unroll
@@ -515,6 +523,7 @@ __global__ void __launch_bounds__(DF8_THREADS, NH == 1 || D == 64 ? 3 : 2) atten
                 const int m = warp * ROWS + 8 * h + 2 * i + b;
                 if (g == 0) {
                     sm_m[m] = m_ref[h][b];
+                    sm_t[m] = t_ref[h][b];
                     sm_l[m] = l_run[h][b];
                 }
 #pragma unroll
@@ -529,34 +538,43 @@ __global__ void __launch_bounds__(DF8_THREADS, NH == 1 || D == 64 ? 3 : 2) atten
         const int slots = (dp.tile_tokens * rep + csize - 1) / csize;
         const bool whole_pair = SHARES ? c0 == 0 && c1 == t.n_chunks : !cluster;
         if (cluster) cg::this_cluster().barrier_wait();
-        for (int idx = threadIdx.x; idx < m_rows * D; idx += 32 * DF8_WARPS) {
-            const int m = idx / D, e = idx - m * D;
+        for (int m = warp; m < m_rows; m += DF8_WARPS) {          // a warp a row, D / 32 neighbouring entries a lane
+            constexpr int E = D / 32;
             const int head = kvh * rep + m % rep;
             const float sink = p.sink && c0 == 0 && split == 0 ? p.sink[head] * 1.4426950408889634f : -INFINITY;
-            float mstar = sink;
-#pragma unroll
-            for (int w = 0; w < DF8_WARPS; ++w) mstar = fmaxf(mstar, sm_m[w * ROWS + m]);
-            float sum = sink == -INFINITY ? 0.f : exp2f(sink - mstar), acc = 0.f;
+            float mstar = DF8_NONE, tstar = fmaxf(DF8_NONE, sink);
 #pragma unroll
             for (int w = 0; w < DF8_WARPS; ++w) {
-                // a warp without keys has maximum -inf and sum 0; one whose keys are all NaN a sum that is NaN
-                const float mw = sm_m[w * ROWS + m], lw = sm_l[w * ROWS + m];
-                const float f = mw == -INFINITY ? 0.f : exp2f(mw - mstar);
-                sum += f * lw;
-                acc += f * sm_o[(w * ROWS + m) * D + e];
+                mstar = fmaxf(mstar, sm_m[w * ROWS + m]);
+                tstar = fmaxf(tstar, sm_t[w * ROWS + m]);
             }
-            const bool empty = mstar == -INFINITY && sum == 0.f;  // no key of this part is seen by the query
+            float sum = sink == -INFINITY ? 0.f : exp2f(sink - tstar), mean[E] = {};
+#pragma unroll
+            for (int w = 0; w < DF8_WARPS; ++w) {                 // a warp without keys has a sum and an output of 0
+                sum += exp2f(sm_t[w * ROWS + m] - tstar) * sm_l[w * ROWS + m];
+                const float f = exp2f(sm_m[w * ROWS + m] - mstar);
+#pragma unroll
+                for (int e = 0; e < E; ++e) mean[e] += f * sm_o[(w * ROWS + m) * D + E * lane + e];
+            }
+            const bool empty = sum == 0.f;                        // no key of this part is seen by the query
+            const float back = exp2f(0.5f * (mstar - tstar));     // in two steps: 2^(m - r) alone may not be a float
+#pragma unroll
+            for (int e = 0; e < E; ++e) mean[e] = mean[e] / sum * back * back;
             if (whole_pair) {
-                p.out[((int64_t)(tok0 + m / rep) * p.nq + head) * D + e] = __float2bfloat16_rn(acc / sum);
+                __nv_bfloat162* dst = reinterpret_cast<__nv_bfloat162*>(p.out + ((int64_t)(tok0 + m / rep) * p.nq + head) * D + E * lane);
+#pragma unroll
+                for (int e = 0; e < E; e += 2) dst[e / 2] = __floats2bfloat162_rn(mean[e], mean[e + 1]);
             } else if (cluster) {
                 // to the CTA that finishes this row; a split without keys sends a log-sum of -inf
                 const uint32_t dst = cluster_map(tc_smem(recv + (split * slots + m / csize) * L::RECV_ROW), m % csize);
-                st_cluster_f32(dst + 4 * e, empty ? 0.f : acc / sum);
-                if (e == 0) st_cluster_f32(dst + 4 * D, empty ? -INFINITY : mstar + log2f(sum));
+#pragma unroll
+                for (int e = 0; e < E; ++e) st_cluster_f32(dst + 4 * (E * lane + e), empty ? 0.f : mean[e]);
+                if (lane == 0) st_cluster_f32(dst + 4 * D, empty ? -INFINITY : tstar + log2f(sum));
             } else {
                 const int64_t at = ((int64_t)blockIdx.x * 2 + (first ? 0 : 1)) * ROWS + m;
-                dp.part_o[at * D + e] = empty ? 0.f : acc / sum;
-                if (e == 0) dp.part_lse[at] = empty ? -INFINITY : mstar + log2f(sum);
+#pragma unroll
+                for (int e = 0; e < E; ++e) dp.part_o[at * D + E * lane + e] = empty ? 0.f : mean[e];
+                if (lane == 0) dp.part_lse[at] = empty ? -INFINITY : tstar + log2f(sum);
             }
         }
         if (cluster) {
