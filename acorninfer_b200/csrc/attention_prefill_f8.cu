@@ -29,7 +29,8 @@
 // 3. Where the tiles are few, a tile's keys are split over several CTAs, whose results (float32, normalised, with the logarithm of
 //    their sums) are joined by a third kernel.
 //
-// Every mbarrier wait is bounded; a wait that gives up records g_attn_pre_f8_error and the CTA drains.
+// Every mbarrier wait is bounded; a wait that gives up records g_attn_pre_f8_error and the CTA drains: it ends, and its tensor
+// memory is given back, when the copies and products that it issued are done.
 #include "f8_tma.cuh"
 
 #define PF8_BM 128
@@ -143,8 +144,8 @@ template <int D> struct PrefillF8 {
     static constexpr int TILE_BYTES = HALVES * HALF_BYTES;           // a K or V tile
     static constexpr int TILES = 2 * Q_BYTES;                        // offsets in shared memory
     static constexpr int BARS = TILES + PF8_SLOTS * TILE_BYTES;
-    // q_full, full, empty [SLOTS], s_full, p_full, o_done [unit]
-    static constexpr int NUM_BARS = 1 + 2 * PF8_SLOTS + 6;
+    // q_full, full, empty [SLOTS], s_full, p_full, o_done [unit], drained
+    static constexpr int NUM_BARS = 1 + 2 * PF8_SLOTS + 6 + 1;
     static constexpr int SHARED = BARS + NUM_BARS * 8 + 16;          // [unit][half][row]: what the two threads of a row exchange
     static constexpr int SMEM = SHARED + 2 * 2 * PF8_BM * 4;
 };
@@ -209,7 +210,7 @@ __global__ void __launch_bounds__(PF8_THREADS, 1) attention_prefill_f8_kernel(co
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
     const uint32_t q_full = tc_smem(bars);
     const uint32_t full0 = q_full + 8, empty0 = full0 + 8 * PF8_SLOTS;
-    const uint32_t s_full0 = empty0 + 8 * PF8_SLOTS, p_full0 = s_full0 + 16, o_done0 = p_full0 + 16;
+    const uint32_t s_full0 = empty0 + 8 * PF8_SLOTS, p_full0 = s_full0 + 16, o_done0 = p_full0 + 16, drained = o_done0 + 16;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L::NUM_BARS);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -226,6 +227,7 @@ __global__ void __launch_bounds__(PF8_THREADS, 1) attention_prefill_f8_kernel(co
     }
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
+        mbar_init(drained, 1);
         for (int s = 0; s < PF8_SLOTS; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
         for (int u = 0; u < 2; ++u) { mbar_init(s_full0 + 8 * u, 1); mbar_init(p_full0 + 8 * u, 8); mbar_init(o_done0 + 8 * u, 1); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -263,8 +265,8 @@ __global__ void __launch_bounds__(PF8_THREADS, 1) attention_prefill_f8_kernel(co
                     for (int h = 0; h < L::HALVES; ++h)
                         tma_load_2d(tc_smem(smem) + u * L::Q_BYTES + h * PF8_BM * 128, &map_q, q_full, (head0 + u) * D + 64 * h, tok0);
             }
-            int slot = 0, phase = 0;
-            for (int n = 0; n < 2 * nb; ++n) {                           // K_0 V_0 K_1 V_1 ...
+            int slot = 0, phase = 0, n = 0;
+            for (; n < 2 * nb; ++n) {                                    // K_0 V_0 K_1 V_1 ...
                 const bool got = mbar_wait(empty0 + 8 * slot, phase ^ 1);
                 if (!got && lane == 0) tc_fail(&g_attn_pre_f8_error, 1, ACORN_KERNEL_ATTN_PREFILL_F8);
                 if (!__all_sync(0xffffffffu, got)) break;
@@ -277,6 +279,9 @@ __global__ void __launch_bounds__(PF8_THREADS, 1) attention_prefill_f8_kernel(co
                 }
                 if (++slot == PF8_SLOTS) { slot = 0; phase ^= 1; }
             }
+            // all copies have landed before the CTA ends, also where the others gave up and read none of them
+            if (nb > 0) mbar_wait(q_full, 0);
+            for (int k = max(0, n - PF8_SLOTS); k < n; ++k) mbar_wait(full0 + 8 * (k % PF8_SLOTS), (k / PF8_SLOTS) & 1);
         } else if (warp == 17) {
             // ------------------------------------------------------------ MMA issuer
             constexpr uint32_t IDESC_QK = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(PF8_BN >> 3) << 17) |
@@ -300,6 +305,7 @@ __global__ void __launch_bounds__(PF8_THREADS, 1) attention_prefill_f8_kernel(co
             };
             bool good = nb > 0 && wait_all(q_full, 0, 2) && wait_all(full0, 0, 3);
             int slot = 0, phase = 0;                                     // the next tile of the ring
+            const bool issued = good;
             if (good) {
                 for (int u = 0; u < units; ++u) issue_qk(u, 0);
                 umma_commit_elect(empty0);
@@ -331,6 +337,11 @@ __global__ void __launch_bounds__(PF8_THREADS, 1) attention_prefill_f8_kernel(co
                 if (!good) break;
                 umma_commit_elect(empty0 + 8 * sv);
                 if (has_next) umma_commit_elect(empty0 + 8 * sk);
+            }
+            // the products are done before the tensor memory is given back, also where somebody gave up in between
+            if (issued) {
+                umma_commit_elect(drained);
+                mbar_wait(drained, 0);
             }
         }
     } else {
