@@ -2,8 +2,8 @@
 // consecutive queries of one request, on the 5th-generation tensor cores.
 //
 // Three kernels.
-// 1. The keys and values that the tiles read become bfloat16 rows, [slot][kv head][key], which is exact (code * 2^e is a
-//    bfloat16 number).  Done once a call, it reads and writes 5 bytes a number; turned into operand tiles by warps of the attention
+// 1. The keys and values of the rows that have tiles become bfloat16 rows, [kv head][place of the row + key], which is exact (code *
+//    2^e is a bfloat16 number).  Done once a call, it reads and writes 5 bytes a number; turned into operand tiles by warps of the attention
 //    kernel itself, every (tile, pair of heads) did it again, in competition with the softmax for the integer pipe and with the matrix
 //    instructions for shared memory (8,192 tokens, 32 heads over 8: 840 us).
 //    Keys outside a row's range within its blocks of 128 get zero rows, so that whatever a slot of a page holds that was never
@@ -46,10 +46,13 @@ struct PrefillF8Params {
     F8AttnParams a;
     int pairs;                // ceil((nq / nkv) / 2): CTAs per (tile, kv head, split)
     int n_tiles, rows;        // rows: of the block table
-    int cap;                  // keys a slot has room for, a multiple of 128
+    const int* slot_rows;     // [slots]: the rows that have tiles, each once; or null: f8_place has the rule
+    int slots;
+    int cap;                  // without slot_rows: keys a slot has room for, a multiple of 128
+    int room;                 // keys the scratch has room for, of one kv head
     int kvh0, kvhs;           // the kv heads of this pass
     int num_splits;
-    bf16* k_rows;             // [slots, kvhs, cap, D]
+    bf16* k_rows;             // [kvhs, room, D]
     bf16* v_rows;
     float* part_o;            // [splits, n_tiles, 128, nq, D] where num_splits > 1
     float* part_lse;          // [splits, n_tiles, 128, nq]
@@ -67,19 +70,37 @@ struct F8Blocks {
     __device__ __forceinline__ int key0(int j) const { return j < nkb ? j * PF8_BN : lo + (j - nkb) * PF8_BN; }
 };
 
-// The slot that holds a row's keys: the row itself, or where there are fewer tiles than rows the first tile of that row.
-// All threads of a warp call it.
-__device__ __forceinline__ int f8_slot(const PrefillF8Params& pp, int r) {
-    if (pp.n_tiles >= pp.rows) return r;
-    const int lane = threadIdx.x & 31;
-    for (int t0 = 0; t0 < pp.n_tiles; t0 += 32) {
-        const uint32_t hit = __ballot_sync(0xffffffffu, t0 + lane < pp.n_tiles && pp.a.tiles[2 * min(t0 + lane, pp.n_tiles - 1)] == r);
-        if (hit) return t0 + __ffs(hit) - 1;
-    }
-    return 0;
-}
-// The key that a row's slot starts with: the first whose page the row still holds, down to a multiple of 128.
+// The key that a row's place starts with: the first whose page the row still holds, down to a multiple of 128.
 __device__ __forceinline__ int f8_slot_key(const F8AttnParams& p, int r) { return (p.page_base[r] << p.logP) & ~(PF8_BN - 1); }
+
+// Where in the scratch (in keys) a row's place starts; -1 for a row that has no tile.  The rows of a list lie one behind the other, each
+// with as many blocks of 128 keys as it holds.  Without a list a place has room for the widest row of the table, and is that of the row's
+// number, or where there are fewer tiles than rows that of the row's first tile.  `tiled`: the caller has the row from a tile.  All
+// threads of a warp call it.
+__device__ __forceinline__ int f8_place(const PrefillF8Params& pp, int r, bool tiled) {
+    if (pp.slots == 1 && (tiled || pp.rows == 1 || pp.slot_rows != nullptr)) return 0;
+    if (pp.slot_rows == nullptr && tiled && pp.n_tiles >= pp.rows) return r * pp.cap;
+    const F8AttnParams& p = pp.a;
+    const int lane = threadIdx.x & 31;
+    if (pp.slot_rows != nullptr) {
+        int before = 0;
+        for (int s0 = 0; s0 < pp.slots; s0 += 32) {
+            const int q = s0 + lane < pp.slots ? pp.slot_rows[s0 + lane] : -1;
+            const int hi = q < 0 ? 0 : p.row_pos[q] + p.row_start[q + 1] - p.row_start[q];
+            const int keys = q < 0 ? 0 : (hi + PF8_BN - 1) / PF8_BN * PF8_BN - f8_slot_key(p, q);
+            const uint32_t hit = __ballot_sync(0xffffffffu, q == r);
+            const int upto = hit ? __ffs(hit) - 1 : 32;
+            before += __reduce_add_sync(0xffffffffu, lane < upto ? keys : 0);
+            if (hit) return before;
+        }
+        return -1;
+    }
+    for (int t0 = 0; t0 < pp.n_tiles; t0 += 32) {
+        const uint32_t hit = __ballot_sync(0xffffffffu, t0 + lane < pp.n_tiles && p.tiles[2 * min(t0 + lane, pp.n_tiles - 1)] == r);
+        if (hit) return (pp.n_tiles >= pp.rows ? r : t0 + __ffs(hit) - 1) * pp.cap;
+    }
+    return -1;
+}
 
 // ---------------------------------------------------------------- 1. pages to rows of bfloat16
 
@@ -94,16 +115,18 @@ __global__ void __launch_bounds__(RB_THREADS) read_pages_f8_kernel(const Prefill
     pdl_wait();
     pdl_trigger();
     const int slot = blockIdx.z, kvh = pp.kvh0 + blockIdx.y;
-    int r = slot;
-    if (pp.n_tiles < pp.rows) {
-        r = p.tiles[2 * slot];
-        if (f8_slot(pp, r) != slot) return;                          // another tile of the row came first
+    const int r = pp.rows == 1 ? 0 : pp.slot_rows != nullptr ? pp.slot_rows[slot] : pp.n_tiles < pp.rows ? p.tiles[2 * slot] : slot;
+    int place = 0;
+    if (pp.slot_rows == nullptr) {
+        place = f8_place(pp, r, false);
+        if (place != slot * pp.cap) return;                          // no tile reads the row, or another tile of the row came first
     }
     const F8Blocks b(p.mask, p.row_pos[r], p.row_start[r + 1] - p.row_start[r]);
     const int* table = p.block_table + (int64_t)r * p.table_stride - p.page_base[r];
     const int first_key = p.page_base[r] << p.logP, slot_key = f8_slot_key(p, r), pmask = (1 << p.logP) - 1;
     constexpr int PIECES = D / 16, KEYS = RB_THREADS / PIECES, PARTS = PF8_BN / KEYS;
     const int piece = threadIdx.x % PIECES;
+    bool placed = pp.slot_rows == nullptr;
     for (int part = blockIdx.x; part < b.n * PARTS; part += gridDim.x) {
         const int key0 = b.key0(part / PARTS), key = key0 + part % PARTS * KEYS + threadIdx.x / PIECES;
         if (key0 < slot_key) continue;                               // (a kept block whose pages are gone)
@@ -127,7 +150,15 @@ __global__ void __launch_bounds__(RB_THREADS) read_pages_f8_kernel(const Prefill
             ko[q] = *reinterpret_cast<const uint32_t*>(&ab);
             vo[q] = *reinterpret_cast<const uint32_t*>(&cb);
         }
-        const int64_t out = ((int64_t)(slot * pp.kvhs + blockIdx.y) * pp.cap + (key - slot_key)) * D + 16 * piece;
+        if (!placed) {                                               // looked up while the first codes are on their way
+            place = f8_place(pp, r, false);
+            if (place + (b.hi + PF8_BN - 1) / PF8_BN * PF8_BN - slot_key > pp.room) {       // the caller's lengths were too short
+                if (threadIdx.x == 0) tc_fail(&g_attn_pre_f8_error, 10, ACORN_KERNEL_ATTN_PREFILL_F8);
+                return;
+            }
+            placed = true;
+        }
+        const int64_t out = ((int64_t)blockIdx.y * pp.room + place + (key - slot_key)) * D + 16 * piece;
         uint4* kd = reinterpret_cast<uint4*>(pp.k_rows + out);
         uint4* vd = reinterpret_cast<uint4*>(pp.v_rows + out);
         kd[0] = make_uint4(ko[0], ko[1], ko[2], ko[3]); kd[1] = make_uint4(ko[4], ko[5], ko[6], ko[7]);
@@ -257,8 +288,8 @@ __global__ void __launch_bounds__(PF8_THREADS, 1) attention_prefill_f8_kernel(co
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         if (warp == 16) {
             // ------------------------------------------------------------ producer
-            const int row0 = (f8_slot(pp, r) * pp.kvhs + kvp) * pp.cap - f8_slot_key(p, r);
-            const int first = f8_slot_key(p, r);
+            const int first = f8_slot_key(p, r), place = f8_place(pp, r, true);
+            const int row0 = kvp * pp.room + max(place, 0) - first;
             if (nb > 0 && elect_one()) {
                 mbar_expect_tx(q_full, units * L::Q_BYTES);
                 for (int u = 0; u < units; ++u)
@@ -279,6 +310,8 @@ __global__ void __launch_bounds__(PF8_THREADS, 1) attention_prefill_f8_kernel(co
                 }
                 if (++slot == PF8_SLOTS) { slot = 0; phase ^= 1; }
             }
+            if ((place < 0 || (pp.slot_rows != nullptr && pp.slots == 1 && pp.slot_rows[0] != r)) && lane == 0)
+                tc_fail(&g_attn_pre_f8_error, 11, ACORN_KERNEL_ATTN_PREFILL_F8);                           // a row that was not listed
             // all copies have landed before the CTA ends, also where the others gave up and read none of them
             if (nb > 0) mbar_wait(q_full, 0);
             for (int k = max(0, n - PF8_SLOTS); k < n; ++k) mbar_wait(full0 + 8 * (k % PF8_SLOTS), (k / PF8_SLOTS) & 1);
@@ -550,11 +583,11 @@ extern "C" int acorn_attention_prefill_f8_supported(int nq, int nkv, int d, int 
 }
 
 template <int D>
-static int launch_prefill_f8(const PrefillF8Params& pp, int tokens, int slots, int blocks, cudaStream_t stream) {
+static int launch_prefill_f8(const PrefillF8Params& pp, int tokens, int blocks, cudaStream_t stream) {
     using L = PrefillF8<D>;
     const F8AttnParams& p = pp.a;
     CUtensorMap mq, mk, mv;
-    const int64_t rows = (int64_t)slots * pp.kvhs * pp.cap;
+    const int64_t rows = (int64_t)pp.kvhs * pp.room;
     if (rows > 0x7fffffff) return ACORN_ERR_UNSUPPORTED;
     int rc = make_map(&mq, p.q, tokens, (int64_t)p.nq * D, p.q_stride, 64, PF8_BM);
     if (rc) return rc;
@@ -568,7 +601,7 @@ static int launch_prefill_f8(const PrefillF8Params& pp, int tokens, int slots, i
         if (e != cudaSuccess) return (int)e;
         configured.mark();
     }
-    rc = acorn_launch(read_pages_f8_kernel<D>, dim3(blocks, pp.kvhs, slots), dim3(RB_THREADS), 0, stream, pp);
+    rc = acorn_launch(read_pages_f8_kernel<D>, dim3(blocks, pp.kvhs, pp.slots), dim3(RB_THREADS), 0, stream, pp);
     if (rc) return rc;
     const int64_t ctas = (int64_t)pp.n_tiles * pp.kvhs * pp.pairs;
     rc = acorn_launch(attention_prefill_f8_kernel<D>, dim3((unsigned)ctas, pp.num_splits), dim3(PF8_THREADS), L::SMEM, stream, mq, mk, mv, pp);
@@ -577,19 +610,19 @@ static int launch_prefill_f8(const PrefillF8Params& pp, int tokens, int slots, i
     return acorn_launch(attention_prefill_f8_join_kernel<D>, dim3((unsigned)((items + 7) / 8)), dim3(256), 0, stream, pp);
 }
 
-// `slots`: min(rows of the table, tiles); k_rows / v_rows: [slots, kvhs, cap, d] bfloat16 for the kv heads kvh0 .. kvh0 + kvhs - 1
-// of this pass; blocks: CTAs along a row's keys.
+// slot_rows [slots]: the rows that have tiles, each once, or null with `slots` = min(rows of the table, tiles) of `cap` keys each;
+// k_rows / v_rows: [kvhs, room, d] bfloat16 for the kv heads kvh0 .. kvh0 + kvhs - 1 of this pass; blocks: CTAs along a row's keys.
 extern "C" int acorn_attention_prefill_f8(const void* q, int64_t q_stride, int tokens, void* out, const void* k_pages,
                                           const void* v_pages, const void* scales, const int* block_table, const int* page_base,
                                           int table_stride, int rows, const int* row_start, const int* row_pos, const int* tiles,
                                           int n_tiles, int nq, int nkv, int d, int P, float scale, int window, int chunk, int keep,
-                                          const float* sink, int kvh0, int kvhs, void* k_rows, void* v_rows, int slots, int cap,
-                                          int blocks, int num_splits, float* part_o, float* part_lse, cudaStream_t stream) {
+                                          const float* sink, int kvh0, int kvhs, void* k_rows, void* v_rows, const int* slot_rows,
+                                          int slots, int cap, int room, int blocks, int num_splits, float* part_o, float* part_lse, cudaStream_t stream) {
     if (n_tiles <= 0) return 0;
     if (!acorn_attention_prefill_f8_supported(nq, nkv, d, P) || q_stride % 8 != 0 || ((uintptr_t)q & 15) || !(scale > 0.f) ||
-        cap % PF8_BN || slots < 1 || slots > 65535 || kvhs < 1 || kvhs > 65535 || kvh0 < 0 || kvh0 + kvhs > nkv || blocks < 1 ||
+        cap % PF8_BN || room % PF8_BN || room < 1 || slots < 1 || slots > 65535 || kvhs < 1 || kvhs > 65535 || kvh0 < 0 || kvh0 + kvhs > nkv || blocks < 1 ||
         num_splits < 1 || num_splits > 65535 || (num_splits > 1 && (part_o == nullptr || part_lse == nullptr)) ||
-        slots != (n_tiles < rows ? n_tiles : rows))
+        (slot_rows == nullptr && (slots != (n_tiles < rows ? n_tiles : rows) || (int64_t)slots * cap > room)))
         return ACORN_ERR_UNSUPPORTED;
     PrefillF8Params pp;
     F8AttnParams& p = pp.a;
@@ -598,10 +631,10 @@ extern "C" int acorn_attention_prefill_f8(const void* q, int64_t q_stride, int t
     p.row_start = row_start; p.row_pos = row_pos; p.tiles = tiles; p.sink = sink; p.table_stride = table_stride;
     p.nq = nq; p.nkv = nkv; p.mask = {window, chunk, keep}; p.scale_log2 = scale * 1.4426950408889634f;
     p.logP = acorn_log2_exact_tc(P);
-    pp.pairs = (nq / nkv + 1) / 2; pp.n_tiles = n_tiles; pp.rows = rows; pp.cap = cap; pp.kvh0 = kvh0; pp.kvhs = kvhs;
+    pp.pairs = (nq / nkv + 1) / 2; pp.n_tiles = n_tiles; pp.rows = rows; pp.cap = cap; pp.room = room; pp.slot_rows = slot_rows; pp.slots = slots; pp.kvh0 = kvh0; pp.kvhs = kvhs;
     pp.num_splits = num_splits; pp.k_rows = (bf16*)k_rows; pp.v_rows = (bf16*)v_rows; pp.part_o = part_o; pp.part_lse = part_lse;
     if ((int64_t)n_tiles * kvhs * pp.pairs > 0x7fffffff || (int64_t)n_tiles * PF8_BM * nq > ((int64_t)1 << 33)) return ACORN_ERR_UNSUPPORTED;
-    return d == 128 ? launch_prefill_f8<128>(pp, tokens, slots, blocks, stream) : launch_prefill_f8<64>(pp, tokens, slots, blocks, stream);
+    return d == 128 ? launch_prefill_f8<128>(pp, tokens, blocks, stream) : launch_prefill_f8<64>(pp, tokens, blocks, stream);
 }
 
 extern "C" int acorn_attention_prefill_f8_error() {

@@ -57,7 +57,7 @@ STEP_ARRAYS = {
 }
 
 # The same for an 8-bit cache (``paged_attention_f8``): single tokens, tiles of the rows of a few tokens (as many tokens a tile as the
-# kernel's sixteen query rows hold), tiles of 128 of the longer ones.
+# kernel's sixteen query rows hold), tiles of 128 of the longer ones and a list of those rows.
 F8_LARGE_MIN = 32
 
 
@@ -73,7 +73,22 @@ def f8_step_arrays(nq: int, nkv: int) -> dict:
         "attention.f8_single": lambda plan: _tiles(plan, 1, 2, 1),
         f"attention.f8_short{step}": lambda plan: _tiles(plan, 2, F8_LARGE_MIN, step),
         "attention.f8_large": large,
+        "attention.f8_large_rows": lambda plan: np.asarray([r for r, n in enumerate(plan.row_lens) if n >= F8_LARGE_MIN], np.int32),
     }
+
+
+def _f8_prompt_keys(inputs, group_index: int, width_keys: int) -> list[int]:
+    """Keys that the rows of "attention.f8_large_rows" hold; in a step that is captured, and replayed for rows of other lengths, as many as the
+    table has room for."""
+    plan = inputs.plan
+    rows = plan.extra["attention.f8_large_rows"]
+    if torch.cuda.is_current_stream_capturing():
+        return [width_keys] * rows.shape[0]
+    key = ("attention.f8_prompt_keys", group_index)
+    if key not in inputs.extra:                   # made by the first layer of a step that asks, and kept for the others
+        base, page = plan.groups[group_index].page_base, width_keys // plan.groups[group_index].block_table.shape[1]
+        inputs.extra[key] = [int(plan.row_pos[r]) + plan.row_lens[r] - int(base[r]) * page for r in rows]
+    return inputs.extra[key]
 
 
 sm_count = ops.device_sms
@@ -215,7 +230,8 @@ def paged_attention_f8(q: torch.Tensor, inputs, group, cache, nq: int, nkv: int,
     rest = (T, nq, nkv, d, scale, window)
     mask = {"out": out, "chunk": chunk, "keep_first": keep_first, "sink32": sink32}
     if hx["attention.f8_large"].shape[0]:
-        ops.attention_prefill_f8(*args, x["attention.f8_large"], *rest, **mask)
+        ops.attention_prefill_f8(*args, x["attention.f8_large"], *rest, prompt_rows=x["attention.f8_large_rows"],
+                                 prompt_keys=_f8_prompt_keys(inputs, cache.group, group.block_table.shape[1] * cache.k_pages.shape[2]), **mask)
     step = ops.f8_tile_tokens(nq, nkv)
     for name, most in ((f"attention.f8_short{step}", step), ("attention.f8_single", 1)):
         if hx[name].shape[0]:

@@ -153,7 +153,8 @@ class _Sigs:
                                  c_int, c_void_p, c_void_p, c_void_p, c_void_p]
     acorn_attention_prefill_f8 = [c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
                                   c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int,
-                                  c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]
+                                  c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p,
+                                  c_void_p, c_void_p]
     acorn_attention_prefill_f8_supported = [c_int, c_int, c_int, c_int]
     acorn_attention_prefill_f8_error = []
     acorn_attention_prefill_f8_set_error_word = [c_void_p]
@@ -1247,14 +1248,27 @@ def attention_prefill_f8(q: torch.Tensor, q_stride: int, k_pages: torch.Tensor, 
                          block_table: torch.Tensor, page_base: torch.Tensor, row_start: torch.Tensor, row_pos: torch.Tensor,
                          tiles: torch.Tensor, num_tokens: int, num_heads: int, num_kv_heads: int, head_dim: int, scale: float,
                          window: int | None, out: torch.Tensor | None = None, chunk: int | None = None, keep_first: int = 0,
-                         sink32: torch.Tensor | None = None, num_splits: int | None = None) -> torch.Tensor:
+                         sink32: torch.Tensor | None = None, num_splits: int | None = None,
+                         prompt_rows: torch.Tensor | None = None, prompt_keys: list[int] | None = None) -> torch.Tensor:
     """Causal attention of prompts, or portions of them, over the pages of an 8-bit cache: as ``attention_decode_f8``, in tiles
     of up to 128 tokens (``F8_PREFILL_TILE``).  CTAs start in the order of the list: give the tiles that read the most keys
-    first.  Head sizes 64 and 128 with a positive scale run on the tensor cores, from bfloat16 rows of the keys and values that
-    the call makes in scratch of its own (of at most ``F8_PREFILL_SCRATCH`` bytes or one kv head's)."""
+    first.  Head sizes 64 and 128 with a positive scale run on the tensor cores, from bfloat16 rows of the keys and values of
+    the rows that have tiles, which the call makes in scratch of its own (of at most ``F8_PREFILL_SCRATCH`` bytes or one kv
+    head's).
+
+    ``prompt_rows`` (int32 [n]) and ``prompt_keys``: the rows that have tiles, each once, and how many keys each of them holds
+    (given-back pages not counted; a bound will do), so that the scratch is for those.  Without them it is for the widest row of the
+    table, as often as there are rows or tiles, whichever are fewer."""
     what = "attention_prefill_f8"
     P, out, stream = _check_f8_attention(what, q, q_stride, k_pages, v_pages, scales, block_table, page_base, row_start, row_pos, tiles,
                                          num_tokens, num_heads, num_kv_heads, head_dim, window, out, chunk, keep_first, sink32)
+    if (prompt_rows is None) != (prompt_keys is None):
+        raise KernelError(f"{what}: prompt_rows and prompt_keys go together")
+    if prompt_rows is not None:
+        _check_tensors(what, q.get_device(), (prompt_rows, "prompt_rows", torch.int32, 1))
+        if prompt_rows.numel() != len(prompt_keys) or not 0 < len(prompt_keys) <= block_table.shape[0] or min(prompt_keys) < 1:
+            raise KernelError(f"{what}: {prompt_rows.numel()} prompt_rows with {len(prompt_keys)} prompt_keys (a positive number each) "
+                              f"for a table of {block_table.shape[0]} rows")
     if not (scale > 0 and lib().acorn_attention_prefill_f8_supported(num_heads, num_kv_heads, head_dim, P)):
         return _attention_f8_plain(q, q_stride, out, k_pages, v_pages, scales, block_table, page_base, row_start, row_pos, tiles,
                                    F8_PREFILL_TILE, num_heads, num_kv_heads, head_dim, P, scale, window, chunk, keep_first, sink32,
@@ -1263,18 +1277,25 @@ def attention_prefill_f8(q: torch.Tensor, q_stride: int, k_pages: torch.Tensor, 
     if n == 0:
         return out
     # the keys of every row that has tiles, as rows of bfloat16, for as many kv heads at a time as the scratch has room for
-    slots, cap = min(rows, n), ((width * P + 127) // 128 + 1) * 128
-    kvhs = max(1, min(num_kv_heads, F8_PREFILL_SCRATCH // (slots * cap * head_dim * 4)))
-    if slots > 65535 or slots * kvhs * cap >= 1 << 31:
+    widest = width * P
+    if prompt_rows is None:
+        slots, cap = min(rows, n), ((widest + 127) // 128 + 1) * 128
+        room = slots * cap
+    else:
+        slots, widest = prompt_rows.shape[0], min(widest, max(prompt_keys))
+        cap = ((widest + 127) // 128 + 1) * 128
+        room = sum((min(k, width * P) + 127) // 128 + 1 for k in prompt_keys) * 128      # (a first page need not start a block)
+    kvhs = max(1, min(num_kv_heads, F8_PREFILL_SCRATCH // (room * head_dim * 4)))
+    if slots > 65535 or kvhs * room >= 1 << 31:
         raise KernelError(f"{what}: {slots} rows of {width} pages are too many for one call")
     pairs = -(-(num_heads // num_kv_heads) // 2)
     spans = [v for v in (window, chunk) if v]
-    keys = min([width * P] + [v + F8_PREFILL_TILE + (keep_first or 0) for v in spans])
+    keys = min([widest] + [v + F8_PREFILL_TILE + (keep_first or 0) for v in spans])
     if num_splits is None:
         num_splits = prefill_f8_splits(n * kvhs * pairs, -(-keys // 128), device_sms(q.device))
     if not 1 <= num_splits <= F8_MAX_SPLITS:
         raise KernelError(f"{what}: num_splits must be in 1..{F8_MAX_SPLITS}, got {num_splits}")
-    scratch = torch.empty((2, slots, kvhs, cap, head_dim), dtype=torch.bfloat16, device=q.device)
+    scratch = torch.empty((2, kvhs, room, head_dim), dtype=torch.bfloat16, device=q.device)
     part_o = part_lse = None
     if num_splits > 1:
         part_o = torch.empty((num_splits, n, F8_PREFILL_TILE, num_heads, head_dim), dtype=torch.float32, device=q.device)
@@ -1285,8 +1306,8 @@ def attention_prefill_f8(q: torch.Tensor, q_stride: int, k_pages: torch.Tensor, 
                                              rows, row_start.data_ptr(), row_pos.data_ptr(), tiles.data_ptr(), n, num_heads,
                                              num_kv_heads, head_dim, P, float(scale), int(window or 0), int(chunk or 0),
                                              int(keep_first or 0), _ptr(sink32), first, min(kvhs, num_kv_heads - first),
-                                             scratch[0].data_ptr(), scratch[1].data_ptr(), slots, cap, min(cap // 32, 4096), num_splits,
-                                             _ptr(part_o), _ptr(part_lse), stream), what)
+                                             scratch[0].data_ptr(), scratch[1].data_ptr(), _ptr(prompt_rows), slots, cap, room,
+                                             min(cap // 32, 4096), num_splits, _ptr(part_o), _ptr(part_lse), stream), what)
     return out
 
 
