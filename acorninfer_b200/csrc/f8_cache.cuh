@@ -58,6 +58,16 @@ __device__ __forceinline__ float2 f8_codes2(uint32_t two) {
     return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
+// A head's norm as the writers of the cache take it.  The reciprocal root of a mean square, to its last bits: codes flip where an
+// entry lies near the middle of two, so a Newton step follows the approximation (not at infinity, where it would make 0 into NaN).
+__device__ __forceinline__ float f8_inverse_root(float mean) {
+    const float guess = rsqrtf(mean);
+    return mean > 1e-30f && mean < INFINITY ? fmaf(0.5f * guess, fmaf(-mean * guess, guess, 1.f), guess) : guess;
+}
+// Finite entries beyond 2^60 or so have a sum of squares beyond the floats; times this power of two they do not, and the norm is
+// the same without its epsilon, which is nothing beside them.
+#define F8_NORM_DOWN 8.4703294725430034e-22f          // 2^-70
+
 // What the attention kernels over these pages are given.
 struct F8AttnParams {
     const bf16* q;            // [tokens, q_stride]: query heads first in each row

@@ -371,8 +371,15 @@ __global__ void __launch_bounds__(TC_THREADS) gemm_tcgen05_kernel(const __grid_c
             for (int j = 0; j < 4; ++j) v[j] = tile_sum(i, lane + 32 * j) * inv_s[m];
             if (is_q || is_k) {
                 if (hw != nullptr) {
-                    const float ss = warp_sum((v[0] * v[0] + v[1] * v[1]) + (v[2] * v[2] + v[3] * v[3]));
-                    const float f = rsqrtf(ss / (float)TC_BM + p.rope_eps);
+                    float ss = warp_sum((v[0] * v[0] + v[1] * v[1]) + (v[2] * v[2] + v[3] * v[3]));
+                    const bool large = p.scales != nullptr && ss == INFINITY;
+                    if (large) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) v[j] *= F8_NORM_DOWN;
+                        ss = warp_sum((v[0] * v[0] + v[1] * v[1]) + (v[2] * v[2] + v[3] * v[3]));
+                    }
+                    const float mean = ss / (float)TC_BM + (large ? 0.f : p.rope_eps);
+                    const float f = p.scales != nullptr ? f8_inverse_root(mean) : rsqrtf(mean);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) v[j] = v[j] * f * wcol[j];
                 }

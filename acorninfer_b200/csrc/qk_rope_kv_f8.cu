@@ -125,10 +125,20 @@ __global__ void __launch_bounds__(KVF8_THREADS, 8) qk_rope_kv_f8_kernel(const Kv
             for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
 #pragma unroll
             for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            const bool large = w && ss == INFINITY;
+            if (__any_sync(0xffffffffu, large)) {             // rare: the same for a row brought down
+                if (large) {
+                    ss = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) { x[i] *= F8_NORM_DOWN; ss = fmaf(x[i], x[i], ss); }
+                }
+                float all = ss;
+#pragma unroll
+                for (int o = LPH / 2; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+                if (large) ss = all;
+            }
             if (w && live) {
-                const float mean = fmaf(ss, p.inv_d, p.eps), guess = rsqrtf(mean);
-                // a Newton step: codes flip where an entry lies near the middle of two, so that every bit counts
-                const float inv = mean > 1e-30f ? fmaf(0.5f * guess, fmaf(-mean * guess, guess, 1.f), guess) : guess;
+                const float inv = f8_inverse_root(fmaf(ss, p.inv_d, large ? 0.f : p.eps));
                 const float4 wa = *reinterpret_cast<const float4*>(w + at0), wb = *reinterpret_cast<const float4*>(w + at1);
                 x[0] *= inv * wa.x; x[1] *= inv * wa.y; x[2] *= inv * wa.z; x[3] *= inv * wa.w;
                 x[4] *= inv * wb.x; x[5] *= inv * wb.y; x[6] *= inv * wb.z; x[7] *= inv * wb.w;
