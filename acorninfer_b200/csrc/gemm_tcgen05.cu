@@ -73,6 +73,7 @@ struct TcParams {
     bf16* k_pages;
     bf16* v_pages;           // nullptr: keys and values are not written (a layer that reads another's cache)
     uint8_t* scales;         // [page, nkv, P, 2]: the pages hold e4m3 codes and these their rows' powers of two (f8_cache.cuh); or nullptr
+    int eight_bit;           // the layer's cache is an 8-bit one, here or in another layer: angles and the norm's root as f8_cache.cuh has them
     int table_stride, nq, nkv, logP;
     float rope_eps;
     // TC_MODE_GELU_ROWS: row gate_ids[m] of gate_rows ([rows, gate_ld] bf16), columns from gate_col0
@@ -372,26 +373,27 @@ __global__ void __launch_bounds__(TC_THREADS) gemm_tcgen05_kernel(const __grid_c
             if (is_q || is_k) {
                 if (hw != nullptr) {
                     float ss = warp_sum((v[0] * v[0] + v[1] * v[1]) + (v[2] * v[2] + v[3] * v[3]));
-                    const bool large = p.scales != nullptr && ss == INFINITY;
+                    const bool large = p.eight_bit && ss == INFINITY;
                     if (large) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j) v[j] *= F8_NORM_DOWN;
                         ss = warp_sum((v[0] * v[0] + v[1] * v[1]) + (v[2] * v[2] + v[3] * v[3]));
                     }
                     const float mean = ss / (float)TC_BM + (large ? 0.f : p.rope_eps);
-                    const float f = p.scales != nullptr ? f8_inverse_root(mean) : rsqrtf(mean);
+                    const float f = p.eight_bit ? f8_inverse_root(mean) : rsqrtf(mean);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) v[j] = v[j] * f * wcol[j];
                 }
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     float sn, cs;
-                    float angle = (float)pos_s[m] * freq[j];
-                    if (p.scales != nullptr) {               // an 8-bit cache: as qk_rope_kv_f8.cu makes it, right at far positions too
-                        const double far = (double)pos_s[m] * (double)freq[j];
-                        angle = (float)fma(-rint(far * 0.15915494309189535), 6.283185307179586, far);
+                    if (p.eight_bit) {
+                        const float2 turn = f8_turn(pos_s[m], freq[j]);
+                        cs = turn.x;
+                        sn = turn.y;
+                    } else {
+                        sincosf((float)pos_s[m] * freq[j], &sn, &cs);
                     }
-                    sincosf(angle, &sn, &cs);
                     const float a = v[j], b = v[j + 2];
                     v[j] = a * cs - b * sn;
                     v[j + 2] = b * cs + a * sn;
@@ -573,15 +575,16 @@ extern "C" int acorn_gemm_tc_gelu_rows(const void* x, int64_t ldx, const void* w
 // The q/k/v product of an attention layer with head size 128 (TC_MODE_QKV_ROPE): w is [(nq + 2 nkv)
 // * 128, K]; out [M, ldo] takes the query heads; k_pages / v_pages ([pages, nkv, P, 128], P a power
 // of two) the keys and values, or nothing when they are nullptr.  With scales ([pages, nkv, P, 2]) the pages are those of an 8-bit
-// cache: e4m3 codes, and their rows' powers of two.
+// cache: e4m3 codes, and their rows' powers of two.  eight_bit: queries for such a cache, whoever writes it.
 extern "C" int acorn_gemm_tc_qkv_rope(const void* x, int64_t ldx, const void* w, int64_t ldw, void* out, int64_t ldo,
                                       int M, int K, int splits, int per_sm, const float* ss_in, int ss_parts,
                                       int norm_width, float eps, const int* positions, const int* token_row,
                                       const int* block_table, const int* page_base, int table_stride, void* k_pages,
                                       void* v_pages, void* scales, const float* q_w, const float* k_w, const float* inv_freq, int nq,
-                                      int nkv, int P, float rope_eps, cudaStream_t stream) {
+                                      int nkv, int P, int eight_bit, float rope_eps, cudaStream_t stream) {
     const int logP = acorn_log2_exact_tc(P);
-    if (scales != nullptr && v_pages == nullptr) return ACORN_ERR_UNSUPPORTED;
+    if (scales != nullptr && (v_pages == nullptr || !eight_bit)) return ACORN_ERR_UNSUPPORTED;
+    if (v_pages != nullptr && scales == nullptr && eight_bit) return ACORN_ERR_UNSUPPORTED;
     if (nq < 1 || nkv < 1 || logP < 0 || positions == nullptr || inv_freq == nullptr) return ACORN_ERR_UNSUPPORTED;
     if ((k_pages == nullptr) != (v_pages == nullptr)) return ACORN_ERR_UNSUPPORTED;
     if (k_pages != nullptr && (token_row == nullptr || block_table == nullptr || page_base == nullptr)) return ACORN_ERR_UNSUPPORTED;
@@ -590,7 +593,7 @@ extern "C" int acorn_gemm_tc_qkv_rope(const void* x, int64_t ldx, const void* w,
     p.mode = TC_MODE_QKV_ROPE; p.ss_in = ss_in; p.ss_parts = ss_parts; p.norm_width = norm_width; p.eps = eps;
     p.positions = positions; p.token_row = token_row; p.block_table = block_table; p.page_base = page_base;
     p.table_stride = table_stride; p.k_pages = (bf16*)k_pages; p.v_pages = (bf16*)v_pages; p.q_w = q_w; p.k_w = k_w;
-    p.scales = (uint8_t*)scales; p.inv_freq = inv_freq; p.nq = nq; p.nkv = nkv; p.logP = logP; p.rope_eps = rope_eps;
+    p.scales = (uint8_t*)scales; p.eight_bit = eight_bit; p.inv_freq = inv_freq; p.nq = nq; p.nkv = nkv; p.logP = logP; p.rope_eps = rope_eps;
     return run_tc(x, ldx, w, ldw, p, splits, per_sm, stream);
 }
 

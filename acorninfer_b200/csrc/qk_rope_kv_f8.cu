@@ -13,9 +13,8 @@
 // largest magnitude are shuffles among them.  Heads rotated whole in pairs (j, j + d/2) give a lane four entries of each half, so
 // that it holds whole pairs (PAIRED); otherwise the eight are neighbours, and the other half of a pair is a shuffle more.
 // What bounds it: its instructions, not its bytes; so only the key and value heads look for their largest magnitude, by a
-// maximum that hands NaN on, which tells infinities and NaN as well.
-// The angle is formed and brought to [-pi, pi] in 64 bits: in 32 its error is 2^-24 of the angle itself, 0.008 radians at
-// position 131,072, against 2^-9 of a rounding to bfloat16.
+// maximum that hands NaN on, which tells infinities and NaN as well.  Without pages the queries alone are made (a layer that reads
+// another one's cache), with the very same angles.
 #include "f8_cache.cuh"
 
 #define KVF8_THREADS 256
@@ -73,7 +72,7 @@ __device__ __forceinline__ uint2 kvf8_codes(const float (&x)[8], int e) {
     return make_uint2(f8_pack2(z[0], z[1]) | f8_pack2(z[2], z[3]) << 16, f8_pack2(z[4], z[5]) | f8_pack2(z[6], z[7]) << 16);
 }
 
-template <int LPH, bool PAIRED>
+template <int LPH, bool PAIRED, bool WRITE>
 __global__ void __launch_bounds__(KVF8_THREADS, 8) qk_rope_kv_f8_kernel(const KvF8Params p) {
     extern __shared__ __align__(16) float2 turn[];            // cos and sin of the token's angles
     pdl_wait();
@@ -81,7 +80,7 @@ __global__ void __launch_bounds__(KVF8_THREADS, 8) qk_rope_kv_f8_kernel(const Kv
     const int t = blockIdx.x;
     const int pos = p.positions[t], r = p.token_row[t];
     const int half = p.rot >> 1;
-    const int heads = p.nq + 2 * p.nkv;
+    const int heads = WRITE ? p.nq + 2 * p.nkv : p.nq;
     const int l = threadIdx.x & (LPH - 1);
     const bool on = 8 * l < p.d;                              // lanes beyond a head whose size is no power of two
     // this lane's entries: at0 .. at0 + 3 and at1 .. at1 + 3
@@ -96,14 +95,10 @@ __global__ void __launch_bounds__(KVF8_THREADS, 8) qk_rope_kv_f8_kernel(const Kv
     const int in_pass = threadIdx.x / LPH, per_cta = blockDim.x / LPH, per_pass = per_cta * gridDim.y;
     int h0 = blockIdx.y * per_cta;
     uint4 raw = fetch(h0 + in_pass);                          // on its way while the angles are made
-    const int page = p.block_table[(int64_t)r * p.table_stride + ((pos >> p.logP) - p.page_base[r])];
+    const int page = WRITE ? p.block_table[(int64_t)r * p.table_stride + ((pos >> p.logP) - p.page_base[r])] : 0;
     for (int j = threadIdx.x; j < half; j += blockDim.x) {
-        const double a = (double)pos * (double)p.inv_freq[j];
-        const double z = fma(-rint(a * 0.15915494309189535), 6.283185307179586, a);
-        const float zh = (float)z, zl = (float)(z - (double)zh);         // sin(zh + zl) = sin zh + zl cos zh, zl < 2^-23
-        float s, c;
-        sincosf(zh, &s, &c);
-        turn[j] = make_float2(fmaf(-s, zl, c) * p.magnitude, fmaf(c, zl, s) * p.magnitude);
+        const float2 cs = f8_turn(pos, p.inv_freq[j]);
+        turn[j] = make_float2(cs.x * p.magnitude, cs.y * p.magnitude);
     }
     __syncthreads();
     const int64_t slot0 = (((int64_t)page * p.nkv) << p.logP) + (pos & ((1 << p.logP) - 1));
@@ -217,18 +212,20 @@ __global__ void __launch_bounds__(KVF8_THREADS, 8) qk_rope_kv_f8_kernel(const Kv
     }
 }
 
-template <int LPH, bool PAIRED>
+template <int LPH, bool PAIRED, bool WRITE>
 static int launch_kv_f8(const KvF8Params& p, cudaStream_t stream) {
     // as few passes as 256 threads need, and as many threads as those passes leave no idle ones; few tokens: a CTA a pass
-    const int lanes = (p.nq + 2 * p.nkv) * LPH, passes = (lanes + KVF8_THREADS - 1) / KVF8_THREADS;
+    const int lanes = (WRITE ? p.nq + 2 * p.nkv : p.nq) * LPH, passes = (lanes + KVF8_THREADS - 1) / KVF8_THREADS;
     const int threads = ((lanes + passes - 1) / passes + 31) / 32 * 32;
-    return acorn_launch(qk_rope_kv_f8_kernel<LPH, PAIRED>, dim3(p.tokens, p.tokens < 2 * acorn_sms() ? passes : 1), dim3(threads),
+    return acorn_launch(qk_rope_kv_f8_kernel<LPH, PAIRED, WRITE>, dim3(p.tokens, p.tokens < 2 * acorn_sms() ? passes : 1), dim3(threads),
                         (size_t)(p.rot / 2) * sizeof(float2), stream, p);
 }
 
 template <int LPH>
 static int launch_kv_f8(const KvF8Params& p, cudaStream_t stream) {
-    return p.rot == p.d && !p.interleaved ? launch_kv_f8<LPH, true>(p, stream) : launch_kv_f8<LPH, false>(p, stream);
+    const bool paired = p.rot == p.d && !p.interleaved;
+    if (p.k_pages == nullptr) return paired ? launch_kv_f8<LPH, true, false>(p, stream) : launch_kv_f8<LPH, false, false>(p, stream);
+    return paired ? launch_kv_f8<LPH, true, true>(p, stream) : launch_kv_f8<LPH, false, true>(p, stream);
 }
 
 extern "C" int acorn_qk_rope_kv_f8(const void* qkv, int64_t ld, const float* q_w, const float* k_w, const float* bias,
@@ -237,6 +234,7 @@ extern "C" int acorn_qk_rope_kv_f8(const void* qkv, int64_t ld, const float* q_w
                                    void* q_out, int64_t ld_q, int tokens, int nq, int nkv, int d, int rot, int interleaved,
                                    int P, float eps, float magnitude, cudaStream_t stream) {
     if (tokens <= 0) return 0;
+    if ((k_pages == nullptr) != (v_pages == nullptr) || (k_pages == nullptr) != (scales == nullptr)) return ACORN_ERR_UNSUPPORTED;
     if (d < 8 || d % 8 || d > 256 || rot < 0 || rot > d || rot % (interleaved ? 2 : 16) || P < 1 || (P & (P - 1)) || nq < 1 || nkv < 1 ||
         ld % 8 || ld_q % 8)
         return ACORN_ERR_UNSUPPORTED;

@@ -284,7 +284,7 @@ class _Sigs:
                                c_void_p, c_void_p, c_int64, c_int, c_void_p]
     acorn_gemm_tc_qkv_rope = [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int, c_int,
                               c_void_p, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
-                              c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_void_p]
+                              c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_float, c_void_p]
     acorn_gemm_tc_supported = [c_int64, c_int64, c_int64, c_int64, c_int64]
     acorn_gemm_tc_pair = [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int,
                           c_int, c_void_p, c_int, c_int, c_float, c_void_p, c_int64, c_void_p, c_void_p, c_void_p]
@@ -682,7 +682,7 @@ def _stream_of(what: str, device: int) -> int:
 
 def qk_rope_kv_f8(qkv: torch.Tensor, q_weight32: torch.Tensor | None, k_weight32: torch.Tensor | None, inv_freq: torch.Tensor,
                   positions: torch.Tensor, token_row: torch.Tensor, block_table: torch.Tensor, page_base: torch.Tensor,
-                  k_pages: torch.Tensor, v_pages: torch.Tensor, scales: torch.Tensor, num_heads: int, num_kv_heads: int,
+                  k_pages: torch.Tensor | None, v_pages: torch.Tensor | None, scales: torch.Tensor | None, num_heads: int, num_kv_heads: int,
                   head_dim: int, rotary_dim: int, interleaved: bool, eps: float, bias32: torch.Tensor | None = None,
                   magnitude: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
     """``qk_rope_kv`` into an 8-bit cache: per-head q/k norm, rotary encoding, keys and values quantised and written into
@@ -696,12 +696,22 @@ def qk_rope_kv_f8(qkv: torch.Tensor, q_weight32: torch.Tensor | None, k_weight32
     numbers (the attention kernels do not expect e4m3's two codes of NaN).  ``k_pages`` / ``v_pages``: float8_e4m3fn [pages, nkv, page, d];
     ``scales``: float8_e8m0fnu [pages, nkv, page, 2], a token's key scale and value scale.
 
+    Without pages (``k_pages``, ``v_pages`` and ``scales`` None) the queries alone are made, as for a cache written with them: what a
+    layer does that reads another layer's cache.
+
     ``bias32`` (float32, an entry per channel of a row) is added first; ``magnitude``: a factor on cos and sin.  Head sizes
     are multiples of 8 up to 256; ``rotary_dim`` is a multiple of 16 (of 2 with ``interleaved`` pairs)."""
     what = "qk_rope_kv_f8"
     _check(qkv, "qkv", torch.bfloat16, 2)
     device = qkv.get_device()
-    P = _check_f8_pages(what, device, k_pages, v_pages, scales, num_kv_heads, head_dim)
+    if k_pages is not None or v_pages is not None or scales is not None:
+        if k_pages is None or v_pages is None or scales is None:
+            raise KernelError(f"{what}: k_pages, v_pages and scales go together")
+        P = _check_f8_pages(what, device, k_pages, v_pages, scales, num_kv_heads, head_dim)
+    else:
+        P = 1
+        if head_dim % 8 or not 8 <= head_dim <= F8_MAX_HEAD:
+            raise KernelError(f"{what}: head sizes are multiples of 8 up to {F8_MAX_HEAD}, got {head_dim}")
     (T, width), channels = qkv.shape, (num_heads + 2 * num_kv_heads) * head_dim
     if num_heads < 1 or num_kv_heads < 1 or width < channels or width % 8 or qkv.data_ptr() % 16:
         raise KernelError(f"{what}: rows of {width} for {channels} channels (a multiple of 8, on 16-byte boundaries)")
@@ -729,7 +739,7 @@ def qk_rope_kv_f8(qkv: torch.Tensor, q_weight32: torch.Tensor | None, k_weight32
         raise KernelError(f"{what}: out {tuple(out.shape)} does not hold [{T}, {num_heads * head_dim}] in rows of a multiple of 8")
     _ok(lib().acorn_qk_rope_kv_f8(qkv.data_ptr(), width, _ptr(q_weight32), _ptr(k_weight32), _ptr(bias32), inv_freq.data_ptr(),
                                   positions.data_ptr(), token_row.data_ptr(), block_table.data_ptr(), page_base.data_ptr(), table_stride,
-                                  k_pages.data_ptr(), v_pages.data_ptr(), scales.data_ptr(), out.data_ptr(), out_width, T, num_heads,
+                                  _ptr(k_pages), _ptr(v_pages), _ptr(scales), out.data_ptr(), out_width, T, num_heads,
                                   num_kv_heads, head_dim, rotary_dim, 1 if interleaved else 0, P, float(eps), float(magnitude),
                                   _stream_of(what, device)), what)
     return out
@@ -1522,6 +1532,7 @@ class RopeKvEpilogue:
     eps: float
     cos_sin: torch.Tensor | None = None      # [M, 128] float32 from ``rope_table``: spares the epilogue its sincosf
     scales: torch.Tensor | None = None       # the pages are an 8-bit cache's, and these its rows' powers of two (``qk_rope_kv_f8``)
+    eight_bit: bool = False                  # without pages: queries for an 8-bit cache of another layer, with its writer's angles
 
 
 def rope_table(positions: torch.Tensor, inv_freq: torch.Tensor) -> torch.Tensor:
@@ -1550,9 +1561,11 @@ def gemm_tc_qkv_rope(x, w: torch.Tensor, ep: RopeKvEpilogue, out: torch.Tensor |
     if ep.inv_freq.numel() != 64 or ep.positions.numel() < M:
         raise KernelError("gemm_tc_qkv_rope: inv_freq must have 64 entries and positions one per row")
     P = 1
+    eight_bit = ep.scales is not None or ep.eight_bit
+    if eight_bit:
+        if M > GEMM_TC_FUSED_MAX_ROWS or (ep.k_pages is None) != (ep.scales is None):
+            raise KernelError(f"gemm_tc_qkv_rope: up to {GEMM_TC_FUSED_MAX_ROWS} rows are made for an 8-bit cache, pages with their scales, got {M}")
     if ep.scales is not None:
-        if M > GEMM_TC_FUSED_MAX_ROWS or ep.k_pages is None:
-            raise KernelError(f"gemm_tc_qkv_rope: up to {GEMM_TC_FUSED_MAX_ROWS} rows are written into an 8-bit cache, got {M}")
         _check_f8_pages("gemm_tc_qkv_rope", xt.get_device(), ep.k_pages, ep.v_pages, ep.scales, nkv, 128)
     if ep.k_pages is not None:
         _check(ep.k_pages, "k_pages", F8 if ep.scales is not None else torch.bfloat16, 4)
@@ -1589,8 +1602,8 @@ def gemm_tc_qkv_rope(x, w: torch.Tensor, ep: RopeKvEpilogue, out: torch.Tensor |
         rows.width if rows is not None else 0, float(rows.eps) if rows is not None else 0.0,
         ep.positions.data_ptr(), _ptr(ep.token_row), _ptr(ep.block_table), _ptr(ep.page_base),
         ep.block_table.stride(0) if ep.block_table is not None else 0, _ptr(ep.k_pages), _ptr(ep.v_pages), _ptr(ep.scales),
-        _ptr(ep.q_weight32), _ptr(ep.k_weight32), ep.inv_freq.data_ptr(), nq, nkv, P, float(ep.eps), _stream()),
-        "gemm_tc_qkv_rope", f"{M}x{N}x{K}")
+        _ptr(ep.q_weight32), _ptr(ep.k_weight32), ep.inv_freq.data_ptr(), nq, nkv, P, 1 if eight_bit else 0,
+        float(ep.eps), _stream()), "gemm_tc_qkv_rope", f"{M}x{N}x{K}")
     return out
 
 

@@ -286,12 +286,11 @@ class Attention(Mixer):
             q = ops.qk_rope_kv_f8(proj, self.q_norm32, self.k_norm32, inv_freq, inputs.positions, inputs.token_row, g.block_table,
                                   g.page_base, cache.k_pages, cache.v_pages, cache.scales, self.nq, self.nkv, self.d, rot, interleaved,
                                   eps, bias32=self.bias32, magnitude=magnitude)
-        else:                                 # another run's cache is read: the queries alone, in place
+        else:                                 # another run's cache is read: the queries alone
             if self.bias:
                 raise ValueError("attention: biased projections need a cache of the run's own")
-            q = proj
-            ops.qk_rope_kv(proj, self.q_norm32, self.k_norm32, inv_freq, inputs.positions, inputs.token_row, g.block_table, g.page_base,
-                           None, None, self.nq, self.nkv, self.d, rot, interleaved, eps, write_kv=False, magnitude=magnitude)
+            q = ops.qk_rope_kv_f8(proj, self.q_norm32, self.k_norm32, inv_freq, inputs.positions, inputs.token_row, g.block_table,
+                                  g.page_base, None, None, None, self.nq, self.nkv, self.d, rot, interleaved, eps, magnitude=magnitude)
         heads = attn_kernels.paged_attention_f8(q, inputs, g, cache, self.nq, self.nkv, self.d, self.scale, self.window,
                                                 chunk=self.chunk, keep_first=self.keep_first, sink32=self.sink32)
         if self.head_gate or out_scale != 1.0 or out is not None:
@@ -322,7 +321,7 @@ class Attention(Mixer):
                 self.q_norm32, self.k_norm32, pos.inv_freq, self.nq, self.nkv,
                 self.qk_norm_eps if self.qk_norm_eps is not None else 0.0,
                 cos_sin=pos.table(inputs) if rows > ops.GEMM_TC_FUSED_MAX_ROWS and hasattr(pos, "table") else None,
-                scales=cache.scales if cache.write else None))
+                scales=cache.scales if cache.write else None, eight_bit=self.eight_bit))
             if self.eight_bit:
                 return self._inner_f8(x, inputs, cache, out_scale, out, qkv)
         elif self.eight_bit:

@@ -69,3 +69,63 @@ def test_norms_of_large_rows_in_the_epilogue(power):
         e = byte.double() - 127
         spacing = torch.exp2(torch.floor(torch.log2((want.abs() * torch.exp2(-e)[..., None]).clamp(min=2.0 ** -6))) - 3 + e[..., None])
         assert bool(((f8.dequantise(codes, byte) - want).abs() <= spacing / 2 + 2 * slack[..., None]).all())
+
+
+@pytest.mark.parametrize("nq,nkv,d,rot,inter", [(4, 2, 64, 64, False), (3, 1, 128, 128, False), (6, 3, 96, 48, False), (2, 1, 256, 256, True), (20, 1, 8, 6, True)])
+@pytest.mark.parametrize("norm,bias", [(True, False), (False, True)])
+def test_queries_alone(nq, nkv, d, rot, inter, norm, bias):
+    """Without pages: the bits of the queries of a call that writes, at near and far positions."""
+    P, T = 16, 300
+    qkv, w, b, inv = write_inputs(T, nq, nkv, d, rot, norm, bias, 63, extra=8)
+    positions = torch.arange(T, dtype=torch.int32, device=DEV) * 449
+    pages = 300 * 449 // P + 1
+    cache, table = empty_cache(pages, nkv, P, d), torch.arange(pages, dtype=torch.int32, device=DEV)[None]
+    call = lambda *c, **kw: ops().qk_rope_kv_f8(qkv, w[0], w[1], inv, positions, i32([0] * T), table, i32([0]), *c, nq, nkv, d, rot, inter, 1e-6,     # noqa: E731
+                                                bias32=b, magnitude=1.25, **kw)
+    want = call(*cache)
+    before = qkv.clone()
+    assert torch.equal(call(None, None, None), want) and torch.equal(qkv, before)
+    out = torch.full((T, nq * d + 8), 7.0, dtype=torch.bfloat16, device=DEV)
+    call(None, None, None, out=out)
+    assert torch.equal(out[:, :nq * d], want) and bool((out[:, nq * d:] == 7).all())
+    for pages_given in ((cache[0], None, None), (None, cache[1], cache[2]), (cache[0], cache[1], None)):
+        with pytest.raises(ops().KernelError, match="go together"):
+            call(*pages_given)
+
+
+def test_queries_alone_in_the_epilogue():
+    o, nq, nkv, d, K, T, P = ops(), 4, 2, 128, 512, 11, 16
+    g = torch.Generator().manual_seed(64)
+    x = torch.randn(T, K, generator=g).to(torch.bfloat16).to(DEV)
+    w = (torch.randn((nq + 2 * nkv) * d, K, generator=g) / K ** 0.5).to(torch.bfloat16).to(DEV)
+    norms = [(1 + 0.2 * torch.randn(d, generator=g)).to(DEV) for _ in range(2)]
+    inv = (1.0 / (1e6 ** (torch.arange(0, d, 2, dtype=torch.float32) / d))).to(DEV)
+    pos = torch.arange(T, dtype=torch.int32, device=DEV) * 13001
+    pages = T * 13001 // P + 1
+    cache, table = empty_cache(pages, nkv, P, d), torch.arange(pages, dtype=torch.int32, device=DEV)[None]
+    ep = lambda k, v, s, **kw: o.RopeKvEpilogue(pos, i32([0] * T), table, i32([0]), k, v, norms[0], norms[1], inv, nq, nkv, 1e-6, scales=s, **kw)     # noqa: E731
+    want = o.gemm_tc_qkv_rope(x, w, ep(*cache))[:, :nq * d]
+    assert torch.equal(o.gemm_tc_qkv_rope(x, w, ep(None, None, None, eight_bit=True))[:, :nq * d], want)
+    for bad in (ep(cache[0], cache[1], None, eight_bit=True), ep(None, None, cache[2])):
+        with pytest.raises(o.KernelError):
+            o.gemm_tc_qkv_rope(x, w, bad)
+
+
+@pytest.mark.parametrize("T", [1, 9, 40])
+def test_both_writers_on_the_same_rows(T):
+    """A projection that hands its input on (so that both have the same rows): each right to half a spacing and 2^-19, at far positions too."""
+    o, nq, nkv, d, P, eps = ops(), 2, 2, 128, 16, 1e-6
+    x, wn, _, inv = write_inputs(T, nq, nkv, d, d, True, False, 65)
+    pos = 131071 - 7 * torch.arange(T, dtype=torch.int32, device=DEV)
+    pages = 131072 // P
+    table = torch.arange(pages, dtype=torch.int32, device=DEV)[None]
+    wq, wk, wv = write_wanted(x, wn, None, inv, pos, nq, nkv, d, d, False, eps, 1.0)
+    eye, a, b = torch.eye(x.shape[1]).to(torch.bfloat16).to(DEV), empty_cache(pages, nkv, P, d), empty_cache(pages, nkv, P, d)
+    q1 = o.qk_rope_kv_f8(x, wn[0], wn[1], inv, pos, i32([0] * T), table, i32([0]), *a, nq, nkv, d, d, False, eps)
+    q2 = o.gemm_tc_qkv_rope(x, eye, o.RopeKvEpilogue(pos, i32([0] * T), table, i32([0]), b[0], b[1], wn[0], wn[1], inv, nq, nkv, eps, scales=b[2]))
+    for q, cache in ((q1, a), (q2[:, :nq * d], b)):
+        off = (q.double().cpu().view(T, nq, d) - wq).abs()
+        assert bool((off <= 2.0 ** -8 * wq.abs() + 2.0 ** -19 * wq.abs().amax(-1, keepdim=True)).all())
+        kc, vc, kb, vb = rows_of(cache, table[0].tolist(), 131072, P)
+        check_rows(kc[pos.cpu().long()], kb[pos.cpu().long()], wk)
+        check_rows(vc[pos.cpu().long()], vb[pos.cpu().long()], wv)
