@@ -5,6 +5,8 @@ import pytest
 import torch
 
 from tests.test_f8_cache_gpu import attend, check_attention, ops, raises, random_cache
+from tests.test_f8_engine_gpu import TOL, cached, plain_over_cache, runner_of
+from tests.tiny import TINY_D, make_model_dir, random_tokens, read_weights
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -152,3 +154,21 @@ def test_lists_that_do_not_fit_are_refused_or_flagged():
     call(i32([0, 1]), [150, 340])
     torch.cuda.synchronize()
     o.raise_on_kernel_error()
+
+
+def test_captured_portions_replayed_for_longer_rows(tmp_path):
+    """A portion of a prompt alone in its step, captured once and replayed for rows that hold more: the plain model's logits."""
+    from acorninfer_b200.engine.batch import StepEntry
+    tiny = {**TINY_D, "page_size": 16}
+    folder = make_model_dir(tmp_path / "m", tiny)
+    V, L, w = tiny["cfg"].vocab_size, tiny["cfg"].num_hidden_layers, read_weights(folder)
+    runner = runner_of(folder, tiny, num_blocks=64)
+    for r in range(5):
+        rc, ids, got = runner.open(f"r{r}"), random_tokens(36 * 7, V, 70 + r), {}
+        for at in range(0, len(ids), 36):                     # buckets of 64; tables of 8 pages, then of 16
+            got[at + 35] = runner.step([StepEntry(rc, ids[at:at + 36], [35])])[0].double().cpu()
+        want, _ = plain_over_cache(tiny, w, ids, [cached(runner, rc, e, len(ids)) for e in range(L)])
+        for pos, row in got.items():
+            assert float((row - want[pos]).abs().max()) < TOL, (r, pos)
+        runner.close(rc)
+    assert runner.graph_replays >= 15
