@@ -95,11 +95,16 @@ __device__ __forceinline__ float ld_global_now(const float* p) {
 
 // FUSED: the modes ADD_NORM, SWIGLU, GEGLU and QKV_ROPE; the others' code is a kernel of its own.  In one kernel a plain product carried
 // the registers and the code of all (a decode step of 16 rows with ten plain products a layer: 783 -> 766 us; one row of Qwen3-0.6B,
-// whose output matrix alone is plain: 691 -> 685).
-template <int MB, int STAGES, bool FUSED>
+// whose output matrix alone is plain: 691 -> 685).  So does QKV_ROPE for an 8-bit cache, whose longer epilogue cost the bfloat16 one 1.3 us a
+// layer (8 rows of Qwen3-8B at 4,000 tokens: a step of 3.62 ms, 3.67 with both in one kernel).
+#define TC_KIND_PLAIN 0
+#define TC_KIND_FUSED 1
+#define TC_KIND_ROPE_F8 2
+template <int MB, int STAGES, int KIND>
 __global__ void __launch_bounds__(TC_THREADS) gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w,
                                                                   const __grid_constant__ CUtensorMap map_x,
                                                                   const TcParams p) {
+    constexpr bool FUSED = KIND != TC_KIND_PLAIN, F8 = KIND == TC_KIND_ROPE_F8;
     constexpr int A_BYTES = TC_BM * TC_BK * 2;           // 16 KB
     constexpr int B_BYTES = MB * TC_BK * 2;
     constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
@@ -215,7 +220,7 @@ __global__ void __launch_bounds__(TC_THREADS) gemm_tcgen05_kernel(const __grid_c
     const int m_valid = min(MB, p.M - m0);
     const int col = threadIdx.x;                                      // 128 threads = 128 columns of the tile
     const bool n_ok = n0 + col < p.N;
-    if (FUSED && p.mode == TC_MODE_QKV_ROPE && warp >= 2) {
+    if (FUSED && (F8 || p.mode == TC_MODE_QKV_ROPE) && warp >= 2) {
         // the step's own arrays (written by the host before the step): no need to wait for the kernel before this one
         for (int m = threadIdx.x - 64; m < m_valid; m += 64) {
             const int t = m0 + m, pos = p.positions[t];
@@ -272,7 +277,7 @@ __global__ void __launch_bounds__(TC_THREADS) gemm_tcgen05_kernel(const __grid_c
     constexpr int MAX_ROWS = MB <= 64 ? MB : 1;                       // the host refuses ADD_NORM for larger tiles
     float r_old[MAX_ROWS];
     float nw = 0.f;
-    if (FUSED && p.mode == TC_MODE_ADD_NORM) {
+    if (FUSED && !F8 && p.mode == TC_MODE_ADD_NORM) {
         if (n_ok) nw = ld_global_now(p.norm_w + n0 + col);
 #pragma unroll
         for (int i = 0; i < MAX_ROWS; ++i) {
@@ -282,7 +287,7 @@ __global__ void __launch_bounds__(TC_THREADS) gemm_tcgen05_kernel(const __grid_c
         }
     }
     // TC_MODE_QKV_ROPE: the tile is one head, a warp finishes a row; lane l has columns l, l + 32, l + 64, l + 96
-    const bool rope = FUSED && p.mode == TC_MODE_QKV_ROPE;
+    const bool rope = FUSED && (F8 || p.mode == TC_MODE_QKV_ROPE);
     const bool is_q = rope && (int)blockIdx.x < p.nq, is_k = rope && !is_q && (int)blockIdx.x < p.nq + p.nkv;
     const float* hw = is_q ? p.q_w : p.k_w;
     float wcol[4] = {1.f, 1.f, 1.f, 1.f}, freq[2] = {0.f, 0.f};
@@ -349,7 +354,7 @@ __global__ void __launch_bounds__(TC_THREADS) gemm_tcgen05_kernel(const __grid_c
                 else reinterpret_cast<bf16*>(p.out)[o] = __float2bfloat16_rn(val);
             }
         }
-    } else if (p.mode == TC_MODE_SWIGLU || p.mode == TC_MODE_GEGLU) {
+    } else if (!F8 && (p.mode == TC_MODE_SWIGLU || p.mode == TC_MODE_GEGLU)) {
         // the tile holds 64 gate columns, then the 64 up columns of the same outputs; half of the threads take every second row
         const int c = col & 63, oc = blockIdx.x * 64 + c;
 #pragma unroll 2
@@ -373,21 +378,21 @@ __global__ void __launch_bounds__(TC_THREADS) gemm_tcgen05_kernel(const __grid_c
             if (is_q || is_k) {
                 if (hw != nullptr) {
                     float ss = warp_sum((v[0] * v[0] + v[1] * v[1]) + (v[2] * v[2] + v[3] * v[3]));
-                    const bool large = p.eight_bit && ss == INFINITY;
+                    const bool large = F8 && ss == INFINITY;
                     if (large) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j) v[j] *= F8_NORM_DOWN;
                         ss = warp_sum((v[0] * v[0] + v[1] * v[1]) + (v[2] * v[2] + v[3] * v[3]));
                     }
                     const float mean = ss / (float)TC_BM + (large ? 0.f : p.rope_eps);
-                    const float f = p.eight_bit ? f8_inverse_root(mean) : rsqrtf(mean);
+                    const float f = F8 ? f8_inverse_root(mean) : rsqrtf(mean);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) v[j] = v[j] * f * wcol[j];
                 }
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     float sn, cs;
-                    if (p.eight_bit) {
+                    if (F8) {
                         const float2 turn = f8_turn(pos_s[m], freq[j]);
                         cs = turn.x;
                         sn = turn.y;
@@ -399,7 +404,7 @@ __global__ void __launch_bounds__(TC_THREADS) gemm_tcgen05_kernel(const __grid_c
                     v[j + 2] = b * cs + a * sn;
                 }
             }
-            if (!is_q && p.scales != nullptr) {              // a key or value row of an 8-bit cache
+            if (F8 && !is_q && p.scales != nullptr) {              // a key or value row of an 8-bit cache
                 const int64_t slot = (((int64_t)slot_s[2 * m] * p.nkv + kvh) << p.logP) + slot_s[2 * m + 1];
                 const uint32_t most = __reduce_max_sync(0xffffffffu, max(max(__float_as_uint(v[0]) & 0x7fffffffu, __float_as_uint(v[1]) & 0x7fffffffu),
                                                                          max(__float_as_uint(v[2]) & 0x7fffffffu, __float_as_uint(v[3]) & 0x7fffffffu)));
@@ -415,7 +420,7 @@ __global__ void __launch_bounds__(TC_THREADS) gemm_tcgen05_kernel(const __grid_c
             }
             bf16* dst = nullptr;
             if (is_q) dst = reinterpret_cast<bf16*>(p.out) + (int64_t)t * p.ldo + head * TC_BM;
-            else if (p.v_pages != nullptr)
+            else if (!F8 && p.v_pages != nullptr)
                 dst = (is_k ? p.k_pages : p.v_pages) + ((((int64_t)slot_s[2 * m] * p.nkv + kvh) << p.logP) + slot_s[2 * m + 1]) * TC_BM;
             if (dst != nullptr) {
 #pragma unroll
@@ -464,7 +469,7 @@ __global__ void __launch_bounds__(TC_THREADS) gemm_tcgen05_kernel(const __grid_c
 
 // ------------------------------------------------------------------ host side
 
-template <int MB, int STAGES, bool FUSED>
+template <int MB, int STAGES, int KIND>
 static int launch_tc_of(const CUtensorMap& mw, const CUtensorMap& mx, TcParams& p, int splits, cudaStream_t stream) {
     constexpr int STAGE_BYTES = TC_BM * TC_BK * 2 + MB * TC_BK * 2;
     const int steps = (p.kblocks + splits - 1) / splits;
@@ -478,7 +483,7 @@ static int launch_tc_of(const CUtensorMap& mw, const CUtensorMap& mx, TcParams& 
     const size_t smem = ring + rest, most = (size_t)STAGES * STAGE_BYTES + rest;
     static AcornPerDevice configured;
     if (!configured.seen()) {
-        cudaError_t e = cudaFuncSetAttribute(gemm_tcgen05_kernel<MB, STAGES, FUSED>,
+        cudaError_t e = cudaFuncSetAttribute(gemm_tcgen05_kernel<MB, STAGES, KIND>,
                                              cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
         if (e != cudaSuccess) return (int)e;
         configured.mark();
@@ -497,14 +502,17 @@ static int launch_tc_of(const CUtensorMap& mw, const CUtensorMap& mx, TcParams& 
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = acorn_pdl_enabled() ? 2 : 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_tcgen05_kernel<MB, STAGES, FUSED>, mw, mx, p);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_tcgen05_kernel<MB, STAGES, KIND>, mw, mx, p);
     return e != cudaSuccess ? (int)e : acorn_launch_status();
 }
 
 template <int MB, int STAGES>
 static int launch_tc(const CUtensorMap& mw, const CUtensorMap& mx, TcParams& p, int splits, cudaStream_t stream) {
     const bool plain = p.mode == TC_MODE_PLAIN || p.mode == TC_MODE_RELU2 || p.mode == TC_MODE_TANH || p.mode == TC_MODE_GELU_ROWS;
-    return plain ? launch_tc_of<MB, STAGES, false>(mw, mx, p, splits, stream) : launch_tc_of<MB, STAGES, true>(mw, mx, p, splits, stream);
+    if (plain) return launch_tc_of<MB, STAGES, TC_KIND_PLAIN>(mw, mx, p, splits, stream);
+    if constexpr (MB <= 64)
+        if (p.eight_bit) return launch_tc_of<MB, STAGES, TC_KIND_ROPE_F8>(mw, mx, p, splits, stream);
+    return launch_tc_of<MB, STAGES, TC_KIND_FUSED>(mw, mx, p, splits, stream);
 }
 
 // What the kernel takes: bf16 operands with K contiguous, K and both row strides multiples of 8
