@@ -82,7 +82,7 @@ template <int D, int NH> struct DecodeF8 {
     static constexpr int SCALES = BARS + 2 * STAGES * 8;
     static constexpr int RECV = SCALES + STAGES * SCALE_BYTES;        // received rows of a cluster, or the sizes of the tiles
     static constexpr int SHARES = (DF8_SHARE_TILES + 4) * 4 + DF8_SHARE_TILES * 16;       // chunks before a tile; row, first token, tokens, position
-    static_assert(RECV % 16 == 0 && MERGE % 16 == 0, "float4 and int4 accesses");
+    static_assert(RECV % 16 == 0 && MERGE % 16 == 0 && RECV_ROW % 4 == 0, "float4 and int4 accesses");
     // byte offset of the 16-byte piece `seg` of row `row` of a stage (boxes of 2^log_box keys, then as many values), as the
     // TMA's swizzle places it
     static __device__ __forceinline__ uint32_t at(int row, int seg) {
@@ -120,6 +120,15 @@ __device__ __forceinline__ float column_sum(float v) {
     v += __shfl_xor_sync(0xffffffffu, v, 4);
     v += __shfl_xor_sync(0xffffffffu, v, 8);
     return v + __shfl_xor_sync(0xffffffffu, v, 16);
+}
+
+// Two or four neighbouring floats, moved together.
+template <int E> struct alignas(4 * E) F8Floats { float v[E]; };
+template <int E> __device__ __forceinline__ void st_cluster(uint32_t addr, const F8Floats<E>& x) {
+    if constexpr (E == 4)
+        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" :: "r"(addr), "f"(x.v[0]), "f"(x.v[1]), "f"(x.v[2]), "f"(x.v[3]) : "memory");
+    else
+        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" :: "r"(addr), "f"(x.v[0]), "f"(x.v[1]) : "memory");
 }
 
 // What a CTA needs to know of a tile.
@@ -548,32 +557,32 @@ __global__ void __launch_bounds__(DF8_THREADS, NH == 1 || D == 64 ? 3 : 2) atten
                 mstar = fmaxf(mstar, sm_m[w * ROWS + m]);
                 tstar = fmaxf(tstar, sm_t[w * ROWS + m]);
             }
-            float sum = sink == -INFINITY ? 0.f : exp2f(sink - tstar), mean[E] = {};
+            float sum = sink == -INFINITY ? 0.f : exp2f(sink - tstar);
+            F8Floats<E> mean = {};
 #pragma unroll
             for (int w = 0; w < DF8_WARPS; ++w) {                 // a warp without keys has a sum and an output of 0
                 sum += exp2f(sm_t[w * ROWS + m] - tstar) * sm_l[w * ROWS + m];
                 const float f = exp2f(sm_m[w * ROWS + m] - mstar);
+                const F8Floats<E> part = reinterpret_cast<const F8Floats<E>*>(sm_o + (w * ROWS + m) * D)[lane];
 #pragma unroll
-                for (int e = 0; e < E; ++e) mean[e] += f * sm_o[(w * ROWS + m) * D + E * lane + e];
+                for (int e = 0; e < E; ++e) mean.v[e] += f * part.v[e];
             }
             const bool empty = sum == 0.f;                        // no key of this part is seen by the query
             const float back = exp2f(0.5f * (mstar - tstar));     // in two steps: 2^(m - r) alone may not be a float
 #pragma unroll
-            for (int e = 0; e < E; ++e) mean[e] = mean[e] / sum * back * back;
+            for (int e = 0; e < E; ++e) mean.v[e] = empty && !whole_pair ? 0.f : mean.v[e] / sum * back * back;
             if (whole_pair) {
                 __nv_bfloat162* dst = reinterpret_cast<__nv_bfloat162*>(p.out + ((int64_t)(tok0 + m / rep) * p.nq + head) * D + E * lane);
 #pragma unroll
-                for (int e = 0; e < E; e += 2) dst[e / 2] = __floats2bfloat162_rn(mean[e], mean[e + 1]);
+                for (int e = 0; e < E; e += 2) dst[e / 2] = __floats2bfloat162_rn(mean.v[e], mean.v[e + 1]);
             } else if (cluster) {
                 // to the CTA that finishes this row; a split without keys sends a log-sum of -inf
                 const uint32_t dst = cluster_map(tc_smem(recv + (split * slots + m / csize) * L::RECV_ROW), m % csize);
-#pragma unroll
-                for (int e = 0; e < E; ++e) st_cluster_f32(dst + 4 * (E * lane + e), empty ? 0.f : mean[e]);
+                st_cluster(dst + 4 * E * lane, mean);
                 if (lane == 0) st_cluster_f32(dst + 4 * D, empty ? -INFINITY : tstar + log2f(sum));
             } else {
                 const int64_t at = ((int64_t)blockIdx.x * 2 + (first ? 0 : 1)) * ROWS + m;
-#pragma unroll
-                for (int e = 0; e < E; ++e) dp.part_o[at * D + E * lane + e] = empty ? 0.f : mean[e];
+                reinterpret_cast<F8Floats<E>*>(dp.part_o + at * D)[lane] = mean;
                 if (lane == 0) dp.part_lse[at] = empty ? -INFINITY : tstar + log2f(sum);
             }
         }
