@@ -29,9 +29,11 @@
 //                  in order, so that a CTA walks from pair to pair: nobody waits for the longest row or for a last wave of few CTAs, and
 //                  the codes of the next pair are on their way while the warps finish one (a CTA's start and end cost some 5
 //                  us).  A pair that several CTAs had parts of is joined by a second, small kernel (some 4 us).  64 rows of 4,096
-//                  keys of 8 kv heads of 128: 124 us whole, 114 in 3 splits, 99 in shares, 545 MB at 5.5 TB/s.
+//                  keys of 8 kv heads of 128: 122 us whole, 111 in 3 splits, 97 in shares, 545 MB at 5.6 TB/s.
 // What bounds it: memory where there is enough of it (that case's main kernel moves its bytes at 0.85 of the copy rate), else
-// a warp's chain of some 290 instructions a chunk, 0.6 us (0.8 with the copies of pages of 16), and the start and the end.
+// a warp's chain of some 300 instructions a chunk, 0.6 us (0.8 with the copies of pages of 16), and the start and the end.  The
+// denominator's own reference costs up to 2.5 % at eight query rows and 1.5 to 6 at sixteen; warps that take whole rows of the join, rather
+// than threads its entries, and move them as vectors, brought up to 7 % (8 rows of 4,000 keys 17.5, 17.8 with the reference, 16.6).
 // Tried and taken back: the next chunk's scores formed among this one's weights (44 bytes spilled; 10 to 15 % slower at head size
 // 128), four CTAs an SM at 96 registers (20 % slower a chunk), more than 16 splits through scratch (59 us for one row of 131,072
 // keys in 48, as the shares).
@@ -189,8 +191,8 @@ __device__ __forceinline__ bool compute_all(bool v) {
 }
 
 // CTAs an SM: three, but two where sixteen rows of 128 entries need more than 128 registers a thread.  (Sixteen rows of 64, three
-// against two: 24 rows of 3 new tokens over a window of 1,024 19.1 us against 20.7, 41 of 2 over up to 1,700 22.9 against 28.0, 64
-// over 4,096 at sixteen heads a group 62.8 against 68.1.)
+// against two, measured before the denominator had a reference of its own: 24 rows of 3 new tokens over a window of 1,024 19.1 us against
+// 20.7, 41 of 2 over up to 1,700 22.9 against 28.0, 64 over 4,096 at sixteen heads a group 62.8 against 68.1.)
 template <int D, int NH, bool SHARES>
 __global__ void __launch_bounds__(DF8_THREADS, NH == 1 || D == 64 ? 3 : 2) attention_decode_f8_kernel(const __grid_constant__ CUtensorMap map_k,
                                                                          const __grid_constant__ CUtensorMap map_v,

@@ -1137,12 +1137,17 @@ def prefill_f8_splits(ctas: int, blocks: int, num_sms: int = 148) -> int:
 @lru_cache(maxsize=4096)
 def decode_f8_splits(tiles: int, num_kv_heads: int, key_bound: int, head_dim: int, shares: int) -> int:
     """How ``attention_decode_f8`` cuts its work: into even shares (0) for ``shares`` CTAs, or into so many parts a (tile, kv
-    head).  By estimates in us, fitted to 1 to 128 rows of 8 kv heads with 300 to 131,072 keys, which they meet to some 20 %: a
-    CTA's start and end take 6, a chunk of 64 keys 0.8 in a CTA (its warps' latencies), all of them together 6.1 TB/s; clusters run in
-    one wave up to 0.9 of the CTAs that the device holds, of sixteen up to 0.57 (444 of them, 8 rows of 4,000 keys: 6 parts, 384 CTAs,
-    18.9, 7 parts 28.4; 4 rows of 300: 8 parts 7.4, 16 14.4); shares take 12
-    and 3 a pair that a CTA comes to (64 rows of 4,096 keys: 99, whole 124, in 3 parts 114; 41 of 600 to 1,700: 33, whole 30;
-    one of 131,072: 61, in 16 parts 105)."""
+    head).  By estimates in us, fitted to 1 to 128 rows of 8 kv heads of 128 with 300 to 131,072 keys and up to eight query rows a
+    tile: a CTA's start and end take 6, a chunk of 64 keys 0.8 in a CTA (its warps' latencies), all of them together 6.1 TB/s; clusters
+    run in one wave up to 0.9 of the CTAs that the device holds, of sixteen up to 0.57 (444 of them, 8 rows of 4,000 keys: 6 parts, 384
+    CTAs, 18.2, 7 parts 26.5; 4 rows of 300: 8 parts 6.5, 16 12.5); shares take 12
+    and 3 a pair that a CTA comes to (64 rows of 4,096 keys: 97, whole 122, in 3 parts 111; 41 of 600 to 1,700: 31, whole 30;
+    one of 131,072: 57, in 16 parts 105).
+
+    How the choice compares with the best of all, over 23 sizes from 1 to 128 rows of 300 to 32,000 keys each: at most 1 % above it where
+    it was fitted, at most 9 % at head size 64 with up to eight query rows.  With sixteen query rows, whose chunks are longer, 3 to 9 % on
+    average and up to 45 % (head size 64, 4 rows of 8,000: shares 23.7, in 16 parts 16.4; head size 128, 128 rows of 350 to 1,000:
+    shares 123, whole 86).  ``key_bound`` is by the table's width, which in the engine is a power of two of pages."""
     pairs, chunks = max(1, tiles * num_kv_heads), -(-key_bound // 64)
     at_once = shares or 444
     stream_us = pairs * chunks * (128 * head_dim + 128) / 6.1e6
@@ -1267,8 +1272,9 @@ def attention_prefill_f8(q: torch.Tensor, q_stride: int, k_pages: torch.Tensor, 
     head's).
 
     ``prompt_rows`` (int32 [n]) and ``prompt_keys``: the rows that have tiles, each once, and how many keys each of them holds
-    (given-back pages not counted; a bound will do), so that the scratch is for those.  Without them it is for the widest row of the
-    table, as often as there are rows or tiles, whichever are fewer."""
+    (given-back pages not counted; a bound will do, and in a captured call has to hold for every replay), so that the scratch is for
+    those.  A row that holds more than it was said to, or a tile's row that is not listed, is reported by ``raise_on_kernel_error``.
+    Without them the scratch is for the widest row of the table, as often as there are rows or tiles, whichever are fewer."""
     what = "attention_prefill_f8"
     P, out, stream = _check_f8_attention(what, q, q_stride, k_pages, v_pages, scales, block_table, page_base, row_start, row_pos, tiles,
                                          num_tokens, num_heads, num_kv_heads, head_dim, window, out, chunk, keep_first, sink32)
